@@ -343,6 +343,7 @@ def _plain_sample(s):
     return token, torch.log(kept.gather(1, token) / total)[:, 0].float()
 
 
+@torch.no_grad()
 def run(state):
     if own:
         return _run_own(state)
