@@ -629,6 +629,106 @@ int parrot_moe_ep_combine_peer_bf16(const parrot_moe_dims* dims, const parrot_ep
 int parrot_ep_read_status(const parrot_ep_dims* ep, const void* buffer, int* host_status4,
                           void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving: a paged key/value cache shared by many sequences, attention of a
+ * ragged batch over it, and drawing tokens.  The dense caches and
+ * parrot_decode_attention_bf16 above take one position for the whole batch;
+ * these take every sequence at its own length, one new token or many.  No
+ * reference counterpart (the reference caches one dense batch,
+ * parrot/model.py:748-925, and decodes greedily, :927-931).
+ *
+ * Calls keep no state and use no workspace: the same call may run on several
+ * streams or in several captured graphs at once, as long as no two write the
+ * same rows.  A page number outside [0, pages) among the pages a call reads
+ * or writes, a context longer than the table, or a position that does not
+ * exist is recorded in `status` (device int[4], may be NULL): such a key and
+ * value read as zeros, such a token is not written.
+ * ---------------------------------------------------------------------- */
+typedef struct parrot_paged_kv {
+  void* key;          /* [pages, n_kv_heads, page_size, head_dim] bf16 or e4m3 */
+  void* value;        /* the same, or NULL: the values are the keys (the latent cache
+                         of parrot/model.py:399-432, one head) */
+  void* key_scale;    /* e4m3: [pages, n_kv_heads, page_size] bytes; a row's values are
+                         its numbers times 2^(byte - 127).  bf16: NULL */
+  void* value_scale;
+  int pages, n_kv_heads, page_size, head_dim;  /* page_size 16, 32, 64, 128 or 256;
+                                                  head_dim 32, 64, 96 or 128 */
+  int e4m3;           /* 0: bf16 pools, 1: e4m3 pools with scales */
+} parrot_paged_kv;
+
+/* Rows [query_start[b], query_start[b + 1]) of the batch are the last tokens
+ * of sequence b, whose context holds context_len[b] tokens with them: row
+ * query_start[b] + i is at position context_len[b] - (rows of b) + i.
+ * Position p is row p % page_size of page page_table[b][p / page_size].  All
+ * three arrays are in device memory; query_start does not decrease.  Rows from
+ * query_start[batch] on belong to no sequence and nothing is written for them. */
+typedef struct parrot_paged_batch {
+  const int* page_table;    /* [batch, table_width] */
+  const int* query_start;   /* [batch + 1] (parrot_paged_gather_bf16: not read) */
+  const int* context_len;   /* [batch] */
+  int batch, table_width;
+  int tokens;               /* rows of the batch's arrays */
+} parrot_paged_batch;
+
+/* Writes the batch's new keys and values to the cache.  qkv: [tokens,
+ * qkv_row_stride] bf16, each row the q_heads query heads, the key heads and
+ * (unless kv->value is NULL) the value heads of one token, the packed
+ * projection of parrot_rope_inplace_bf16.  With cos_table / sin_table (fp32
+ * [rope_positions, head_dim / 2]) queries and keys are rotated at their
+ * position as in parrot/model.py:206-216, here in fp32 with one rounding at
+ * the end.  q_out: [tokens, q_heads, head_dim], the (rotated) queries; qkv is
+ * not written.  An e4m3 cache takes for each row the least power of two that
+ * brings its largest magnitude to 448 or below (exponents -110 .. 119) and
+ * rounds to nearest; infinities saturate, NaN stays NaN.  Two tokens that
+ * write one row of one page in the same call race. */
+int parrot_paged_append_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                             const void* qkv, long long qkv_row_stride, int q_heads, void* q_out,
+                             const float* cos_table, const float* sin_table, int rope_positions,
+                             int* status, void* stream);
+
+/* Reads the sequences back as dense bf16 [batch, n_kv_heads, max_len,
+ * head_dim] (the layout of the dense caches above), exactly; zeros from
+ * context_len[b] on.  value_out is NULL exactly when kv->value is. */
+int parrot_paged_gather_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                             void* key_out, void* value_out, int max_len, int* status,
+                             void* stream);
+
+/* Attention of every query over its sequence's cached keys (which hold the
+ * batch's own: append first):
+ *   out = sum_j softmax_j(scale q . k_j) v_j over the keys j that a token at
+ *   position p sees: j <= p and (window == 0 or p - j < window or j < sinks).
+ * window > 0 with sinks > 0 keeps the first `sinks` tokens visible behind the
+ * sliding window of parrot/model.py:264-301.  n_heads a multiple of
+ * kv->n_kv_heads; query head h reads head h / (n_heads / n_kv_heads).  q:
+ * [tokens, q_row_stride] bf16 with the heads side by side, out: [tokens,
+ * n_heads, head_dim] bf16.  A token that sees no key gets zeros.  What no
+ * token of the batch sees is not used: pages wholly outside the window and
+ * the sinks may be given away, and numbers in masked places may be anything,
+ * NaN and infinities included. */
+int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                                const void* q, long long q_row_stride, void* out, int n_heads,
+                                int window, int sinks, float scale, int* status, void* stream);
+
+/* Draws one token per row of logits [rows, row_stride] (bf16, or fp32 with
+ * logits_f32; vocab <= 2^19).  With w_i = exp((l_i - max l) / temperature):
+ * the top_k tokens of largest w (0, or vocab and above: all; the lower index
+ * first among equals), of those each whose predecessors' mass is below top_p
+ * of their mass (1: all), of those each with w_i >= min_p; the first always
+ * stays.  ids[r] is the first token by index whose cumulative mass over the
+ * kept set exceeds uniform[r] (in [0, 1)) times the set's mass, logprobs[r]
+ * (may be NULL) the logarithm of its share of it.  temperature 0: the largest
+ * logit (lowest index), log-probability 0; -inf and NaN logits are never
+ * drawn, and a row of nothing else gives id -1 and -inf.  temperature, top_k,
+ * top_p, min_p: [rows] in device memory, or NULL for the *_all value in every
+ * row.  Beside parrot_vocab_argmax_bf16 / parrot_argmax_rows_bf16, the greedy
+ * choice of parrot/model.py:927-931.  Masses are summed exactly (fixed
+ * point), so a draw depends on nothing but its arguments. */
+int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int logits_f32,
+                       long long row_stride, int rows, int vocab, const float* uniform,
+                       const float* temperature, float temperature_all, const int* top_k,
+                       int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                       float min_p_all, void* stream);
+
 /* ---- self-test --------------------------------------------------------------
  * The failure path of the kernels' bounded mbarrier waits, without a fault: a
  * one-warp kernel waits on an mbarrier nobody arrives at through the same wait

@@ -1695,6 +1695,188 @@ int parrot_moe_read_status(const void* workspace, const parrot_moe_dims* dims, i
   return PARROT_OK;
 }
 
+}  // extern "C"
+
+// ---- serving: paged cache, attention over it, sampling ----------------------
+namespace {
+
+int paged_kv(const parrot_paged_kv* kv, parrot::PagedKV* out) {
+  if (kv == nullptr) return fail(PARROT_EINVAL, "paged: kv is NULL%s");
+  if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 &&
+      kv->page_size != 128 && kv->page_size != 256)
+    return fail(PARROT_EINVAL, "paged: page_size must be 16, 32, 64, 128 or 256%s");
+  if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 96 && kv->head_dim != 128)
+    return fail(PARROT_EUNSUPPORTED, "paged: head_dim must be 32, 64, 96 or 128%s");
+  if (kv->pages < 0 || kv->n_kv_heads <= 0 || kv->n_kv_heads > 1024)
+    return fail(PARROT_EINVAL, "paged: pages >= 0 and 1 <= n_kv_heads <= 1024 required%s");
+  // a row index of a pool, and the tile rows of one head, fit 31 bits
+  if ((long long)kv->pages * kv->n_kv_heads * kv->page_size > 0x7fffffffll)
+    return fail(PARROT_EINVAL, "paged: pools of more than 2^31 rows%s");
+  if (kv->pages > 0 && (kv->key == nullptr || !aligned16(kv->key) || !aligned16(kv->value)))
+    return fail(PARROT_EINVAL, "paged: the pools must be given and 16-byte aligned%s");
+  if (kv->e4m3 != 0 && kv->e4m3 != 1) return fail(PARROT_EINVAL, "paged: e4m3 must be 0 or 1%s");
+  if (kv->pages > 0 &&
+      ((kv->key_scale != nullptr) != (kv->e4m3 == 1) ||
+       (kv->value_scale != nullptr) != (kv->e4m3 == 1 && kv->value != nullptr)))
+    return fail(PARROT_EINVAL, "paged: e4m3 pools need their scales, bf16 pools have none%s");
+  out->key = kv->key;
+  out->value = kv->value;
+  out->key_scale = static_cast<uint8_t*>(kv->key_scale);
+  out->value_scale = static_cast<uint8_t*>(kv->value_scale);
+  out->pages = kv->pages;
+  out->kv_heads = kv->n_kv_heads;
+  out->head_dim = kv->head_dim;
+  out->page_shift = __builtin_ctz(kv->page_size);
+  out->page_mask = kv->page_size - 1;
+  return PARROT_OK;
+}
+
+int paged_batch(const parrot_paged_batch* b, const parrot_paged_kv* kv, bool ragged,
+                parrot::PagedBatch* out) {
+  if (b == nullptr) return fail(PARROT_EINVAL, "paged: batch is NULL%s");
+  if (b->batch < 0 || b->batch > 65535 || b->table_width < 0 || b->tokens < 0)
+    return fail(PARROT_EINVAL, "paged: 0 <= batch <= 65535, table_width and tokens >= 0%s");
+  if ((long long)b->table_width * kv->page_size > 0x7fffffffll - 512)
+    return fail(PARROT_EINVAL, "paged: a context of more than 2^31 positions%s");
+  if (b->batch > 0 && (b->context_len == nullptr || (ragged && b->query_start == nullptr) ||
+                       (b->table_width > 0 && b->page_table == nullptr)))
+    return fail(PARROT_EINVAL, "paged: null page_table, query_start or context_len%s");
+  out->page_table = b->page_table;
+  out->query_start = b->query_start;
+  out->context_len = b->context_len;
+  out->batch = b->batch;
+  out->table_width = b->table_width;
+  out->tokens = b->tokens;
+  return PARROT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int parrot_paged_append_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                             const void* qkv, long long qkv_row_stride, int q_heads, void* q_out,
+                             const float* cos_table, const float* sin_table, int rope_positions,
+                             int* status, void* stream) {
+  parrot::PagedAppendArgs a{};
+  int rc = paged_kv(kv, &a.kv);
+  if (rc || (rc = paged_batch(batch, kv, true, &a.batch))) return rc;
+  if (q_heads < 0 || q_heads > 4096)
+    return fail(PARROT_EINVAL, "paged_append: 0 <= q_heads <= 4096 required%s");
+  const long long width =
+      (long long)(q_heads + kv->n_kv_heads * (kv->value != nullptr ? 2 : 1)) * kv->head_dim;
+  if (qkv_row_stride < width || qkv_row_stride % 8)
+    return fail(PARROT_EINVAL, "paged_append: qkv rows must hold every head, stride %% 8 == 0%s");
+  if ((cos_table == nullptr) != (sin_table == nullptr) || (cos_table != nullptr && rope_positions <= 0))
+    return fail(PARROT_EINVAL, "paged_append: cos and sin tables go together%s");
+  if (a.batch.tokens == 0 || a.batch.batch == 0) return PARROT_OK;
+  if (qkv == nullptr || !aligned16(qkv) || (q_heads > 0) != (q_out != nullptr) ||
+      !aligned16(q_out) || !aligned16(cos_table) || !aligned16(sin_table))
+    return fail(PARROT_EINVAL, "paged_append: null or misaligned pointer (q_out with q_heads)%s");
+  a.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  a.qkv_row = qkv_row_stride;
+  a.q_out = static_cast<__nv_bfloat16*>(q_out);
+  a.q_heads = q_heads;
+  a.cos_t = cos_table;
+  a.sin_t = sin_table;
+  a.rope_positions = rope_positions;
+  a.status = status;
+  rc = parrot::launch_paged_append(a, static_cast<cudaStream_t>(stream));
+  if (rc == -1) return fail(PARROT_EINVAL, "paged_append: too many rows for one launch%s");
+  if (rc) return fail(PARROT_ECUDA, "paged_append: launch failed%s");
+  return check_launch("paged_append_kernel");
+}
+
+int parrot_paged_gather_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                             void* key_out, void* value_out, int max_len, int* status,
+                             void* stream) {
+  parrot::PagedGatherArgs a{};
+  int rc = paged_kv(kv, &a.kv);
+  if (rc || (rc = paged_batch(batch, kv, false, &a.batch))) return rc;
+  if (max_len < 0) return fail(PARROT_EINVAL, "paged_gather: max_len >= 0 required%s");
+  if (max_len == 0 || a.batch.batch == 0) return PARROT_OK;
+  if (key_out == nullptr || (value_out != nullptr) != (kv->value != nullptr) ||
+      !aligned16(key_out) || !aligned16(value_out))
+    return fail(PARROT_EINVAL, "paged_gather: null or misaligned output (value_out with value)%s");
+  a.key_out = static_cast<__nv_bfloat16*>(key_out);
+  a.value_out = static_cast<__nv_bfloat16*>(value_out);
+  a.max_len = max_len;
+  a.status = status;
+  if (parrot::launch_paged_gather(a, static_cast<cudaStream_t>(stream)))
+    return fail(PARROT_ECUDA, "paged_gather: launch failed%s");
+  return check_launch("paged_gather_kernel");
+}
+
+int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                                const void* q, long long q_row_stride, void* out, int n_heads,
+                                int window, int sinks, float scale, int* status, void* stream) {
+  parrot::PagedAttnArgs a{};
+  int rc = paged_kv(kv, &a.kv);
+  if (rc || (rc = paged_batch(batch, kv, true, &a.batch))) return rc;
+  if (n_heads <= 0 || n_heads > 4096 || n_heads % kv->n_kv_heads)
+    return fail(PARROT_EINVAL, "paged_attention: n_heads must be a multiple of n_kv_heads, <= 4096%s");
+  if (window < 0 || sinks < 0)
+    return fail(PARROT_EINVAL, "paged_attention: window and sinks must be >= 0%s");
+  if (!(scale > 0.f) || scale > 1e30f)
+    return fail(PARROT_EINVAL, "paged_attention: scale must be positive and finite%s");
+  if (q_row_stride < (long long)n_heads * kv->head_dim || q_row_stride % 8)
+    return fail(PARROT_EINVAL, "paged_attention: q rows must hold every head, stride %% 8 == 0%s");
+  if ((long long)a.batch.tokens * n_heads > 0x7fffffffll)
+    return fail(PARROT_EINVAL, "paged_attention: tokens * n_heads must fit 31 bits%s");
+  if (a.batch.tokens == 0 || a.batch.batch == 0) return PARROT_OK;
+  if (q == nullptr || out == nullptr || !aligned16(q) || !aligned16(out))
+    return fail(PARROT_EINVAL, "paged_attention: null or misaligned pointer%s");
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_row = q_row_stride;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.heads = n_heads;
+  a.window = window;
+  a.sinks = window > 0 ? sinks : 0;
+  a.scale = scale;
+  a.status = status;
+  rc = parrot::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  if (rc) return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
+  return check_launch("paged_attn_kernel");
+}
+
+int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int logits_f32,
+                       long long row_stride, int rows, int vocab, const float* uniform,
+                       const float* temperature, float temperature_all, const int* top_k,
+                       int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                       float min_p_all, void* stream) {
+  if (rows < 0 || vocab <= 0 || vocab > parrot::kSampleMaxVocab || row_stride < vocab)
+    return fail(PARROT_EINVAL, "sample: rows >= 0, 1 <= vocab <= 2^19 and row_stride >= vocab required%s");
+  if ((temperature == nullptr && !(temperature_all >= 0.f)) ||
+      (top_p == nullptr && !(top_p_all >= 0.f)) ||
+      (min_p == nullptr && !(min_p_all >= 0.f && min_p_all <= 1.f)) ||
+      (top_k == nullptr && top_k_all < 0))
+    return fail(PARROT_EINVAL, "sample: temperature, top_k, top_p >= 0 and 0 <= min_p <= 1 required%s");
+  if (rows == 0) return PARROT_OK;
+  if (ids == nullptr || logits == nullptr || uniform == nullptr ||
+      (reinterpret_cast<uintptr_t>(logits) & (logits_f32 ? 3u : 1u)))
+    return fail(PARROT_EINVAL, "sample: null or misaligned pointer%s");
+  parrot::SampleArgs a{};
+  a.logits = logits;
+  a.logits_f32 = logits_f32;
+  a.row_stride = row_stride;
+  a.uniform = uniform;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.temperature_all = temperature_all;
+  a.top_k_all = top_k_all;
+  a.top_p_all = top_p_all;
+  a.min_p_all = min_p_all;
+  a.ids = ids;
+  a.logprobs = logprobs;
+  a.rows = rows;
+  a.vocab = vocab;
+  if (parrot::launch_sample(a, static_cast<cudaStream_t>(stream)))
+    return fail(PARROT_ECUDA, "sample: launch failed%s");
+  return check_launch("sample_kernel");
+}
+
 int parrot_selftest_wait_timeout(unsigned long long limit_ns, int* device_out8, void* stream) {
   if (limit_ns < 1000 || limit_ns > 1000000000ull)
     return fail(PARROT_EINVAL, "selftest_wait_timeout: 1 us <= limit_ns <= 1 s required%s");

@@ -332,6 +332,76 @@ struct LinearSmallArgs {
 };
 int launch_linear_small(const LinearSmallArgs& args, cudaStream_t stream);
 
+// The paged key/value cache (paged.cu, paged_attn.cu).
+struct PagedKV {
+  void* key;            // [pages, kv_heads, page size, head_dim] bf16 or e4m3
+  void* value;          // the same, or null: the values are the keys
+  uint8_t* key_scale;   // [pages, kv_heads, page size] exponent + 127 (e4m3), or null (bf16)
+  uint8_t* value_scale;
+  int pages, kv_heads, head_dim;
+  int page_shift, page_mask;  // page size = 1 << page_shift
+};
+// A ragged batch: rows [query_start[b], query_start[b + 1]) are the last
+// tokens of sequence b's context.
+struct PagedBatch {
+  const int* page_table;   // [batch, table_width]
+  const int* query_start;  // [batch + 1], or null (gather)
+  const int* context_len;  // [batch], new tokens included
+  int batch, table_width, tokens;
+};
+struct PagedAppendArgs {
+  PagedKV kv;
+  PagedBatch batch;
+  const __nv_bfloat16* qkv;  // [tokens, (q_heads + kv_heads (x 2)) * head_dim]
+  long long qkv_row;         // elements between rows
+  __nv_bfloat16* q_out;      // [tokens, q_heads, head_dim], or null (q_heads 0)
+  int q_heads;
+  const float* cos_t;        // [rope_positions, head_dim / 2] fp32, or null: no rotation
+  const float* sin_t;
+  int rope_positions;
+  int* status;
+};
+struct PagedGatherArgs {
+  PagedKV kv;
+  PagedBatch batch;
+  __nv_bfloat16* key_out;    // [batch, kv_heads, max_len, head_dim]
+  __nv_bfloat16* value_out;
+  int max_len;
+  int* status;
+};
+struct PagedAttnArgs {
+  PagedKV kv;
+  PagedBatch batch;
+  const __nv_bfloat16* q;    // [tokens, heads, head_dim]
+  long long q_row;           // elements between tokens
+  __nv_bfloat16* out;        // [tokens, heads, head_dim]
+  int heads, window, sinks;
+  float scale;
+  int* status;
+};
+int launch_paged_append(const PagedAppendArgs& args, cudaStream_t stream);
+int launch_paged_gather(const PagedGatherArgs& args, cudaStream_t stream);
+int launch_paged_attention(const PagedAttnArgs& args, cudaStream_t stream);
+
+// Drawing tokens (sample.cu).  A null array: the *_all value for every row.
+struct SampleArgs {
+  const void* logits;        // [rows, vocab] bf16, or fp32 when logits_f32
+  int logits_f32;
+  long long row_stride;      // elements between rows
+  const float* uniform;      // [rows]
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  long long* ids;            // [rows]
+  float* logprobs;           // [rows], or null
+  int rows, vocab;
+};
+constexpr int kSampleMaxVocab = 1 << 19;  // 2^19 masses of at most 2^44 fit 63 bits
+int launch_sample(const SampleArgs& args, cudaStream_t stream);
+
 int launch_rmsnorm(__nv_bfloat16* out, const __nv_bfloat16* x, const __nv_bfloat16* w,
                    int rows, int dim, float eps, cudaStream_t stream);
 int launch_depthmix(const DepthMixArgs& args, cudaStream_t stream);

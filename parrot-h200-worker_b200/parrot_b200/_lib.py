@@ -67,6 +67,17 @@ class EpPeers(ctypes.Structure):
     _fields_ = [("buffers", c_void_p * EP_MAX_RANKS)]
 
 
+class PagedKVStruct(ctypes.Structure):
+    _fields_ = [("key", c_void_p), ("value", c_void_p), ("key_scale", c_void_p),
+                ("value_scale", c_void_p), ("pages", c_int), ("n_kv_heads", c_int),
+                ("page_size", c_int), ("head_dim", c_int), ("e4m3", c_int)]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    _fields_ = [("page_table", c_void_p), ("query_start", c_void_p), ("context_len", c_void_p),
+                ("batch", c_int), ("table_width", c_int), ("tokens", c_int)]
+
+
 _SIGNATURES = {
     "parrot_b200_version": (c_int, []),
     "parrot_b200_last_error": (ctypes.c_char_p, []),
@@ -168,6 +179,17 @@ _SIGNATURES = {
                                                 c_void_p, c_size_t, c_void_p, c_void_p,
                                                 c_void_p]),
     "parrot_ep_read_status": (c_int, [POINTER(EpDims), c_void_p, POINTER(c_int), c_void_p]),
+    "parrot_paged_append_bf16": (c_int, [POINTER(PagedKVStruct), POINTER(PagedBatchStruct),
+                                         c_void_p, ctypes.c_longlong, c_int, c_void_p, c_void_p,
+                                         c_void_p, c_int, c_void_p, c_void_p]),
+    "parrot_paged_gather_bf16": (c_int, [POINTER(PagedKVStruct), POINTER(PagedBatchStruct),
+                                         c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "parrot_paged_attention_bf16": (c_int, [POINTER(PagedKVStruct), POINTER(PagedBatchStruct),
+                                            c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int,
+                                            c_int, c_float, c_void_p, c_void_p]),
+    "parrot_sample_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int, ctypes.c_longlong, c_int,
+                                   c_int, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p,
+                                   c_float, c_void_p, c_float, c_void_p]),
     "parrot_selftest_wait_timeout": (c_int, [ctypes.c_ulonglong, c_void_p, c_void_p]),
 }
 

@@ -720,3 +720,286 @@ def read_status(flat_tokens: int, cfg, device: torch.device) -> list[int]:
     _lib.check(_lib.load().parrot_moe_read_status(_p(ws), ctypes.byref(dims), buf, _stream()),
                "parrot_moe_read_status")
     return list(buf)
+
+
+# ---------------------------------------------------------------------------
+# Serving: the paged cache, attention over it, sampling (no reference
+# counterpart: the reference keeps one dense cache per batch and decodes
+# greedily, model.py:748-931)
+# ---------------------------------------------------------------------------
+PAGE_SIZES = (16, 32, 64, 128, 256)
+PAGED_HEAD_DIMS = (32, 64, 96, 128)
+
+
+class PagedKV:
+    """The pools of one layer's paged cache.
+
+    ``key`` [pages, kv heads, page size, head_dim] bf16 or ``float8_e4m3fn``;
+    ``value`` the same, or None when the values are the keys (a latent cache).
+    An 8-bit pool comes with ``key_scale`` / ``value_scale`` [pages, kv heads,
+    page size] uint8: a row's values are its numbers times 2**(byte - 127).
+    Position ``p`` of sequence ``b`` is row ``p % page size`` of page
+    ``page_table[b, p // page size]``.
+    """
+
+    __slots__ = ("key", "value", "key_scale", "value_scale", "struct")
+
+    def __init__(self, key: Tensor, value: Tensor | None = None, key_scale: Tensor | None = None,
+                 value_scale: Tensor | None = None):
+        if key.ndim != 4 or key.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("key must be a bf16 or float8_e4m3fn pool [pages, kv heads, page size, head_dim]")
+        pages, heads, page, dim = key.shape
+        if page not in PAGE_SIZES or dim not in PAGED_HEAD_DIMS:
+            raise ValueError(f"page size must be one of {PAGE_SIZES} and head_dim one of "
+                             f"{PAGED_HEAD_DIMS}, got {page} and {dim}")
+        if value is not None and (value.shape != key.shape or value.dtype != key.dtype):
+            raise ValueError("value must match key in shape and type")
+        e4m3 = key.dtype == torch.float8_e4m3fn
+        for scale, pool in ((key_scale, key), (value_scale, value)):
+            if (scale is not None) != (e4m3 and pool is not None):
+                raise ValueError("8-bit pools need their scales, bf16 pools have none")
+            if scale is not None and (scale.shape != key.shape[:3] or scale.dtype != torch.uint8):
+                raise ValueError("scales must be uint8 [pages, kv heads, page size]")
+        for t in (key, value, key_scale, value_scale):
+            if t is not None and (t.device != key.device or not t.is_contiguous()):
+                raise ValueError("the pools and scales must be contiguous, on one device")
+        self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
+        self.struct = _lib.PagedKVStruct(
+            key.data_ptr(), None if value is None else value.data_ptr(),
+            None if key_scale is None else key_scale.data_ptr(),
+            None if value_scale is None else value_scale.data_ptr(), pages, heads, page, dim,
+            int(e4m3))
+
+    @classmethod
+    def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device,
+                 dtype: torch.dtype = torch.bfloat16, latent: bool = False) -> "PagedKV":
+        """Pools of ``pages`` pages (``latent``: no value pool)."""
+        shape = (pages, kv_heads, page_size, head_dim)
+
+        def pool():
+            return torch.empty(shape, device=device, dtype=dtype)
+
+        def scale():
+            return torch.empty(shape[:3], device=device, dtype=torch.uint8) \
+                if dtype == torch.float8_e4m3fn else None
+
+        if latent:
+            return cls(pool(), None, scale(), None)
+        return cls(pool(), pool(), scale(), scale())
+
+
+def _serving_device(dev: torch.device, what: str) -> torch.device:
+    """``dev``, checked to be an sm_100 GPU."""
+    if dev.type != "cuda":
+        raise RuntimeError(f"The B200 {what} backend requires CUDA tensors, got {dev}")
+    ok = _SUPPORTED.get(dev.index)
+    if ok is None:
+        ok = _SUPPORTED[dev.index] = bool(_lib.load().parrot_b200_device_supported(dev.index))
+    if not ok:
+        raise RuntimeError(f"The B200 {what} backend requires an sm_100 GPU (device {dev.index})")
+    return dev
+
+
+def _on_device(dev: torch.device, what: str, fn, args) -> None:
+    """``fn(*args, stream)`` with ``dev`` current, on its current stream."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _paged_batch(kv: PagedKV, page_table: Tensor, query_start: Tensor | None, context_len: Tensor,
+                 tokens: int):
+    """(struct, the tensors it points into)."""
+    dev = kv.key.device
+    if page_table.ndim != 2 or context_len.ndim != 1 or page_table.shape[0] != context_len.shape[0]:
+        raise ValueError("page_table must be [sequences, pages] and context_len [sequences]")
+    if query_start is not None and query_start.shape != (context_len.shape[0] + 1,):
+        raise ValueError("query_start must be [sequences + 1]")
+    for t in (page_table, context_len) if query_start is None else (page_table, context_len, query_start):
+        if t.dtype != torch.int32 or t.device != dev:
+            raise ValueError(f"page_table, query_start and context_len must be int32 on {dev}")
+    table, length = page_table.contiguous(), context_len.contiguous()
+    start = None if query_start is None else query_start.contiguous()
+    return _lib.PagedBatchStruct(table.data_ptr(), None if start is None else start.data_ptr(),
+                                 length.data_ptr(), table.shape[0], table.shape[1], tokens), \
+        (table, start, length)
+
+
+def _status_ptr(status: Tensor | None, dev) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() < 4 or status.device != dev or \
+            not status.is_contiguous():
+        raise ValueError(f"status must be a contiguous int32 tensor of 4 on {dev}")
+    return status.data_ptr()
+
+
+def _row_view(t: Tensor) -> Tensor:
+    """``t`` [rows, width] with unit column stride and 16-byte rows (a copy if need be)."""
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start: Tensor,
+                      context_len: Tensor, n_heads: int,
+                      rope: tuple[Tensor, Tensor] | None = None,
+                      status: Tensor | None = None) -> Tensor | None:
+    """Write a ragged batch's new keys and values to the cache; returns its queries.
+
+    ``qkv`` [tokens, width] bf16: each row the ``n_heads`` query heads, the key
+    heads and (unless the values are the keys) the value heads of one token.
+    Rows ``[query_start[b], query_start[b + 1])`` are the last tokens of
+    sequence ``b``, whose context holds ``context_len[b]`` tokens with them.
+    ``rope = (cos, sin)``, fp32 [positions, head_dim / 2]: queries and keys are
+    rotated at their positions (in fp32, rounded once).  Returns the queries
+    [tokens, n_heads, head_dim], or None for ``n_heads = 0``.  A token whose
+    page or position does not exist is not written; ``status`` (int32 [4])
+    records it.
+    """
+    dev = _serving_device(kv.key.device, "paged append")
+    _require_inference("paged append")
+    if qkv.ndim != 2 or qkv.dtype != torch.bfloat16 or qkv.device != dev:
+        raise RuntimeError(f"The B200 paged append takes bf16 rows [tokens, width] on {dev}")
+    s = kv.struct
+    width = (n_heads + s.n_kv_heads * (1 if kv.value is None else 2)) * s.head_dim
+    if qkv.shape[1] != width:
+        raise ValueError(f"qkv rows must be {width} wide, got {qkv.shape[1]}")
+    tokens = qkv.shape[0]
+    batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
+    qkv = _row_view(qkv)
+    cos = sin = None
+    if rope is not None:
+        cos, sin = rope
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous() or \
+                    t.ndim != 2 or t.shape[1] * 2 != s.head_dim or t.shape != cos.shape:
+                raise ValueError("rope tables must be contiguous fp32 [positions, head_dim / 2]")
+    out = torch.empty((tokens, n_heads, s.head_dim), device=dev, dtype=torch.bfloat16) \
+        if n_heads else None
+    _on_device(dev, "parrot_paged_append_bf16", _lib.load().parrot_paged_append_bf16, (
+        s, batch, qkv.data_ptr(), max(qkv.stride(0), width), n_heads,
+        None if out is None or tokens == 0 else out.data_ptr(),
+        None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
+        0 if cos is None else cos.shape[0], _status_ptr(status, dev)))
+    return out
+
+
+def b200_paged_gather(kv: PagedKV, page_table: Tensor, context_len: Tensor, max_len: int,
+                      out: tuple[Tensor, Tensor | None] | None = None,
+                      status: Tensor | None = None) -> tuple[Tensor, Tensor | None]:
+    """The sequences' cached keys and values as dense bf16 [sequences, kv heads,
+    ``max_len``, head_dim] (``LocalKVCache``'s layout; value None for a latent
+    cache), exactly; zeros past ``context_len``.  ``out``: tensors to fill."""
+    dev = _serving_device(kv.key.device, "paged gather")
+    _require_inference("paged gather")
+    batch, keep = _paged_batch(kv, page_table, None, context_len, 0)
+    s = kv.struct
+    shape = (batch.batch, s.n_kv_heads, max_len, s.head_dim)
+    if out is None:
+        key = torch.empty(shape, device=dev, dtype=torch.bfloat16)
+        value = None if kv.value is None else torch.empty_like(key)
+    else:
+        key, value = out
+        if (value is None) != (kv.value is None):
+            raise ValueError("out must hold a value tensor exactly when the cache does")
+        for t in (key, value):
+            if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or
+                                  t.device != dev or not t.is_contiguous() or t.data_ptr() % 16):
+                raise ValueError(f"out must be contiguous bf16 {shape} on {dev}")
+    if key.numel():
+        _on_device(dev, "parrot_paged_gather_bf16", _lib.load().parrot_paged_gather_bf16, (
+            s, batch, key.data_ptr(), None if value is None else value.data_ptr(), max_len,
+            _status_ptr(status, dev)))
+    return key, value
+
+
+def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start: Tensor,
+                         context_len: Tensor, *, window: int = 0, sinks: int = 0,
+                         scale: float | None = None, status: Tensor | None = None) -> Tensor:
+    """Causal attention of a ragged batch over the paged cache (append first).
+
+    ``q`` [tokens, heads, head_dim] bf16 (rows may be strided); token ``i`` of
+    sequence ``b`` sees the keys ``j <= p`` of its context with ``window == 0``,
+    ``p - j < window`` or ``j < sinks``.  Query head ``h`` reads key head
+    ``h // (heads / kv heads)``.  ``scale`` defaults to head_dim ** -0.5.  Returns
+    [tokens, heads, head_dim] bf16; zeros for a token that sees no key.
+    """
+    dev = _serving_device(kv.key.device, "paged attention")
+    _require_inference("paged attention")
+    s = kv.struct
+    if q.ndim != 3 or q.dtype != torch.bfloat16 or q.device != dev or q.shape[2] != s.head_dim:
+        raise RuntimeError(f"The B200 paged attention takes bf16 queries [tokens, heads, "
+                           f"{s.head_dim}] on {dev}")
+    tokens, heads, dim = q.shape
+    batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
+    if heads % s.n_kv_heads:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
+        q = q.contiguous()
+    q2 = _row_view(q.view(tokens, heads * dim) if q.is_contiguous() else
+                   q.as_strided((tokens, heads * dim), (q.stride(0), 1)))
+    out = torch.empty((tokens, heads, dim), device=dev, dtype=torch.bfloat16)
+    if tokens:
+        _on_device(dev, "parrot_paged_attention_bf16", _lib.load().parrot_paged_attention_bf16, (
+            s, batch, q2.data_ptr(), max(q2.stride(0), heads * dim), out.data_ptr(), heads,
+            window, sinks, dim ** -0.5 if scale is None else scale, _status_ptr(status, dev)))
+    return out
+
+
+def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1.0,
+                top_k: Tensor | int = 0, top_p: Tensor | float = 1.0,
+                min_p: Tensor | float = 0.0) -> tuple[Tensor, Tensor]:
+    """Draw a token per row: ``(ids [rows, 1] int64, log-probabilities [rows] fp32)``.
+
+    ``logits`` [rows, (1,) vocab] bf16 or fp32; ``uniform`` [rows] fp32 in
+    [0, 1), the rows' random numbers.  Each of ``temperature`` (0: the largest
+    logit, as ``b200_vocab_argmax``), ``top_k`` (0: all), ``top_p`` (1: all) and
+    ``min_p`` is a number for every row or a tensor [rows] (fp32; ``top_k``
+    int32).  The filters apply in that order; the token is the first by index
+    whose cumulative share of the kept set exceeds ``uniform``, and its
+    log-probability is the logarithm of its own share.  A row of only -inf or
+    NaN gives id -1 and -inf.
+    """
+    dev = _serving_device(logits.device, "sampling")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"The B200 sampling backend takes bf16 or fp32, got {logits.dtype}")
+    _require_inference("sampling")
+    if logits.ndim == 3 and logits.shape[1] == 1:
+        logits = logits[:, 0]
+    if logits.ndim != 2:
+        raise ValueError("logits must be [rows, vocab] or [rows, 1, vocab]")
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 or logits.stride(0) < vocab:
+        logits = logits.contiguous()
+
+    def param(v, name, dtype):
+        if not isinstance(v, Tensor):
+            return None, v
+        if v.shape != (rows,) or v.dtype != dtype or v.device != dev:
+            raise ValueError(f"{name} must be a number or {dtype} [{rows}] on {dev}")
+        return v.contiguous(), 0
+
+    uniform, _ = param(uniform, "uniform", torch.float32)
+    if uniform is None:
+        raise ValueError(f"uniform must be {torch.float32} [{rows}] on {dev}")
+    t, t_all = param(temperature, "temperature", torch.float32)
+    k, k_all = param(top_k, "top_k", torch.int32)
+    p, p_all = param(top_p, "top_p", torch.float32)
+    m, m_all = param(min_p, "min_p", torch.float32)
+    ids = torch.empty((rows, 1), device=dev, dtype=torch.int64)
+    logprobs = torch.empty(rows, device=dev, dtype=torch.float32)
+
+    def ptr(v):
+        return None if v is None else v.data_ptr()
+
+    _on_device(dev, "parrot_sample_rows", _lib.load().parrot_sample_rows, (
+        ids.data_ptr(), logprobs.data_ptr(), logits.data_ptr(),
+        int(logits.dtype == torch.float32), max(logits.stride(0), vocab), rows, vocab,
+        uniform.data_ptr(), ptr(t), t_all, ptr(k), k_all, ptr(p), p_all, ptr(m), m_all))
+    return ids, logprobs
