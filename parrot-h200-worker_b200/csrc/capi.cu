@@ -1834,7 +1834,7 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
   a.sinks = window > 0 ? sinks : 0;
   a.scale = scale;
   a.status = status;
-  rc = parrot::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  rc = parrot::launch_paged_attention(a, sm_count(), static_cast<cudaStream_t>(stream));
   if (rc) return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
   return check_launch("paged_attn_kernel");
 }

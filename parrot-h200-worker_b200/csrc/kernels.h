@@ -376,12 +376,13 @@ struct PagedAttnArgs {
   long long q_row;           // elements between tokens
   __nv_bfloat16* out;        // [tokens, heads, head_dim]
   int heads, window, sinks;
+  int cluster;               // CTAs that share a tile (set at launch)
   float scale;
   int* status;
 };
 int launch_paged_append(const PagedAppendArgs& args, cudaStream_t stream);
 int launch_paged_gather(const PagedGatherArgs& args, cudaStream_t stream);
-int launch_paged_attention(const PagedAttnArgs& args, cudaStream_t stream);
+int launch_paged_attention(const PagedAttnArgs& args, int sms, cudaStream_t stream);
 
 // Drawing tokens (sample.cu).  A null array: the *_all value for every row.
 struct SampleArgs {

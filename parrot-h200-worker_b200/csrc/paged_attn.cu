@@ -4,110 +4,556 @@
 // over the keys j that token i (at position p of its sequence) sees:
 //   j <= p, and without a window or p - j < window or j < sinks.
 // A token that sees no key gets zeros.
+//
+// The query heads of one key head and a run of tokens share their keys: a
+// tile is 16 consecutive (token, head) rows of one sequence, token major, so
+// each key is read once for all of them.
 #include "paged.cuh"
+#include <algorithm>
+
+#include "tc.cuh"
 
 namespace parrot {
 
 namespace {
-constexpr int kAttnThreads = 128;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One CTA per (token, query head); a thread scores one key per step, then the
-// CTA adds the step's weighted values, a column per thread.
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(kAttnThreads) paged_attn_kernel(PagedAttnArgs a) {
-  __shared__ float q_s[D], p_s[kAttnThreads], red_s[kAttnThreads / 32];
-  __shared__ long long row_s[kAttnThreads];
+// A tile: `rows_per` consecutive (token, head) rows of one sequence.
+struct Tile {
+  int b;           // sequence, -1: no such tile
+  int first;       // batch row of the sequence's first token
+  int n;           // its tokens in the batch
+  int row0;        // first (token, head) row of the tile
+};
+
+// The tile with this number, sequences in order, ceil(n_b * group / rows_per)
+// tiles each.  A whole warp calls; 32 sequences a step, their lengths loaded
+// side by side.
+__device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int rows_per, int tile) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < s.batch; b0 += 32) {
+    const int b = b0 + lane;
+    int2 r = make_int2(0, 0);
+    if (b < s.batch) r = batch_rows(s, b);
+    const int n = r.y - r.x;
+    const int mine = (int)(((long long)n * group + rows_per - 1) / rows_per);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + upto > tile);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      Tile t;
+      t.b = b0 + l;
+      t.first = __shfl_sync(0xffffffffu, r.x, l);
+      t.n = __shfl_sync(0xffffffffu, n, l);
+      t.row0 = (tile - base - __shfl_sync(0xffffffffu, upto - mine, l)) * rows_per;
+      return t;
+    }
+    base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Tile{-1, 0, 0, 0};
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) != 0x7f80u; }
+
+// ---------------------------------------------------------------------------
+// Few rows per sequence (decode): bound by reading the keys.
+//
+// A tile's visible keys are cut into 32-key chunks.  The chunks are dealt to
+// the warps of a cluster of CTAs; each warp keeps its own ring of chunks in
+// flight (16-byte asynchronous copies, no barrier between warps), multiplies
+// with m16n8k16 matrix instructions (the 16 rows of the tile; at 8 rows or fewer
+// half of the product is idle, which reading the keys hides) and carries its
+// own running maximum, sum and fp32 weighted values.  The warps' results are
+// merged in shared memory, the CTAs' over distributed shared memory, in a
+// fixed order: no workspace, no second launch, no atomics.
+// ---------------------------------------------------------------------------
+constexpr int kDecWarps = 4;
+constexpr int kDecKeys = 32;
+constexpr int kDecRows = 16;
+
+template <int D, bool E4M3, bool SEP>
+struct DecodeShape {
+  static constexpr int kStages = E4M3 ? 3 : 2;
+  // bf16 rows are padded by 16 bytes: an odd number of 16-byte units, so the
+  // eight rows of a matrix load fall in different banks
+  static constexpr int kRow = 2 * D + 16;
+  static constexpr int kTile = kDecKeys * kRow;
+  static constexpr int kRaw = kDecKeys * D;
+  static constexpr int kSide = E4M3 ? kRaw : kTile;
+  static constexpr int kStage = kSide * (SEP ? 2 : 1);
+  // e4m3: a bf16 tile that the chunk's keys, then its values, are expanded to
+  static constexpr int kWarp = kStage * kStages + (E4M3 ? kTile : 0);
+  static constexpr int kPart = kDecRows * D * 4 + 2 * kDecRows * 4;  // a CTA's result
+  static constexpr int kBytes = kWarp * kDecWarps + kPart;
+  static_assert(kWarp >= kPart, "a warp's ring holds its result");
+};
+
+template <int D, bool E4M3, bool SEP>
+__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnArgs a) {
+  using S = DecodeShape<D, E4M3, SEP>;
+  constexpr int KS = D / 16;  // k steps of q . k
+  constexpr int NT = D / 8;   // column tiles of the output
+  extern __shared__ __align__(128) unsigned char dec_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  const int kvh = blockIdx.y, group = a.heads / a.kv.kv_heads;
   griddep_wait();
   griddep_launch();
-  const int token = blockIdx.x, h = blockIdx.y, kvh = h / (a.heads / a.kv.kv_heads);
-  const int b = sequence_of(a.batch, token);
-  if (b < 0) return;
-  const int2 rows = batch_rows(a.batch, b);
-  const int n = context_of(a.batch, a.kv, b, a.status);
-  const int pos = n - (rows.y - token);
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int sinks = min(a.sinks, lo);  // keys [0, sinks) and [lo, pos]
-  const int seen = pos < 0 ? 0 : sinks + pos - lo + 1;
-  const int x = threadIdx.x;
-  if (x < D) q_s[x] = __bfloat162float(a.q[(long long)token * a.q_row + h * D + x]);
-  auto load8 = [&](const void* pool, const uint8_t* scale, long long r, int c, float* f) {
-    uint4 v;
-    if constexpr (E4M3) {
-      const uint2 w = reinterpret_cast<const uint2*>(pool)[r * (D / 8) + c];
-      const uint32_t s2 = scale_pair(scale[r]);
-      const uint2 l = e4m3x4_to_bf16(w.x, s2), u = e4m3x4_to_bf16(w.y, s2);
-      v = make_uint4(l.x, l.y, u.x, u.y);
-    } else {
-      v = reinterpret_cast<const uint4*>(pool)[r * (D / 8) + c];
-    }
-    bf16x8_to_float(v, f);
+  const Tile tile = find_tile(a.batch, group, kDecRows, blockIdx.x / ranks);
+  if (tile.b < 0) return;  // the whole cluster
+  const int n = context_of(a.batch, a.kv, tile.b, a.status);
+  const int rows = min(kDecRows, tile.n * group - tile.row0);
+  const int pos0 = n - tile.n;  // position of the sequence's first batch row
+  const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;
+
+  // the two (token, head) rows of this thread in the product's layout
+  int pos[2];
+  uint32_t qf[KS][4];
+  const __nv_bfloat16* qrow[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = tile.row0 + min(g + 8 * i, rows - 1);
+    pos[i] = pos0 + r / group;
+    qrow[i] = a.q + (long long)(tile.first + r / group) * a.q_row +
+              (long long)(kvh * group + r % group) * D;
+  }
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      qf[k][j] = *reinterpret_cast<const uint32_t*>(qrow[j & 1] + k * 16 + 2 * t + 8 * (j >> 1));
+
+  // chunks: those of the sinks that lie before the window's first, then the
+  // window's; key base of chunk c
+  const int lo = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+  const int c_lo = lo / kDecKeys;
+  const int sink_chunks = min((min(a.sinks, lo) + kDecKeys - 1) / kDecKeys, c_lo);
+  const int chunks = pmax < 0 ? 0 : sink_chunks + pmax / kDecKeys - c_lo + 1;
+  auto base_of = [&](int c) { return (c < sink_chunks ? c : c - sink_chunks + c_lo) * kDecKeys; };
+  const int workers = ranks * kDecWarps, me = rank * kDecWarps + warp;
+
+  unsigned char* ring = dec_smem + warp * S::kWarp;
+  const uint32_t ring_u = tc::smem_u32(ring);
+  const uint32_t wide_u = ring_u + S::kStage * S::kStages;
+  uint32_t sc[S::kStages];  // e4m3: this lane's key's two scale bytes, per stage
+#pragma unroll
+  for (int i = 0; i < S::kStages; ++i) sc[i] = 0;
+  // the page of this lane's key of a chunk, -1 where nobody of the tile sees it
+  auto page_for = [&](int c) {
+    if (c >= chunks) return -1;
+    const int j = base_of(c) + lane;
+    const bool seen = j <= pmax && (a.window == 0 || j > pmin - a.window || j < a.sinks);
+    return seen ? page_of(a.batch, a.kv, tile.b, j, a.status) : -1;
   };
-  const bool sep = a.kv.value != nullptr;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int k0 = 0; k0 < seen; k0 += kAttnThreads) {
-    __syncthreads();
-    const int i = k0 + x;
-    float s = -INFINITY;
-    if (i < seen) {
-      const int j = i < sinks ? i : lo + i - sinks;
-      const int page = page_of(a.batch, a.kv, b, j, a.status);
-      const long long r = page < 0 ? -1 : pool_row(a.kv, page, kvh, j);
-      row_s[x] = r;
-      float dot = 0.f;
-      if (r >= 0)
-        for (int c = 0; c < D / 8; ++c) {
-          float f[8];
-          load8(a.kv.key, a.kv.key_scale, r, c, f);
-          for (int e = 0; e < 8; ++e) dot = fmaf(q_s[c * 8 + e], f[e], dot);
-        }
-      s = dot * a.scale;
+  // start the copies of chunk c into a stage; keys nobody sees become zeros
+  auto fetch = [&](int c, int page, uint32_t stage, uint32_t& scales) {
+    if (c < chunks) {
+      const int j = base_of(c) + lane;
+      const int row = page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, j);
+      if constexpr (E4M3) {
+        scales = row < 0 ? 0u
+                         : (uint32_t)a.kv.key_scale[row] |
+                               (SEP ? (uint32_t)a.kv.value_scale[row] << 8 : 0u);
+      }
+      constexpr int VR = E4M3 ? D / 16 : D / 8;  // 16-byte vectors of a row
+#pragma unroll
+      for (int i = 0; i < VR; ++i) {
+        const int v = lane + 32 * i, r = v / VR, cv = v - r * VR;
+        const int rr = __shfl_sync(0xffffffffu, row, r);
+        const long long at = ((long long)max(rr, 0) * VR + cv) * 16;
+        const uint32_t dst = ring_u + stage * S::kStage + r * (E4M3 ? D : S::kRow) + cv * 16;
+        cp_async16_zfill(dst, static_cast<const char*>(a.kv.key) + at, rr >= 0);
+        if (SEP) cp_async16_zfill(dst + S::kSide, static_cast<const char*>(a.kv.value) + at, rr >= 0);
+      }
     }
-    float mx = warp_max(s);
-    if ((x & 31) == 0) red_s[x >> 5] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
-    const float mn = fmaxf(m, mx);
-    const float corr = __expf(m - mn);
-    const float p = i < seen ? __expf(s - mn) : 0.f;
-    p_s[x] = p;
-    const float ps = warp_sum(p);
-    __syncthreads();
-    if ((x & 31) == 0) red_s[x >> 5] = ps;
-    __syncthreads();
-    l = l * corr + red_s[0] + red_s[1] + red_s[2] + red_s[3];
-    m = mn;
-    acc *= corr;
-    if (x < D) {
-      const int here = min(kAttnThreads, seen - k0);
-      for (int j = 0; j < here; ++j) {
-        const long long r = row_s[j];
-        if (r < 0) continue;
-        float f[8];
-        load8(sep ? a.kv.value : a.kv.key, sep ? a.kv.value_scale : a.kv.key_scale, r, x >> 3, f);
-        acc = fmaf(p_s[j], f[x & 7], acc);
+    cp_async_commit();
+  };
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+  const float scale2 = a.scale * kLog2e;
+
+  int c = me;
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s)
+    fetch(c + s * workers, page_for(c + s * workers), s, sc[s]);
+  int next_page = page_for(c + (S::kStages - 1) * workers);
+  int it = 0;
+  for (; c < chunks; c += workers, ++it) {
+    const int slot = it % S::kStages, fill = (it + S::kStages - 1) % S::kStages;
+    uint32_t new_sc = 0;
+    fetch(c + (S::kStages - 1) * workers, next_page, fill, new_sc);
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int s = 0; s < S::kStages; ++s)
+        if (s == fill) sc[s] = new_sc;
+    }
+    next_page = page_for(c + S::kStages * workers);
+    cp_async_wait<S::kStages - 1>();
+    __syncwarp();
+    uint32_t k_u = ring_u + slot * S::kStage, v_u = SEP ? k_u + S::kSide : k_u;
+    uint32_t scales = 0;
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int s = 0; s < S::kStages; ++s)
+        if (s == slot) scales = sc[s];
+    }
+    // a side's 32 rows of e4m3 numbers to bf16 values
+    auto widen = [&](uint32_t raw, int shift) {
+      constexpr int VR = D / 16;
+#pragma unroll
+      for (int i = 0; i < VR; ++i) {
+        const int v = lane + 32 * i, r = v / VR, cv = v - r * VR;
+        const uint32_t s2 = scale_pair((__shfl_sync(0xffffffffu, scales, r) >> shift) & 0xff);
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(raw + v * 16));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 x = e4m3x4_to_bf16(w[2 * h], s2), y = e4m3x4_to_bf16(w[2 * h + 1], s2);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(wide_u + r * S::kRow +
+                                                                        cv * 32 + h * 16),
+                       "r"(x.x), "r"(x.y), "r"(y.x), "r"(y.y)
+                       : "memory");
+        }
+      }
+      __syncwarp();
+    };
+    if constexpr (E4M3) {
+      widen(k_u, 0);
+      k_u = wide_u;
+    }
+    // scores of the 16 rows and 32 keys
+    float s[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int k2 = 0; k2 < KS / 2; ++k2) {
+        uint32_t b[4];
+        ldmatrix_x4(b, k_u + (nt * 8 + (lane & 7)) * S::kRow + k2 * 64 + (lane >> 3) * 16);
+        mma_16816(s[nt], qf[2 * k2], b[0], b[1]);
+        mma_16816(s[nt], qf[2 * k2 + 1], b[2], b[3]);
+      }
+    const int base = base_of(c);
+    const bool whole = base + kDecKeys - 1 <= pmin &&
+                       (a.window == 0 || base > pmax - a.window || base + kDecKeys <= a.sinks);
+    auto sees = [&](int i, int j) {
+      return j <= pos[i] && (a.window == 0 || pos[i] - j < a.window || j < a.sinks);
+    };
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[nt][j] *= scale2;
+        if (!whole && !sees(j >> 1, base + nt * 8 + 2 * t + (j & 1))) s[nt][j] = -INFINITY;
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * i], s[nt][2 * i + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float corr = exp2_fast(m[i] - ref);
+      m[i] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = exp2_fast(s[nt][2 * i + e] - ref);
+          s[nt][2 * i + e] = p;
+          sum += p;
+        }
+      l[i] = fmaf(l[i], corr, sum);  // this thread's columns; the quad is summed at the end
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        o[nt][2 * i] *= corr;
+        o[nt][2 * i + 1] *= corr;
+      }
+    }
+    if constexpr (E4M3 && SEP) {
+      __syncwarp();  // the keys have been read
+      widen(v_u, 8);
+    }
+    if constexpr (E4M3) v_u = wide_u;
+    if (!whole && pmin != pmax) {
+      // A value that is not finite would reach, as 0 * NaN in the product, the
+      // rows that do not see its key.  Take such numbers out of the tile and add
+      // them to the rows that see them.
+      unsigned bad_row = 0;
+#pragma unroll 1
+      for (int i = 0; i < D / 2; ++i) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(v_u + lane * S::kRow + i * 4));
+        bad_row |= !finite_bf16(w) || !finite_bf16(w >> 16);
+      }
+      const unsigned bad = __ballot_sync(0xffffffffu, bad_row);
+      if (bad) {
+        for (unsigned left = bad; left; left &= left - 1) {
+          const int j = __ffs(left) - 1;  // key base + j: column tile j / 8, thread (j % 8) / 2
+          const int src = (lane & ~3) | ((j & 7) >> 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float p = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+              if (nt == j >> 3) p = j & 1 ? s[nt][2 * i + 1] : s[nt][2 * i];
+            p = __shfl_sync(0xffffffffu, p, src);
+            const bool vis = sees(i, base + j);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];"
+                           : "=r"(w)
+                           : "r"(v_u + j * S::kRow + (nt * 8 + 2 * t) * 2));
+              const float2 v = bf16x2_to_float2(w);
+              if (vis && !finite_bf16(w)) o[nt][2 * i] = fmaf(p, v.x, o[nt][2 * i]);
+              if (vis && !finite_bf16(w >> 16)) o[nt][2 * i + 1] = fmaf(p, v.y, o[nt][2 * i + 1]);
+            }
+          }
+        }
+        __syncwarp();
+        if (bad_row) {
+#pragma unroll 1
+          for (int i = 0; i < D / 2; ++i) {
+            const uint32_t at = v_u + lane * S::kRow + i * 4;
+            uint32_t w;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+            if (!finite_bf16(w)) w &= 0xffff0000u;
+            if (!finite_bf16(w >> 16)) w &= 0x0000ffffu;
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // weighted values: the probabilities rounded to bf16, as the matrix
+    // instructions take them (half a step of 2^-8 relative each, unbiased)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint32_t p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nt = 2 * kk + (j >> 1);
+        p[j] = tc::pack_bf16x2(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
+      }
+#pragma unroll
+      for (int n2 = 0; n2 < NT / 2; ++n2) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, v_u + (kk * 16 + (lane & 15)) * S::kRow + n2 * 32 + (lane >> 4) * 16);
+        mma_16816(o[2 * n2], p, b[0], b[1]);
+        mma_16816(o[2 * n2 + 1], p, b[2], b[3]);
+      }
+    }
+    __syncwarp();  // the stage may be filled again
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+
+  // ---- merge: warps of the CTA, then CTAs of the cluster -------------------
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+  }
+  float* mine = reinterpret_cast<float*>(ring);  // [rows][D], then m, l
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = g + 8 * i;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      *reinterpret_cast<float2*>(mine + r * D + nt * 8 + 2 * t) =
+          make_float2(o[nt][2 * i], o[nt][2 * i + 1]);
+    if (t == 0) {
+      mine[kDecRows * D + r] = m[i];
+      mine[kDecRows * D + kDecRows + r] = l[i];
+    }
+  }
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(dec_smem + S::kWarp * kDecWarps);
+  auto write = [&](int r, int col, float4 v, float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
+    const int row = tile.row0 + r;
+    uint2 w;
+    w.x = tc::pack_bf16x2(v.x * inv, v.y * inv);
+    w.y = tc::pack_bf16x2(v.z * inv, v.w * inv);
+    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + row / group) * a.heads +
+                                       kvh * group + row % group) * D + col) = w;
+  };
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kDecWarps) {
+    const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
+    float mx = -INFINITY, sum = 0.f;
+    const float* w0 = reinterpret_cast<const float*>(dec_smem);
+    constexpr int kStride = S::kWarp / 4;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, w0[w * kStride + kDecRows * D + r]);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float* p = w0 + w * kStride;
+      const float mw = p[kDecRows * D + r];
+      const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
+      sum = fmaf(f, p[kDecRows * D + kDecRows + r], sum);
+      const float4 x = *reinterpret_cast<const float4*>(p + r * D + col);
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+      v.z = fmaf(f, x.z, v.z);
+      v.w = fmaf(f, x.w, v.w);
+    }
+    if (ranks == 1) {
+      write(r, col, v, sum);
+    } else {
+      *reinterpret_cast<float4*>(part + r * D + col) = v;
+      if (col == 0) {
+        part[kDecRows * D + r] = mx;
+        part[kDecRows * D + kDecRows + r] = sum;
       }
     }
   }
-  if (x < D)
-    a.out[((long long)token * a.heads + h) * D + x] = __float2bfloat16_rn(seen > 0 ? acc / l : 0.f);
+  if (ranks == 1) return;
+  tc::cluster_sync();
+  for (int i = rank * 32 * kDecWarps + threadIdx.x; i < rows * (D / 4);
+       i += ranks * 32 * kDecWarps) {
+    const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
+    float mx = -INFINITY, sum = 0.f;
+    for (int k = 0; k < ranks; ++k)
+      mx = fmaxf(mx, ld_cluster_f1(tc::mapa_shared(part + kDecRows * D + r, k)));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < ranks; ++k) {
+      const float mk = ld_cluster_f1(tc::mapa_shared(part + kDecRows * D + r, k));
+      const float f = mk == -INFINITY ? 0.f : exp2_fast(mk - mx);
+      sum = fmaf(f, ld_cluster_f1(tc::mapa_shared(part + kDecRows * D + kDecRows + r, k)), sum);
+      const float4 x = ld_cluster_f4(tc::mapa_shared(part + r * D + col, k));
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+      v.z = fmaf(f, x.z, v.z);
+      v.w = fmaf(f, x.w, v.w);
+    }
+    write(r, col, v, sum);
+  }
+  tc::cluster_sync();  // nobody leaves while its result may be read
+}
+
+// CTAs per tile: as many as keep every warp two chunks or more of the longest
+// possible context, while the grid stays within about three CTAs per SM.
+int decode_ranks(const PagedAttnArgs& a, long long tiles, int sms) {
+  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
+  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
+  const long long chunks = (keys + kDecKeys - 1) / kDecKeys;
+  int ranks = 1;
+  while (ranks < 8 && chunks >= 4LL * ranks * kDecWarps && tiles * ranks * 2 <= 3LL * sms) ranks *= 2;
+  return ranks;
+}
+
+template <int D, bool E4M3, bool SEP>
+int launch_decode(PagedAttnArgs a, cudaStream_t stream, int sms) {
+  using S = DecodeShape<D, E4M3, SEP>;
+  auto k = paged_decode_kernel<D, E4M3, SEP>;
+  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
+  const long long tiles = std::min(n * ((group + kDecRows - 1) / kDecRows),
+                                   n * group / kDecRows + std::min<long long>(a.batch.batch, n));
+  a.cluster = decode_ranks(a, tiles * a.kv.kv_heads, sms);
+  if (tiles * a.cluster > 0x7fffffffll) return -1;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
+    return -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * a.cluster), a.kv.kv_heads);
+  cfg.blockDim = dim3(32 * kDecWarps);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)a.cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k, a) == cudaSuccess ? 0 : -2;
 }
 
 template <int D>
-static int launch_attn_d(const PagedAttnArgs& a, cudaStream_t stream) {
-  auto k = a.kv.key_scale != nullptr ? paged_attn_kernel<D, true> : paged_attn_kernel<D, false>;
-  return launch_pdl(k, dim3(a.batch.tokens, a.heads), dim3(kAttnThreads), 0, stream, a) ==
-                 cudaSuccess
-             ? 0
-             : -2;
+int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
+  const bool e = a.kv.key_scale != nullptr, sep = a.kv.value != nullptr;
+  if (e) return sep ? launch_decode<D, true, true>(a, stream, sms) : launch_decode<D, true, false>(a, stream, sms);
+  return sep ? launch_decode<D, false, true>(a, stream, sms) : launch_decode<D, false, false>(a, stream, sms);
 }
 
-int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t stream) {
+}  // namespace
+
+int launch_paged_attention(const PagedAttnArgs& a, int sms, cudaStream_t stream) {
   switch (a.kv.head_dim) {
-    case 32: return launch_attn_d<32>(a, stream);
-    case 64: return launch_attn_d<64>(a, stream);
-    case 96: return launch_attn_d<96>(a, stream);
-    case 128: return launch_attn_d<128>(a, stream);
+    case 32: return launch_decode_d<32>(a, stream, sms);
+    case 64: return launch_decode_d<64>(a, stream, sms);
+    case 96: return launch_decode_d<96>(a, stream, sms);
+    case 128: return launch_decode_d<128>(a, stream, sms);
   }
   return -1;
 }
