@@ -1872,7 +1872,7 @@ int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int 
   a.logprobs = logprobs;
   a.rows = rows;
   a.vocab = vocab;
-  if (parrot::launch_sample(a, static_cast<cudaStream_t>(stream)))
+  if (parrot::launch_sample(a, sm_count(), static_cast<cudaStream_t>(stream)))
     return fail(PARROT_ECUDA, "sample: launch failed%s");
   return check_launch("sample_kernel");
 }
