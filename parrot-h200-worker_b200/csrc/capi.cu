@@ -84,9 +84,9 @@ struct MapKeyHash {
 std::mutex g_map_mutex;
 std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_maps;
 
-// Row-major bf16 [rows, cols] matrix, box = 64 columns x box_rows rows, 128-B swizzle.
-bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
-  const MapKey key{ptr, rows, cols, box_rows};
+// Row-major bf16 [rows, cols] matrix, box = box_cols columns (one swizzle span) x box_rows rows.
+bool tensor_map(CUtensorMap* out, const MapKey& key, int box_cols, int box_rows,
+                CUtensorMapSwizzle swizzle) {
   {
     std::lock_guard<std::mutex> lock(g_map_mutex);
     auto it = g_maps.find(key);
@@ -97,21 +97,34 @@ bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long col
   }
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kGemmBlockK, (cuuint32_t)box_rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)key.cols, (cuuint64_t)key.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)key.cols * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   CUtensorMap map;
-  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims,
-                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(key.ptr), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return false;
   std::lock_guard<std::mutex> lock(g_map_mutex);
   if (g_maps.size() > 4096) g_maps.clear();
   g_maps.emplace(key, map);
   *out = map;
   return true;
+}
+
+// Boxes of 64 columns, 128-byte swizzle.
+bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
+  return tensor_map(out, MapKey{ptr, rows, cols, box_rows}, kGemmBlockK, box_rows,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// A paged pool's rows: boxes of 32 columns x a page's rows (at most 128),
+// 64-byte swizzle; the key's row count is negative to tell the two apart.
+bool pool_map(CUtensorMap* out, const void* ptr, long long rows, int cols, int page_size) {
+  const int box_rows = page_size < 128 ? page_size : 128;
+  return tensor_map(out, MapKey{ptr, rows, cols, -box_rows}, 32, box_rows,
+                    CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int sm_count() {
@@ -1834,9 +1847,22 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
   a.sinks = window > 0 ? sinks : 0;
   a.scale = scale;
   a.status = status;
-  rc = parrot::launch_paged_attention(a, sm_count(), static_cast<cudaStream_t>(stream));
-  if (rc) return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
-  return check_launch("paged_attn_kernel");
+  if (parrot::paged_few_queries(a)) {
+    if (parrot::launch_paged_decode(a, sm_count(), static_cast<cudaStream_t>(stream)))
+      return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
+    return check_launch("paged_decode_kernel");
+  }
+  CUtensorMap k_map{}, v_map{};
+  if (!kv->e4m3 && kv->pages > 0) {
+    const long long pool_rows = (long long)kv->pages * kv->n_kv_heads * kv->page_size;
+    if (!pool_map(&k_map, kv->key, pool_rows, kv->head_dim, kv->page_size) ||
+        (kv->value != nullptr &&
+         !pool_map(&v_map, kv->value, pool_rows, kv->head_dim, kv->page_size)))
+      return fail(PARROT_ECUDA, "paged_attention: tensor map encode failed%s");
+  }
+  if (parrot::launch_paged_prefill(a, k_map, v_map, sm_count(), static_cast<cudaStream_t>(stream)))
+    return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
+  return check_launch("paged_prefill_kernel");
 }
 
 int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int logits_f32,

@@ -8,63 +8,13 @@
 // The query heads of one key head and a run of tokens share their keys: a
 // tile is 16 consecutive (token, head) rows of one sequence, token major, so
 // each key is read once for all of them.
-#include "paged.cuh"
 #include <algorithm>
 
-#include "tc.cuh"
+#include "paged_attn.cuh"
 
 namespace parrot {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// A tile: `rows_per` consecutive (token, head) rows of one sequence.
-struct Tile {
-  int b;           // sequence, -1: no such tile
-  int first;       // batch row of the sequence's first token
-  int n;           // its tokens in the batch
-  int row0;        // first (token, head) row of the tile
-};
-
-// The tile with this number, sequences in order, ceil(n_b * group / rows_per)
-// tiles each.  A whole warp calls; 32 sequences a step, their lengths loaded
-// side by side.
-__device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int rows_per, int tile) {
-  const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int b0 = 0; b0 < s.batch; b0 += 32) {
-    const int b = b0 + lane;
-    int2 r = make_int2(0, 0);
-    if (b < s.batch) r = batch_rows(s, b);
-    const int n = r.y - r.x;
-    const int mine = (int)(((long long)n * group + rows_per - 1) / rows_per);
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += t;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + upto > tile);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      Tile t;
-      t.b = b0 + l;
-      t.first = __shfl_sync(0xffffffffu, r.x, l);
-      t.n = __shfl_sync(0xffffffffu, n, l);
-      t.row0 = (tile - base - __shfl_sync(0xffffffffu, upto - mine, l)) * rows_per;
-      return t;
-    }
-    base += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return Tile{-1, 0, 0, 0};
-}
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -95,20 +45,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) != 0x7f80u; }
 
 // ---------------------------------------------------------------------------
@@ -548,7 +484,13 @@ int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
 
 }  // namespace
 
-int launch_paged_attention(const PagedAttnArgs& a, int sms, cudaStream_t stream) {
+// Up to four new tokens per sequence on the average, the kernel above (its
+// tile reads the keys for 16 rows); beyond, paged_prefill.cu's (for 256).
+bool paged_few_queries(const PagedAttnArgs& a) {
+  return a.batch.tokens <= 4LL * a.batch.batch;
+}
+
+int launch_paged_decode(const PagedAttnArgs& a, int sms, cudaStream_t stream) {
   switch (a.kv.head_dim) {
     case 32: return launch_decode_d<32>(a, stream, sms);
     case 64: return launch_decode_d<64>(a, stream, sms);

@@ -1,0 +1,743 @@
+// Attention of many queries per sequence over the paged cache: the tensor-core
+// kernel behind launch_paged_attention (paged_attn.cu states the formula and
+// takes the batches of few queries).
+//
+// A CTA takes 256 (token, head) rows of one sequence and key head as two halves
+// of 128, and streams the keys they see in tiles of 128:
+//   S_h = Q_h K^T (tcgen05, both operands in shared memory, S in TMEM),
+//   one thread per row: running maximum, p = 2^(s - m), P in bf16 back into
+//   TMEM over S, O_h += P_h V (tcgen05, P from TMEM, V from shared memory).
+// While the threads of one half exponentiate, the tensor core multiplies for
+// the other.  A row's maximum m is only moved when it grows by more than 2^8
+// (p then stays below 2^8, and O and the sum are fp32), so O is rarely
+// rescaled.  The sum is of the unrounded p.
+//
+// Warps: 0-3 and 4-7 the halves' rows, 8-10 bring K and V, 11 issues the matrix
+// instructions.  A bf16 cache comes by TMA, a page's rows of 32 columns at a
+// time into a 64-byte-swizzled tile (three boxes for a 96-wide head); an e4m3
+// cache is read, widened and stored to the same tiles by warps 8-10.
+//
+// Tiles at an edge of what the rows see (the diagonal, the window's start, the
+// sinks) pass through warps 9-10 first: in a product 0 * NaN would carry a
+// number from a masked place to every row, so rows of V that nobody sees become
+// zeros, and numbers that are not finite are taken out and noted; a row that
+// does see one gets NaN in that column.
+//
+// With few tiles a cluster of CTAs shares one, each taking a run of its key
+// tiles, and merges the results over distributed shared memory.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace parrot {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kPfThreads = 384;
+constexpr int kPfHalf = 128;            // rows of a half, and keys of a tile
+constexpr int kPfRows = 2 * kPfHalf;    // rows of a tile
+constexpr int kLoadWarps = 3;
+constexpr int kMmaWarp = 11;
+constexpr int kMaxRanks = 8;
+constexpr uint32_t kTmemS = 0, kTmemO = 256;  // + 128 * half
+constexpr float kGrowth = 8.f;          // log2 of the growth of a maximum let through
+
+template <int D, bool SEP>
+struct PrefillShape {
+  static constexpr int kSlabs = D / 32;              // 64-byte columns of a tile
+  static constexpr int kTile = kPfHalf * D * 2;
+  static constexpr int kSlab = kPfHalf * 64;
+  static constexpr int kStages = D == 128 && SEP ? 2 : 3;
+  static constexpr int kSides = SEP ? 2 : 1;
+  static constexpr int kQ = 2 * kTile;
+  static constexpr int kRing = kStages * kTile;
+  static constexpr int kBad = kStages * kPfHalf * 16;  // noted columns of each row of a V tile
+  static constexpr int kPart = kPfRows * D * 4;        // a CTA's result, over Q and the rings
+  static constexpr int kBytes0 = kQ + kSides * kRing + kBad + 1024;
+  // one CTA per SM: each takes all of the TMEM
+  static constexpr int kBytes = kBytes0 < 118784 ? 118784 : kBytes0;
+  static_assert(kPart <= kQ + kSides * kRing, "the result fits the tiles");
+};
+
+struct PrefillState {
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], raw[3];
+  uint64_t s_full[2], p_ready[2], o_done[2], q_ready, drain;
+  uint32_t tmem;
+  int abort;
+  int bad[3];
+  uint64_t* armed[2][3];       // the barrier of each stage's last copy, and its phase
+  uint32_t armed_parity[2][3];
+  int row[kPfHalf];            // e4m3: pool row of each key of the tile, -1: zeros
+  uint32_t scale[kPfHalf];     // its scale bytes (key, value)
+  float m[kPfRows], l[kPfRows];  // merge
+};
+
+__device__ __forceinline__ uint64_t sw64_desc(uint32_t addr, uint32_t lead) {
+  return ((uint64_t)(addr >> 4) & 0x3FFFull)  // start address
+         | ((uint64_t)(lead >> 4) << 16)      // leading byte offset
+         | (32ull << 32)                      // stride byte offset: 512 B between 8-row groups
+         | (1ull << 46)                       // descriptor version (sm_100)
+         | (4ull << 61);                      // 64-byte swizzle
+}
+
+// D += A B with A (bf16 pairs, one row a lane) in TMEM.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// a barrier of the first `threads` threads that name it, and the or of a flag
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool named_or(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+// byte offset of 16-byte vector c of row r in a 64-byte-swizzled tile
+template <int D>
+__device__ __forceinline__ uint32_t sw64_at(int r, int c) {
+  return (uint32_t)((c >> 2) * (kPfHalf * 64) + r * 64 + (((c & 3) ^ ((r >> 1) & 3)) << 4));
+}
+
+// bits of the four bf16 pairs of a vector that are not finite, one a number
+__device__ __forceinline__ uint32_t not_finite8(const uint4& v) {
+  uint32_t bits = 0;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    bits |= (w[i] & 0x7f80u) == 0x7f80u ? 1u << (2 * i) : 0u;
+    bits |= (w[i] & 0x7f800000u) == 0x7f800000u ? 2u << (2 * i) : 0u;
+  }
+  return bits;
+}
+__device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pair i
+  return (bits >> (2 * i) & 1 ? 0u : 0xffffu) | (bits >> (2 * i) & 2 ? 0u : 0xffff0000u);
+}
+
+}  // namespace
+
+template <int D, bool E4M3, bool SEP>
+__global__ void __launch_bounds__(kPfThreads, 1)
+    paged_prefill_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map) {
+  using S = PrefillShape<D, SEP>;
+  constexpr int NS = S::kStages;
+  extern __shared__ unsigned char pf_raw[];
+  __shared__ PrefillState st;
+  // tiles start on 1024 bytes, the swizzle's period and more
+  unsigned char* smem = pf_raw + (1024 - (smem_u32(pf_raw) & 1023)) % 1024;
+  const uint32_t q_u = smem_u32(smem), k_u = q_u + S::kQ, v_u = SEP ? k_u + S::kRing : k_u;
+  uint4* bad_cols = reinterpret_cast<uint4*>(smem + S::kQ + S::kSides * S::kRing);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  const int kvh = blockIdx.y, group = a.heads / a.kv.kv_heads;
+  volatile int* abort_flag = &st.abort;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&st.k_full[s], 1);
+      mbar_init(&st.k_empty[s], 1);
+      mbar_init(&st.v_full[s], 1);
+      mbar_init(&st.v_empty[s], 1);
+      mbar_init(&st.raw[s], 1);
+      st.bad[s] = 0;
+      st.armed[0][s] = st.armed[1][s] = nullptr;
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&st.s_full[h], 1);
+      mbar_init(&st.p_ready[h], 4);
+      mbar_init(&st.o_done[h], 1);
+    }
+    mbar_init(&st.q_ready, 8);
+    mbar_init(&st.drain, 1);
+    st.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  griddep_wait();
+  // tiles in reverse: a long sequence's last tiles see the most keys
+  const Tile tile =
+      find_tile(a.batch, group, kPfRows, gridDim.x / ranks - 1 - blockIdx.x / ranks);
+  if (tile.b < 0) return;  // the whole cluster, before any wait
+  if (warp == kMmaWarp) tmem_alloc(&st.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = st.tmem;
+  // not before: a kernel launched early may want TMEM, and holds it until this
+  // one has finished
+  griddep_launch();
+
+  const int ctx = context_of(a.batch, a.kv, tile.b, a.status);
+  const int rows = min(kPfRows, tile.n * group - tile.row0);
+  const int halves = rows > kPfHalf ? 2 : 1;
+  const int pos0 = ctx - tile.n;
+  const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;
+  // key tiles: the sinks' that lie before the window's first, then the window's
+  const int lo = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+  const int t_lo = lo / kPfHalf;
+  const int sink_tiles = min((min(a.sinks, lo) + kPfHalf - 1) / kPfHalf, t_lo);
+  const int all = pmax < 0 ? 0 : sink_tiles + pmax / kPfHalf - t_lo + 1;
+  const int i0 = (int)((long long)all * rank / ranks), i1 = (int)((long long)all * (rank + 1) / ranks);
+  const int n = i1 - i0;  // of this CTA
+  auto base_of = [&](int i) {
+    i += i0;
+    return (i < sink_tiles ? i : i - sink_tiles + t_lo) * kPfHalf;
+  };
+  auto some_row_sees = [&](int j) {
+    return j <= pmax && (a.window == 0 || j > pmin - a.window || j < a.sinks);
+  };
+  auto is_edge = [&](int base) {  // not every row sees every key of the tile
+    return base + kPfHalf - 1 > pmin ||
+           (a.window > 0 && base <= pmax - a.window && base + kPfHalf > a.sinks);
+  };
+
+  if (warp < 8) {
+    // ---------------- rows ----------------
+    const int half = warp >> 2, r = half * kPfHalf + (warp & 3) * 32 + lane;
+    const int row = tile.row0 + min(r, rows - 1);
+    const int token = tile.first + row / group, head = kvh * group + row % group;
+    const int pos = pos0 + row / group;
+    {  // the row's query, swizzled; rows that do not exist are zeros
+      const uint4* q = reinterpret_cast<const uint4*>(a.q + (long long)token * a.q_row + (long long)head * D);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = r < rows ? q[c] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(smem + half * S::kTile + sw64_at<D>(r & (kPfHalf - 1), c)) = v;
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st.q_ready);
+    }
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_at = lane_addr + kTmemS + half * 128, o_at = lane_addr + kTmemO + half * 128;
+    const float scale2 = a.scale * kLog2e;
+    const float growth = kGrowth / scale2;
+    float m = -INFINITY, l = 0.f;
+    uint32_t poison[S::kSlabs];
+#pragma unroll
+    for (int i = 0; i < S::kSlabs; ++i) poison[i] = 0;
+    bool ok = half < halves;
+    const bool busy = ok;
+    for (int i = 0; ok && i < n; ++i) {
+      if (!mbar_wait_fast(&st.s_full[half], i & 1, abort_flag, a.status, 60)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32_async(s_at + 32 * c, s[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+      const int base = base_of(i);
+      const bool edge = is_edge(base);
+      if (edge) {
+        const int hi = pos - base;  // keys [lo, hi] and [0, sk) of the tile
+        const int low = a.window > 0 ? hi - a.window + 1 : -0x7fffffff, sk = a.sinks - base;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int k = 32 * c + j;
+            if (!(k <= hi && (k >= low || k < sk))) s[c][j] = 0xff800000u;
+          }
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+#pragma unroll
+        for (int j = 2; j < 32; j += 2)
+          mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool move = top > m + growth || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, move)) {
+        const float corr = move ? exp2_fast((m - top) * scale2) : 1.f;
+        if (move) m = top;
+        l *= corr;
+        if (i > 0) {  // the previous product is complete: S was issued after it
+#pragma unroll
+          for (int c = 0; c < S::kSlabs; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+            tmem_st32(o_at + 32 * c, o);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : -m * scale2;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const uint32_t* src = s[2 * c + (j >> 4)];
+          const float x = exp2_fast(fmaf(__uint_as_float(src[2 * (j & 15)]), scale2, off));
+          const float y = exp2_fast(fmaf(__uint_as_float(src[2 * (j & 15) + 1]), scale2, off));
+          sum[j & 1] += x;
+          sum[2 + (j & 1)] += y;
+          p[j] = pack_bf16x2(x, y);
+        }
+        tmem_st32(s_at + 32 * c, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      if (edge) {
+        // was a value taken out of the tile that this row sees?
+        const int stage = i % NS;
+        uint64_t* full = SEP ? &st.v_full[stage] : &st.k_full[stage];
+        if (!mbar_wait_fast(full, (i / NS) & 1, abort_flag, a.status, 61)) {
+          ok = false;
+          break;
+        }
+        if (*reinterpret_cast<volatile int*>(&st.bad[stage])) {
+          for (int k = 0; k < kPfHalf; ++k) {
+            const int j = base + k;
+            if (j <= pos && (a.window == 0 || pos - j < a.window || j < a.sinks)) {
+              const uint4 w = bad_cols[stage * kPfHalf + k];
+              const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int c = 0; c < S::kSlabs; ++c) poison[c] |= b[c];
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st.p_ready[half]);
+    }
+    // ---------------- result ----------------
+    for (int h = 0; ok && n > 0 && h < halves; ++h)
+      ok = mbar_wait(&st.o_done[h], 0, abort_flag, a.status, 62);
+    tc_fence_after();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat16* out = a.out + ((long long)token * a.heads + head) * D;
+    float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int c = 0; c < S::kSlabs; ++c) {
+      uint32_t o[32];
+      if (busy && n > 0) {
+        tmem_ld32(o_at + 32 * c, o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = 0;
+      }
+      if (poison[c]) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (poison[c] >> j & 1) o[j] = 0x7fc00000u;
+      }
+      if (!ok || r >= rows) continue;
+      if (ranks == 1) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          uint4 w;
+          w.x = pack_bf16x2(__uint_as_float(o[8 * v]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
+          w.y = pack_bf16x2(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
+          w.z = pack_bf16x2(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
+          w.w = pack_bf16x2(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
+          reinterpret_cast<uint4*>(out)[c * 4 + v] = w;
+        }
+      } else {
+        // rows of D floats, 16-byte vectors exchanged by the row's low bits so
+        // that the lanes' stores fall in different banks
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          *reinterpret_cast<uint4*>(part + r * D + (((c * 8 + v) ^ (r & 7)) << 2)) =
+              make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      }
+    }
+    st.m[r] = m * scale2;
+    st.l[r] = l;
+  } else if (warp < 8 + kLoadWarps) {
+    // ---------------- keys and values ----------------
+    const int lt = threadIdx.x - 256;  // 0 .. 95
+    uint32_t raw_phase = 0;            // a bit per stage
+    if constexpr (!E4M3) {
+      if (warp == 8) {
+        bool ok = true;
+        const int box = min(1 << a.kv.page_shift, kPfHalf);  // rows of a TMA box
+        const int pieces = kPfHalf / box;
+        const int beyond = a.kv.pages * a.kv.kv_heads << a.kv.page_shift;  // past the pool: zeros
+        for (int i = 0; ok && i < n; ++i) {
+          const int s = i % NS;
+          const int base = base_of(i);
+          const bool edge = is_edge(base);
+          // lane p holds the pool row of piece p
+          int at = beyond;
+          if (lane < pieces) {
+            const int j0 = base + lane * box;
+            // a piece that some row sees part of (its sinks, or a key up to pmax
+            // behind the window's start)
+            if (j0 <= pmax && (j0 < a.sinks || a.window == 0 || j0 + box - 1 > pmin - a.window)) {
+              // a page partly in sight: its first position that is
+              const int page = page_of(a.batch, a.kv, tile.b, j0, a.status);
+              if (page >= 0) at = (int)pool_row(a.kv, page, kvh, j0);
+            }
+          }
+          for (int side = 0; side < S::kSides; ++side) {
+            uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
+            if (i >= NS && !mbar_wait_fast(empty, (i / NS - 1) & 1, abort_flag, a.status, 63)) {
+              ok = false;
+              break;
+            }
+            uint64_t* full = side ? &st.v_full[s] : &st.k_full[s];
+            // the side that holds the values passes the check at an edge
+            if (edge && side == S::kSides - 1) full = &st.raw[s];
+            if (lane == 0) mbar_arrive_expect_tx(full, S::kTile);
+            __syncwarp();
+            unsigned char* dst = smem + S::kQ + side * S::kRing + s * S::kTile;
+            for (int b0 = 0; b0 < pieces * S::kSlabs; b0 += 32) {
+              const int b = b0 + lane, piece = b / S::kSlabs, slab = b - piece * S::kSlabs;
+              const int y = __shfl_sync(0xffffffffu, at, piece & 31);
+              if (b < pieces * S::kSlabs)
+                tma_load_2d(dst + slab * S::kSlab + piece * box * 64, side ? &v_map : &k_map,
+                            slab * 32, y, full);
+            }
+            // what is to be waited for should the CTA give up
+            if (full == &st.raw[s]) raw_phase ^= 1u << s;
+            if (lane == 0) {
+              st.armed[side][s] = full;
+              st.armed_parity[side][s] =
+                  full == &st.raw[s] ? (raw_phase >> s & 1) ^ 1 : (uint32_t)(i / NS) & 1;
+            }
+            __syncwarp();
+          }
+        }
+        // if a wait ran out somewhere: copies on their way land before the CTA goes on
+        if (lane == 0 && *abort_flag) {
+          for (int side = 0; side < S::kSides; ++side)
+            for (int s = 0; s < NS; ++s)
+              if (st.armed[side][s] != nullptr) mbar_drain(st.armed[side][s], st.armed_parity[side][s]);
+        }
+        __syncwarp();
+      } else {
+        // warps 9-10: the edge tiles' values
+        const int ct = lt - 32;
+        for (int i = 0; i < n; ++i) {
+          const int base = base_of(i);
+          if (!is_edge(base)) continue;
+          const int s = i % NS;
+          const bool mine = mbar_wait(&st.raw[s], raw_phase >> s & 1, abort_flag, a.status, 64);
+          if (named_or(1, 64, !mine)) break;  // both warps stop together
+          raw_phase ^= 1u << s;
+          unsigned char* tile_p = smem + S::kQ + (S::kSides - 1) * S::kRing + s * S::kTile;
+          bool any = false;
+          for (int k = ct; k < kPfHalf; k += 64) {
+            const bool seen = some_row_sees(base + k);
+            uint32_t cols[4] = {0, 0, 0, 0};
+            bool row_bad = false;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              uint4* p = reinterpret_cast<uint4*>(tile_p + sw64_at<D>(k, c));
+              if (!seen) {
+                *p = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 v = *p;
+              const uint32_t bits = not_finite8(v);
+              if (bits) {
+                cols[c >> 2] |= bits << (8 * (c & 3));
+                row_bad = true;
+                v.x &= keep_mask(bits, 0);
+                v.y &= keep_mask(bits, 1);
+                v.z &= keep_mask(bits, 2);
+                v.w &= keep_mask(bits, 3);
+                *p = v;
+              }
+            }
+            // a latent's key is its value: a row that sees it has no score left
+            if (!SEP && row_bad) cols[0] = cols[1] = cols[2] = cols[3] = 0xffffffffu;
+            bad_cols[s * kPfHalf + k] = make_uint4(cols[0], cols[1], cols[2], cols[3]);
+            any |= row_bad;
+          }
+          fence_async_shared();
+          any = named_or(1, 64, any);
+          if (ct == 0) {
+            st.bad[s] = any;
+            mbar_arrive(SEP ? &st.v_full[s] : &st.k_full[s]);
+          }
+        }
+      }
+    } else {
+      constexpr int VR = D / 16;                           // 16-byte vectors of a raw row
+      constexpr int kPer = (kPfHalf * VR + 95) / 96;       // of a thread
+      bool ok = true;
+      uint4 raw[kPer];
+      auto fetch = [&](const void* pool) {
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          const int v = lt + 96 * x;
+          raw[x] = make_uint4(0, 0, 0, 0);
+          if (v < kPfHalf * VR) {
+            const int k = v / VR, c = v - k * VR, at = st.row[k];
+            if (at >= 0) raw[x] = reinterpret_cast<const uint4*>(pool)[(long long)at * VR + c];
+          }
+        }
+      };
+      auto widen = [&](unsigned char* dst, int shift, int s, bool check) {
+        bool any = false;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          const int v = lt + 96 * x;
+          if (v < kPfHalf * VR) {
+            const int k = v / VR, c = v - k * VR;
+            const uint32_t s2 = scale_pair(st.scale[k] >> shift & 0xff);
+            const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint2 y = e4m3x4_to_bf16(w[2 * h], s2), z = e4m3x4_to_bf16(w[2 * h + 1], s2);
+              uint4 o = make_uint4(y.x, y.y, z.x, z.y);
+              if (check) {
+                const uint32_t bits = not_finite8(o);
+                if (bits) {
+                  any = true;
+                  const int c8 = 2 * c + h;
+                  uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * kPfHalf + k);
+                  if (SEP) {
+                    atomicOr(cols + (c8 >> 2), bits << (8 * (c8 & 3)));
+                  } else {
+                    for (int q = 0; q < 4; ++q) atomicOr(cols + q, 0xffffffffu);
+                  }
+                  o.x &= keep_mask(bits, 0);
+                  o.y &= keep_mask(bits, 1);
+                  o.z &= keep_mask(bits, 2);
+                  o.w &= keep_mask(bits, 3);
+                }
+              }
+              *reinterpret_cast<uint4*>(dst + sw64_at<D>(k, 2 * c + h)) = o;
+            }
+          }
+        }
+        return any;
+      };
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i % NS, base = base_of(i);
+        const bool edge = is_edge(base);
+        for (int k = lt; k < kPfHalf; k += 96) {
+          const int j = base + k;
+          int at = -1;
+          if (some_row_sees(j)) {
+            const int page = page_of(a.batch, a.kv, tile.b, j, a.status);
+            if (page >= 0) at = (int)pool_row(a.kv, page, kvh, j);
+          }
+          st.row[k] = at;
+          st.scale[k] = at < 0 ? 0u : (uint32_t)a.kv.key_scale[at] |
+                                          (SEP ? (uint32_t)a.kv.value_scale[at] << 8 : 0u);
+        }
+        named_sync(1, 96);
+        for (int side = 0; side < S::kSides; ++side) {
+          fetch(side ? a.kv.value : a.kv.key);
+          uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
+          bool mine = i < NS || mbar_wait_fast(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
+          ok = !named_or(1, 96, !mine);  // all 96 stop together
+          if (!ok) break;
+          const bool check = edge && side == S::kSides - 1;
+          if (check)
+            for (int k = lt; k < kPfHalf; k += 96) bad_cols[s * kPfHalf + k] = make_uint4(0, 0, 0, 0);
+          if (check) named_sync(1, 96);
+          const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, 8 * side, s, check);
+          fence_async_shared();
+          const bool found = named_or(1, 96, any);
+          if (lt == 0) {
+            if (check) st.bad[s] = found;
+            mbar_arrive(side ? &st.v_full[s] : &st.k_full[s]);
+          }
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------- matrix instructions ----------------
+    if (lane == 0 && n > 0) {
+      const uint32_t id_s = make_idesc(kPfHalf, kPfHalf);
+      const uint32_t id_o = make_idesc(kPfHalf, D) | (1u << 16);  // V: columns contiguous
+      bool ok = mbar_wait_fast(&st.q_ready, 0, abort_flag, a.status, 65);
+      auto scores = [&](int h, int s) {
+        const uint64_t qd = sw64_desc(q_u + h * S::kTile, 16), kd = sw64_desc(k_u + s * S::kTile, 16);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)((k >> 1) * S::kSlab + (k & 1) * 32) >> 4;
+          mma_bf16(tmem + kTmemS + h * 128, qd + off, kd + off, id_s, k != 0);
+        }
+      };
+      auto values = [&](int h, int s, uint32_t accumulate) {
+        const uint64_t vd = sw64_desc(v_u + s * S::kTile, S::kSlab);
+#pragma unroll
+        for (int k = 0; k < kPfHalf / 16; ++k)
+          mma_bf16_ts(tmem + kTmemO + h * 128, tmem + kTmemS + h * 128 + k * 8,
+                      vd + (uint32_t)(k * 1024 >> 4), id_o, accumulate | (k != 0));
+      };
+      if (ok && (ok = mbar_wait_fast(&st.k_full[0], 0, abort_flag, a.status, 66))) {
+        tc_fence_after();
+        for (int h = 0; h < halves; ++h) {
+          scores(h, 0);
+          mma_commit(&st.s_full[h]);
+        }
+        if (SEP) mma_commit(&st.k_empty[0]);
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i % NS, s1 = (i + 1) % NS;
+        if (SEP && !(ok = mbar_wait_fast(&st.v_full[s], (i / NS) & 1, abort_flag, a.status, 67))) break;
+        for (int h = 0; ok && h < halves; ++h) {
+          if (!(ok = mbar_wait_fast(&st.p_ready[h], i & 1, abort_flag, a.status, 68))) break;
+          tc_fence_after();
+          values(h, s, i > 0);
+          if (i == n - 1) mma_commit(&st.o_done[h]);
+          if (h == halves - 1) mma_commit(SEP ? &st.v_empty[s] : &st.k_empty[s]);
+          if (i + 1 < n) {
+            if (h == 0) {
+              if (!(ok = mbar_wait_fast(&st.k_full[s1], ((i + 1) / NS) & 1, abort_flag, a.status, 66))) break;
+              tc_fence_after();
+            }
+            scores(h, s1);
+            mma_commit(&st.s_full[h]);
+            if (SEP && h == halves - 1) mma_commit(&st.k_empty[s1]);
+          }
+        }
+      }
+      // all matrix instructions have finished before TMEM is freed
+      mma_commit(&st.drain);
+      mbar_drain(&st.drain, 0);
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // freed before the cluster waits: a CTA that waits for TMEM on this SM may
+  // be the one that a peer of this cluster waits behind
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+  if (ranks == 1) return;
+  cluster_sync();
+  // each CTA merges its share of the tile's 16-byte vectors
+  const float* part = reinterpret_cast<const float*>(smem);
+  for (int v = rank * kPfThreads + threadIdx.x; v < rows * (D / 4); v += ranks * kPfThreads) {
+    const int r = v / (D / 4), c = v - r * (D / 4);
+    const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
+    float mx = -INFINITY, sum = 0.f;
+    float mk[kMaxRanks];
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      mk[k] = k < ranks ? ld_cluster_f1(mapa_addr(smem_u32(&st.m[r]), k)) : -INFINITY;
+      mx = fmaxf(mx, mk[k]);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      if (k >= ranks) break;
+      const float f = mk[k] == -INFINITY ? 0.f : exp2_fast(mk[k] - mx);
+      sum = fmaf(f, ld_cluster_f1(mapa_addr(smem_u32(&st.l[r]), k)), sum);
+      if (mk[k] == -INFINITY) continue;  // it saw nothing, and may have stored nothing
+      const float4 x = ld_cluster_f4(mapa_addr(at, k));
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int row = tile.row0 + r;
+    uint2 w;
+    w.x = pack_bf16x2(o.x * inv, o.y * inv);
+    w.y = pack_bf16x2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + row / group) * a.heads +
+                                       kvh * group + row % group) * D + c * 4) = w;
+  }
+  cluster_sync();  // nobody leaves while its result may be read
+}
+
+namespace {
+
+template <int D, bool E4M3, bool SEP>
+int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map, int sms,
+                   cudaStream_t stream) {
+  using S = PrefillShape<D, SEP>;
+  auto k = paged_prefill_kernel<D, E4M3, SEP>;
+  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
+  const long long tiles = std::min(n * ((group + kPfRows - 1) / kPfRows),
+                                   n * group / kPfRows + std::min<long long>(a.batch.batch, n));
+  // CTAs per tile while the GPU has SMs to spare
+  int ranks = 1;
+  while (ranks < kMaxRanks && 2 * ranks * tiles * a.kv.kv_heads <= sms) ranks *= 2;
+  a.cluster = ranks;
+  if (tiles * ranks > 0x7fffffffll) return -1;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
+    return -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);
+  cfg.blockDim = dim3(kPfThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)ranks, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k, a, k_map, v_map) == cudaSuccess ? 0 : -2;
+}
+
+template <int D>
+int launch_prefill_d(const PagedAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, int sms,
+                     cudaStream_t stream) {
+  const bool sep = a.kv.value != nullptr;
+  if (a.kv.key_scale != nullptr)
+    return sep ? launch_prefill<D, true, true>(a, k, v, sms, stream)
+               : launch_prefill<D, true, false>(a, k, v, sms, stream);
+  return sep ? launch_prefill<D, false, true>(a, k, v, sms, stream)
+             : launch_prefill<D, false, false>(a, k, v, sms, stream);
+}
+
+}  // namespace
+
+int launch_paged_prefill(const PagedAttnArgs& a, const CUtensorMap& k_map,
+                         const CUtensorMap& v_map, int sms, cudaStream_t stream) {
+  switch (a.kv.head_dim) {
+    case 32: return launch_prefill_d<32>(a, k_map, v_map, sms, stream);
+    case 64: return launch_prefill_d<64>(a, k_map, v_map, sms, stream);
+    case 96: return launch_prefill_d<96>(a, k_map, v_map, sms, stream);
+    case 128: return launch_prefill_d<128>(a, k_map, v_map, sms, stream);
+  }
+  return -1;
+}
+
+}  // namespace parrot
