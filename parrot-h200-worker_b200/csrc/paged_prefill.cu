@@ -110,6 +110,34 @@ __device__ __forceinline__ void tmem_wait_st() {
 __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+// The bounded wait of these warps: the thread sleeps in the barrier for up to
+// 0.1 ms at a time instead of polling, so that waiting warps leave the issue
+// slots to the exponentials (polling cost the other warps of a scheduler half
+// their speed).
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity,
+                                            volatile int* abort_flag, int* status, int site) {
+  const uint32_t at = smem_u32(bar);
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(100000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      report_status(status, kStatusWaitTimeout, site, (int)blockIdx.x);
+      return false;
+    }
+  }
+}
 // a barrier of the first `threads` threads that name it, and the or of a flag
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -146,6 +174,57 @@ __device__ __forceinline__ uint32_t not_finite8(const uint4& v) {
 }
 __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pair i
   return (bits >> (2 * i) & 1 ? 0u : 0xffffu) | (bits >> (2 * i) & 2 ? 0u : 0xffff0000u);
+}
+
+// The end of the rows' warps: with several CTAs to a tile, each merges its
+// share of the tile's 16-byte vectors.
+template <int D>
+__device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState& st,
+                                            unsigned char* smem, const Tile& tile, int rows,
+                                            int kvh, int group, int rank, int ranks) {
+  tc_fence_before();
+  __syncthreads();
+  if (ranks == 1) return;
+  cluster_sync();
+  const float* part = reinterpret_cast<const float*>(smem);
+  for (int v = rank * 256 + threadIdx.x; v < rows * (D / 4); v += ranks * 256) {
+    const int r = v / (D / 4), c = v - r * (D / 4);
+    const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
+    const uint32_t m_at = smem_u32(&st.m[r]), l_at = smem_u32(&st.l[r]);
+    float mk[kMaxRanks], lk[kMaxRanks];
+    float4 x[kMaxRanks];
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      if (k >= ranks) break;
+      mk[k] = ld_cluster_f1(mapa_addr(m_at, k));
+      lk[k] = ld_cluster_f1(mapa_addr(l_at, k));
+      x[k] = ld_cluster_f4(mapa_addr(at, k));
+    }
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k)
+      if (k < ranks) mx = fmaxf(mx, mk[k]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMaxRanks; ++k) {
+      if (k >= ranks) break;
+      const float f = mk[k] == -INFINITY ? 0.f : exp2_fast(mk[k] - mx);
+      sum = fmaf(f, lk[k], sum);
+      if (mk[k] == -INFINITY) continue;  // it saw nothing, and may have stored nothing
+      o.x = fmaf(f, x[k].x, o.x);
+      o.y = fmaf(f, x[k].y, o.y);
+      o.z = fmaf(f, x[k].z, o.z);
+      o.w = fmaf(f, x[k].w, o.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int row = tile.row0 + r;
+    uint2 w;
+    w.x = pack_bf16x2(o.x * inv, o.y * inv);
+    w.y = pack_bf16x2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + row / group) * a.heads +
+                                       kvh * group + row % group) * D + c * 4) = w;
+  }
+  cluster_sync();  // nobody leaves while its result may be read
 }
 
 }  // namespace
@@ -228,16 +307,27 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
   if (warp < 8) {
     // ---------------- rows ----------------
+    // a row of S is 128 registers: 8 warps x 208 + 4 x 88 = 12 x 168 of launch
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int half = warp >> 2, r = half * kPfHalf + (warp & 3) * 32 + lane;
     const int row = tile.row0 + min(r, rows - 1);
     const int token = tile.first + row / group, head = kvh * group + row % group;
     const int pos = pos0 + row / group;
-    {  // the row's query, swizzled; rows that do not exist are zeros
-      const uint4* q = reinterpret_cast<const uint4*>(a.q + (long long)token * a.q_row + (long long)head * D);
+    {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
+      const uint4* mine = reinterpret_cast<const uint4*>(a.q + (long long)token * a.q_row + (long long)head * D);
+      const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(mine) : 0ull;
+      constexpr int VR = D / 8;
+      uint4 v[VR];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 v = r < rows ? q[c] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(smem + half * S::kTile + sw64_at<D>(r & (kPfHalf - 1), c)) = v;
+      for (int x = 0; x < VR; ++x) {  // side by side: 32 vectors of the warp's rows a step
+        const int i = 32 * x + lane;
+        const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
+        v[x] = src != nullptr ? src[i % VR] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int x = 0; x < VR; ++x) {
+        const int i = 32 * x + lane;
+        *reinterpret_cast<uint4*>(smem + half * S::kTile + sw64_at<D>((warp & 3) * 32 + i / VR, i % VR)) = v[x];
       }
       fence_async_shared();
       __syncwarp();
@@ -254,7 +344,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     bool ok = half < halves;
     const bool busy = ok;
     for (int i = 0; ok && i < n; ++i) {
-      if (!mbar_wait_fast(&st.s_full[half], i & 1, abort_flag, a.status, 60)) {
+      if (!wait_asleep(&st.s_full[half], i & 1, abort_flag, a.status, 60)) {
         ok = false;
         break;
       }
@@ -274,7 +364,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const int k = 32 * c + j;
-            if (!(k <= hi && (k >= low || k < sk))) s[c][j] = 0xff800000u;
+            // no short circuits: they would become branches
+            s[c][j] = (int)(k <= hi) & ((int)(k >= low) | (int)(k < sk)) ? s[c][j] : 0xff800000u;
           }
       }
       float mx[4];
@@ -303,28 +394,33 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
       }
       const float off = m == -INFINITY ? 0.f : -m * scale2;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 scale_2 = make_float2(scale2, scale2), off_2 = make_float2(off, off);
+      float2 sum[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t p[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           const uint32_t* src = s[2 * c + (j >> 4)];
-          const float x = exp2_fast(fmaf(__uint_as_float(src[2 * (j & 15)]), scale2, off));
-          const float y = exp2_fast(fmaf(__uint_as_float(src[2 * (j & 15) + 1]), scale2, off));
-          sum[j & 1] += x;
-          sum[2 + (j & 1)] += y;
-          p[j] = pack_bf16x2(x, y);
+          float2 x = make_float2(__uint_as_float(src[2 * (j & 15)]), __uint_as_float(src[2 * (j & 15) + 1]));
+          x = __ffma2_rn(x, scale_2, off_2);
+          x.x = exp2_fast(x.x);
+          x.y = exp2_fast(x.y);
+          sum[j & 3] = __fadd2_rn(sum[j & 3], x);
+          p[j] = pack_bf16x2(x.x, x.y);
         }
         tmem_st32(s_at + 32 * c, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sum[0] = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+      l += sum[0].x + sum[0].y;
       tmem_wait_st();
       if (edge) {
         // was a value taken out of the tile that this row sees?
         const int stage = i % NS;
         uint64_t* full = SEP ? &st.v_full[stage] : &st.k_full[stage];
-        if (!mbar_wait_fast(full, (i / NS) & 1, abort_flag, a.status, 61)) {
+        if (!wait_asleep(full, (i / NS) & 1, abort_flag, a.status, 61)) {
           ok = false;
           break;
         }
@@ -346,7 +442,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     // ---------------- result ----------------
     for (int h = 0; ok && n > 0 && h < halves; ++h)
-      ok = mbar_wait(&st.o_done[h], 0, abort_flag, a.status, 62);
+      ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62);
     tc_fence_after();
     const float inv = l == 0.f ? 0.f : 1.f / l;
     __nv_bfloat16* out = a.out + ((long long)token * a.heads + head) * D;
@@ -387,7 +483,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     st.m[r] = m * scale2;
     st.l[r] = l;
-  } else if (warp < 8 + kLoadWarps) {
+    finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks);
+    return;
+  }
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp < 8 + kLoadWarps) {
     // ---------------- keys and values ----------------
     const int lt = threadIdx.x - 256;  // 0 .. 95
     uint32_t raw_phase = 0;            // a bit per stage
@@ -415,7 +515,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
           for (int side = 0; side < S::kSides; ++side) {
             uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
-            if (i >= NS && !mbar_wait_fast(empty, (i / NS - 1) & 1, abort_flag, a.status, 63)) {
+            if (i >= NS && !wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63)) {
               ok = false;
               break;
             }
@@ -456,7 +556,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           const int base = base_of(i);
           if (!is_edge(base)) continue;
           const int s = i % NS;
-          const bool mine = mbar_wait(&st.raw[s], raw_phase >> s & 1, abort_flag, a.status, 64);
+          const bool mine = wait_asleep(&st.raw[s], raw_phase >> s & 1, abort_flag, a.status, 64);
           if (named_or(1, 64, !mine)) break;  // both warps stop together
           raw_phase ^= 1u << s;
           unsigned char* tile_p = smem + S::kQ + (S::kSides - 1) * S::kRing + s * S::kTile;
@@ -567,7 +667,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int side = 0; side < S::kSides; ++side) {
           fetch(side ? a.kv.value : a.kv.key);
           uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
-          bool mine = i < NS || mbar_wait_fast(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
+          bool mine = i < NS || wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
           ok = !named_or(1, 96, !mine);  // all 96 stop together
           if (!ok) break;
           const bool check = edge && side == S::kSides - 1;
@@ -589,7 +689,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     if (lane == 0 && n > 0) {
       const uint32_t id_s = make_idesc(kPfHalf, kPfHalf);
       const uint32_t id_o = make_idesc(kPfHalf, D) | (1u << 16);  // V: columns contiguous
-      bool ok = mbar_wait_fast(&st.q_ready, 0, abort_flag, a.status, 65);
+      bool ok = wait_asleep(&st.q_ready, 0, abort_flag, a.status, 65);
       auto scores = [&](int h, int s) {
         const uint64_t qd = sw64_desc(q_u + h * S::kTile, 16), kd = sw64_desc(k_u + s * S::kTile, 16);
 #pragma unroll
@@ -605,7 +705,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           mma_bf16_ts(tmem + kTmemO + h * 128, tmem + kTmemS + h * 128 + k * 8,
                       vd + (uint32_t)(k * 1024 >> 4), id_o, accumulate | (k != 0));
       };
-      if (ok && (ok = mbar_wait_fast(&st.k_full[0], 0, abort_flag, a.status, 66))) {
+      if (ok && (ok = wait_asleep(&st.k_full[0], 0, abort_flag, a.status, 66))) {
         tc_fence_after();
         for (int h = 0; h < halves; ++h) {
           scores(h, 0);
@@ -613,25 +713,27 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         if (SEP) mma_commit(&st.k_empty[0]);
       }
+      // The thread issues at the tensor core's pace, so what it does between
+      // the products is time lost: copies are waited for ahead of the rows.
       for (int i = 0; ok && i < n; ++i) {
         const int s = i % NS, s1 = (i + 1) % NS;
-        if (SEP && !(ok = mbar_wait_fast(&st.v_full[s], (i / NS) & 1, abort_flag, a.status, 67))) break;
-        for (int h = 0; ok && h < halves; ++h) {
-          if (!(ok = mbar_wait_fast(&st.p_ready[h], i & 1, abort_flag, a.status, 68))) break;
+        const bool more = i + 1 < n;
+        if (SEP && !(ok = wait_asleep(&st.v_full[s], (i / NS) & 1, abort_flag, a.status, 67))) break;
+        if (more && !(ok = wait_asleep(&st.k_full[s1], ((i + 1) / NS) & 1, abort_flag, a.status, 66))) break;
+        for (int h = 0; h < halves; ++h) {
+          if (!(ok = wait_asleep(&st.p_ready[h], i & 1, abort_flag, a.status, 68))) break;
           tc_fence_after();
           values(h, s, i > 0);
-          if (i == n - 1) mma_commit(&st.o_done[h]);
-          if (h == halves - 1) mma_commit(SEP ? &st.v_empty[s] : &st.k_empty[s]);
-          if (i + 1 < n) {
-            if (h == 0) {
-              if (!(ok = mbar_wait_fast(&st.k_full[s1], ((i + 1) / NS) & 1, abort_flag, a.status, 66))) break;
-              tc_fence_after();
-            }
+          if (more) {
             scores(h, s1);
             mma_commit(&st.s_full[h]);
-            if (SEP && h == halves - 1) mma_commit(&st.k_empty[s1]);
+          } else {
+            mma_commit(&st.o_done[h]);
           }
         }
+        if (!ok) break;
+        mma_commit(SEP ? &st.v_empty[s] : &st.k_empty[s]);
+        if (SEP && more) mma_commit(&st.k_empty[s1]);
       }
       // all matrix instructions have finished before TMEM is freed
       mma_commit(&st.drain);
@@ -646,42 +748,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   // freed before the cluster waits: a CTA that waits for TMEM on this SM may
   // be the one that a peer of this cluster waits behind
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-  if (ranks == 1) return;
-  cluster_sync();
-  // each CTA merges its share of the tile's 16-byte vectors
-  const float* part = reinterpret_cast<const float*>(smem);
-  for (int v = rank * kPfThreads + threadIdx.x; v < rows * (D / 4); v += ranks * kPfThreads) {
-    const int r = v / (D / 4), c = v - r * (D / 4);
-    const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
-    float mx = -INFINITY, sum = 0.f;
-    float mk[kMaxRanks];
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      mk[k] = k < ranks ? ld_cluster_f1(mapa_addr(smem_u32(&st.m[r]), k)) : -INFINITY;
-      mx = fmaxf(mx, mk[k]);
-    }
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      if (k >= ranks) break;
-      const float f = mk[k] == -INFINITY ? 0.f : exp2_fast(mk[k] - mx);
-      sum = fmaf(f, ld_cluster_f1(mapa_addr(smem_u32(&st.l[r]), k)), sum);
-      if (mk[k] == -INFINITY) continue;  // it saw nothing, and may have stored nothing
-      const float4 x = ld_cluster_f4(mapa_addr(at, k));
-      o.x = fmaf(f, x.x, o.x);
-      o.y = fmaf(f, x.y, o.y);
-      o.z = fmaf(f, x.z, o.z);
-      o.w = fmaf(f, x.w, o.w);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int row = tile.row0 + r;
-    uint2 w;
-    w.x = pack_bf16x2(o.x * inv, o.y * inv);
-    w.y = pack_bf16x2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + row / group) * a.heads +
-                                       kvh * group + row % group) * D + c * 4) = w;
+  if (ranks > 1) {
+    cluster_sync();
+    cluster_sync();
   }
-  cluster_sync();  // nobody leaves while its result may be read
 }
 
 namespace {
