@@ -119,10 +119,10 @@ bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long col
                     CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// A paged pool's rows: boxes of 32 columns x a page's rows (at most 128),
-// 64-byte swizzle; the key's row count is negative to tell the two apart.
+// A paged pool's rows: boxes of 32 columns, 64-byte swizzle; the key's row
+// count is negative to tell the two apart.
 bool pool_map(CUtensorMap* out, const void* ptr, long long rows, int cols, int page_size) {
-  const int box_rows = page_size < 128 ? page_size : 128;
+  const int box_rows = parrot::paged_prefill_box_rows(cols, page_size);
   return tensor_map(out, MapKey{ptr, rows, cols, -box_rows}, 32, box_rows,
                     CU_TENSOR_MAP_SWIZZLE_64B);
 }

@@ -385,7 +385,8 @@ int launch_paged_gather(const PagedGatherArgs& args, cudaStream_t stream);
 bool paged_few_queries(const PagedAttnArgs& args);
 int launch_paged_decode(const PagedAttnArgs& args, int sms, cudaStream_t stream);
 // k_map / v_map: the bf16 pools as [rows, head_dim], boxes of 32 columns x
-// min(page size, 128) rows, 64-byte swizzle (not read for e4m3 pools)
+// paged_prefill_box_rows rows, 64-byte swizzle (not read for e4m3 pools)
+int paged_prefill_box_rows(int head_dim, int page_size);
 int launch_paged_prefill(const PagedAttnArgs& args, const CUtensorMap& k_map,
                          const CUtensorMap& v_map, int sms, cudaStream_t stream);
 

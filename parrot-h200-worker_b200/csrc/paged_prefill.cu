@@ -2,23 +2,31 @@
 // kernel behind launch_paged_attention (paged_attn.cu states the formula and
 // takes the batches of few queries).
 //
-// A CTA takes 256 (token, head) rows of one sequence and key head as two halves
-// of 128, and streams the keys they see in tiles of 128:
-//   S_h = Q_h K^T (tcgen05, both operands in shared memory, S in TMEM),
+// A CTA takes 384 (token, head) rows of one sequence and key head in three groups
+// of 128 (head width 128: 256 rows in two), and streams the keys they see in
+// tiles of 64 (128):
+//   S_g = Q_g K^T (tcgen05, both operands in shared memory, S in TMEM),
 //   one thread per row: running maximum, p = 2^(s - m), P in bf16 back into
-//   TMEM over S, O_h += P_h V (tcgen05, P from TMEM, V from shared memory).
-// While the threads of one half exponentiate, the tensor core multiplies for
-// the other.  A row's maximum m is only moved when it grows by more than 2^8
-// (p then stays below 2^8, and O and the sum are fp32), so O is rarely
-// rescaled.  The sum is of the unrounded p.
+//   TMEM over S, O_g += P_g V (tcgen05, P from TMEM, V from shared memory).
+// A group's threads wait for its two products, about a third of its time; the
+// other groups' exponentials (16 a clock and SM) and products fill it.  TMEM
+// holds three groups of S and O up to width 96.  A row's maximum m is only moved
+// when it grows by more than 2^8 (p then stays below 2^8, and O and the sum are
+// fp32), so O is rarely rescaled.  The sum is of the unrounded p.
+// Measured slower on four prompts of 4096 each: two groups with tiles of 128
+// keys (135 us); with P in shared memory (its reads and Q's fill shared
+// memory's bandwidth: 151 us); with 96 keys, P apart from S and the next scores
+// computed early (152 us); with steps of 64 keys over two S blocks a group
+// (146 us); with two threads a row (145 us).
 //
-// Warps: 0-3 and 4-7 the halves' rows, 8-10 bring K and V, 11 issues the matrix
-// instructions.  A bf16 cache comes by TMA, a page's rows of 32 columns at a
-// time into a 64-byte-swizzled tile (three boxes for a 96-wide head); an e4m3
-// cache is read, widened and stored to the same tiles by warps 8-10.
+// Warps: the groups' rows first, then three that bring K and V and one that
+// issues the matrix instructions.  A bf16 cache comes by TMA, a page's rows of
+// 32 columns at a time into a 64-byte-swizzled tile (three boxes for a 96-wide
+// head); an e4m3 cache is read, widened and stored to the same tiles by the
+// three warps.
 //
 // Tiles at an edge of what the rows see (the diagonal, the window's start, the
-// sinks) pass through warps 9-10 first: in a product 0 * NaN would carry a
+// sinks) pass through two of the three first: in a product 0 * NaN would carry a
 // number from a masked place to every row, so rows of V that nobody sees become
 // zeros, and numbers that are not finite are taken out and noted; a row that
 // does see one gets NaN in that column.
@@ -35,61 +43,103 @@ namespace {
 
 using namespace tc;
 
-constexpr int kPfThreads = 384;
-constexpr int kPfHalf = 128;            // rows of a half, and keys of a tile
-constexpr int kPfRows = 2 * kPfHalf;    // rows of a tile
+constexpr int kGroup = 128;             // rows of a group
+constexpr int kMaxGroups = 3;
 constexpr int kLoadWarps = 3;
-constexpr int kMmaWarp = 11;
 constexpr int kMaxRanks = 8;
-constexpr uint32_t kTmemS = 0, kTmemO = 256;  // + 128 * half
 constexpr float kGrowth = 8.f;          // log2 of the growth of a maximum let through
+
+// Groups of rows, and keys of a tile.
+__host__ __device__ constexpr int tile_groups(int d) { return d == 128 ? 2 : 3; }
+__host__ __device__ constexpr int tile_keys(int d) { return d == 128 ? 128 : 64; }
+// Rows of a TMA box: as many as a page and a tile both hold whole.
+__host__ __device__ constexpr int paged_box_rows(int d, int page) {
+  return page < tile_keys(d) ? page : tile_keys(d);
+}
 
 template <int D, bool SEP>
 struct PrefillShape {
+  static constexpr int kGroups = tile_groups(D), kKeys = tile_keys(D);
+  static constexpr int kRows = kGroup * kGroups, kRowWarps = 4 * kGroups;
+  static constexpr int kMmaWarp = kRowWarps + kLoadWarps, kThreads = 32 * (kMmaWarp + 1);
+  // TMEM columns: S (and P over it) of group g at g * kKeys, O behind
+  static constexpr uint32_t kTmemO = kGroups * kKeys;
+  static_assert(kGroups * (kKeys + D) <= 512, "S and O of all groups");
   static constexpr int kSlabs = D / 32;              // 64-byte columns of a tile
-  static constexpr int kTile = kPfHalf * D * 2;
-  static constexpr int kSlab = kPfHalf * 64;
-  static constexpr int kStages = D == 128 && SEP ? 2 : 3;
+  static constexpr int kTile = kKeys * D * 2;
+  static constexpr int kSlab = kKeys * 64;
+  static constexpr int kStages = D == 128 ? (SEP ? 2 : 4) : SEP ? 4 : 6;
   static constexpr int kSides = SEP ? 2 : 1;
-  static constexpr int kQ = 2 * kTile;
+  static constexpr int kQGroup = kGroup * D * 2, kQSlab = kGroup * 64;
+  static constexpr int kQ = kGroups * kQGroup;
   static constexpr int kRing = kStages * kTile;
-  static constexpr int kBad = kStages * kPfHalf * 16;  // noted columns of each row of a V tile
-  static constexpr int kPart = kPfRows * D * 4;        // a CTA's result, over Q and the rings
+  static constexpr int kBad = kStages * kKeys * 16;  // noted columns of each row of a V tile
+  static constexpr int kPart = kRows * D * 4;        // a CTA's result, over Q and the rings
   static constexpr int kBytes0 = kQ + kSides * kRing + kBad + 1024;
+  static_assert(kPart <= kQ + kSides * kRing, "the result fits the tiles");
   // one CTA per SM: each takes all of the TMEM
   static constexpr int kBytes = kBytes0 < 118784 ? 118784 : kBytes0;
-  static_assert(kPart <= kQ + kSides * kRing, "the result fits the tiles");
 };
 
 struct PrefillState {
-  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], raw[3];
-  uint64_t s_full[2], p_ready[2], o_done[2], q_ready, drain;
+  uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6], raw[6];
+  uint64_t s_full[kMaxGroups], p_ready[kMaxGroups], o_done[kMaxGroups], drain;
   uint32_t tmem;
   int abort;
-  int bad[3];
-  uint64_t* armed[2][3];       // the barrier of each stage's last copy, and its phase
-  uint32_t armed_parity[2][3];
-  int row[kPfHalf];            // e4m3: pool row of each key of the tile, -1: zeros
-  uint32_t scale[kPfHalf];     // its scale bytes (key, value)
-  float m[kPfRows], l[kPfRows];  // merge
+  int bad[6];
+  uint64_t* armed[2][6];       // the barrier of each stage's last copy, and its phase
+  uint32_t armed_parity[2][6];
+  int row[128];                // e4m3: pool row of each key of the tile, -1: zeros
+  uint32_t scale[128];         // its scale bytes (key, value)
+  float m[kGroup * kMaxGroups], l[kGroup * kMaxGroups];  // merge
 };
 
-__device__ __forceinline__ uint64_t sw64_desc(uint32_t addr, uint32_t lead) {
-  return ((uint64_t)(addr >> 4) & 0x3FFFull)  // start address
-         | ((uint64_t)(lead >> 4) << 16)      // leading byte offset
-         | (32ull << 32)                      // stride byte offset: 512 B between 8-row groups
-         | (1ull << 46)                       // descriptor version (sm_100)
-         | (4ull << 61);                      // 64-byte swizzle
+// Shared-memory descriptors as two words: tiles with a 64-byte swizzle, 512 B
+// between 8-row groups; `lead` bytes between slabs (columns contiguous: V).
+// The low word moves with the address, the high word is a constant.
+__device__ __forceinline__ uint32_t sw64_lo(uint32_t addr, uint32_t lead) {
+  return (addr >> 4 & 0x3FFFu) | (lead >> 4) << 16;
 }
+constexpr uint32_t kSw64Hi = 32u          // stride byte offset 512
+                             | 1u << 14   // descriptor version (sm_100)
+                             | 4u << 29;  // 64-byte swizzle
 
-// D += A B with A (bf16 pairs, one row a lane) in TMEM.
-__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
-                                            uint32_t idesc, uint32_t accumulate) {
+// The matrix instructions, by one thread of a warp that stays together: the
+// operands are then uniform values, and the issue is not held up by moving
+// them between register files (measured: 1150 clocks for ten instructions
+// issued from a divergent thread, beside the exponentials of the other warps).
+// D (+)= A B, both from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kSw64Hi), "r"(leader));
+}
+// D (+)= A B with A (bf16 pairs, one row a lane) in TMEM
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kSw64Hi), "r"(leader));
+}
+__device__ __forceinline__ void commit_to(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
@@ -102,6 +152,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
       "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -155,10 +213,14 @@ __device__ __forceinline__ bool named_or(int id, int threads, bool v) {
   return r != 0;
 }
 
-// byte offset of 16-byte vector c of row r in a 64-byte-swizzled tile
-template <int D>
+// byte offset of 16-byte vector c of row r in a 64-byte-swizzled tile of R rows
+template <int R>
 __device__ __forceinline__ uint32_t sw64_at(int r, int c) {
-  return (uint32_t)((c >> 2) * (kPfHalf * 64) + r * 64 + (((c & 3) ^ ((r >> 1) & 3)) << 4));
+  return (uint32_t)((c >> 2) * (R * 64) + r * 64 + (((c & 3) ^ ((r >> 1) & 3)) << 4));
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) {  // the n lowest bits, n clamped to 0 .. 32
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
 
 // bits of the four bf16 pairs of a vector that are not finite, one a number
@@ -181,13 +243,13 @@ __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pai
 template <int D>
 __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState& st,
                                             unsigned char* smem, const Tile& tile, int rows,
-                                            int kvh, int group, int rank, int ranks) {
+                                            int kvh, int group, int rank, int ranks, int threads) {
   tc_fence_before();
   __syncthreads();
   if (ranks == 1) return;
   cluster_sync();
   const float* part = reinterpret_cast<const float*>(smem);
-  for (int v = rank * 256 + threadIdx.x; v < rows * (D / 4); v += ranks * 256) {
+  for (int v = rank * threads + threadIdx.x; v < rows * (D / 4); v += ranks * threads) {
     const int r = v / (D / 4), c = v - r * (D / 4);
     const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
     const uint32_t m_at = smem_u32(&st.m[r]), l_at = smem_u32(&st.l[r]);
@@ -230,11 +292,11 @@ __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState
 }  // namespace
 
 template <int D, bool E4M3, bool SEP>
-__global__ void __launch_bounds__(kPfThreads, 1)
+__global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     paged_prefill_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map) {
   using S = PrefillShape<D, SEP>;
-  constexpr int NS = S::kStages;
+  constexpr int NS = S::kStages, T = S::kKeys, NG = S::kGroups, R = S::kRows;
   extern __shared__ unsigned char pf_raw[];
   __shared__ PrefillState st;
   // tiles start on 1024 bytes, the swizzle's period and more
@@ -247,7 +309,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   volatile int* abort_flag = &st.abort;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 3; ++s) {
+    for (int s = 0; s < NS; ++s) {
       mbar_init(&st.k_full[s], 1);
       mbar_init(&st.k_empty[s], 1);
       mbar_init(&st.v_full[s], 1);
@@ -256,12 +318,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       st.bad[s] = 0;
       st.armed[0][s] = st.armed[1][s] = nullptr;
     }
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < NG; ++h) {
       mbar_init(&st.s_full[h], 1);
       mbar_init(&st.p_ready[h], 4);
       mbar_init(&st.o_done[h], 1);
     }
-    mbar_init(&st.q_ready, 8);
     mbar_init(&st.drain, 1);
     st.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -270,9 +331,31 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   griddep_wait();
   // tiles in reverse: a long sequence's last tiles see the most keys
   const Tile tile =
-      find_tile(a.batch, group, kPfRows, gridDim.x / ranks - 1 - blockIdx.x / ranks);
+      find_tile(a.batch, group, R, gridDim.x / ranks - 1 - blockIdx.x / ranks);
   if (tile.b < 0) return;  // the whole cluster, before any wait
-  if (warp == kMmaWarp) tmem_alloc(&st.tmem, 512);
+  if (warp == S::kMmaWarp) tmem_alloc(&st.tmem, 512);
+  const int rows = min(R, tile.n * group - tile.row0);
+  if (warp < S::kRowWarps) {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
+    const int r = warp * 32 + lane, row = tile.row0 + r, head = kvh * group + row % group;
+    const uint4* mine = reinterpret_cast<const uint4*>(
+        a.q + (long long)(tile.first + row / group) * a.q_row + (long long)head * D);
+    const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(mine) : 0ull;
+    constexpr int VR = D / 8;
+    uint4 v[VR];
+#pragma unroll
+    for (int x = 0; x < VR; ++x) {  // side by side: 32 vectors of the warp's rows a step
+      const int i = 32 * x + lane;
+      const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
+      v[x] = src != nullptr ? src[i % VR] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int x = 0; x < VR; ++x) {
+      const int i = 32 * x + lane;
+      *reinterpret_cast<uint4*>(smem + (warp >> 2) * S::kQGroup +
+                                sw64_at<kGroup>((warp & 3) * 32 + i / VR, i % VR)) = v[x];
+    }
+    fence_async_shared();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -282,153 +365,123 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   griddep_launch();
 
   const int ctx = context_of(a.batch, a.kv, tile.b, a.status);
-  const int rows = min(kPfRows, tile.n * group - tile.row0);
-  const int halves = rows > kPfHalf ? 2 : 1;
+  const int groups = (rows + kGroup - 1) / kGroup;
   const int pos0 = ctx - tile.n;
   const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;
   // key tiles: the sinks' that lie before the window's first, then the window's
   const int lo = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
-  const int t_lo = lo / kPfHalf;
-  const int sink_tiles = min((min(a.sinks, lo) + kPfHalf - 1) / kPfHalf, t_lo);
-  const int all = pmax < 0 ? 0 : sink_tiles + pmax / kPfHalf - t_lo + 1;
+  const int t_lo = lo / T;
+  const int sink_tiles = min((min(a.sinks, lo) + T - 1) / T, t_lo);
+  const int all = pmax < 0 ? 0 : sink_tiles + pmax / T - t_lo + 1;
   const int i0 = (int)((long long)all * rank / ranks), i1 = (int)((long long)all * (rank + 1) / ranks);
   const int n = i1 - i0;  // of this CTA
   auto base_of = [&](int i) {
     i += i0;
-    return (i < sink_tiles ? i : i - sink_tiles + t_lo) * kPfHalf;
+    return (i < sink_tiles ? i : i - sink_tiles + t_lo) * T;
   };
   auto some_row_sees = [&](int j) {
     return j <= pmax && (a.window == 0 || j > pmin - a.window || j < a.sinks);
   };
   auto is_edge = [&](int base) {  // not every row sees every key of the tile
-    return base + kPfHalf - 1 > pmin ||
-           (a.window > 0 && base <= pmax - a.window && base + kPfHalf > a.sinks);
+    return base + T - 1 > pmin ||
+           (a.window > 0 && base <= pmax - a.window && base + T > a.sinks);
   };
 
-  if (warp < 8) {
+  if (warp < S::kRowWarps) {
     // ---------------- rows ----------------
-    // a row of S is 128 registers: 8 warps x 208 + 4 x 88 = 12 x 168 of launch
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int half = warp >> 2, r = half * kPfHalf + (warp & 3) * 32 + lane;
-    const int row = tile.row0 + min(r, rows - 1);
-    const int token = tile.first + row / group, head = kvh * group + row % group;
-    const int pos = pos0 + row / group;
-    {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
-      const uint4* mine = reinterpret_cast<const uint4*>(a.q + (long long)token * a.q_row + (long long)head * D);
-      const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(mine) : 0ull;
-      constexpr int VR = D / 8;
-      uint4 v[VR];
-#pragma unroll
-      for (int x = 0; x < VR; ++x) {  // side by side: 32 vectors of the warp's rows a step
-        const int i = 32 * x + lane;
-        const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
-        v[x] = src != nullptr ? src[i % VR] : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int x = 0; x < VR; ++x) {
-        const int i = 32 * x + lane;
-        *reinterpret_cast<uint4*>(smem + half * S::kTile + sw64_at<D>((warp & 3) * 32 + i / VR, i % VR)) = v[x];
-      }
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st.q_ready);
-    }
-    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_at = lane_addr + kTmemS + half * 128, o_at = lane_addr + kTmemO + half * 128;
+    // a row of 128 keys is 128 registers: 8 warps x 208 + 4 x 88 = 12 x 168 of launch
+    if constexpr (NG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int g = warp >> 2, quarter = warp & 3, r = warp * 32 + lane;
+    const int pos = pos0 + (tile.row0 + min(r, rows - 1)) / group;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_at = lane_addr + g * T, o_at = lane_addr + S::kTmemO + g * D;
     const float scale2 = a.scale * kLog2e;
     const float growth = kGrowth / scale2;
     float m = -INFINITY, l = 0.f;
     uint32_t poison[S::kSlabs];
 #pragma unroll
     for (int i = 0; i < S::kSlabs; ++i) poison[i] = 0;
-    bool ok = half < halves;
-    const bool busy = ok;
-    for (int i = 0; ok && i < n; ++i) {
-      if (!wait_asleep(&st.s_full[half], i & 1, abort_flag, a.status, 60)) {
-        ok = false;
-        break;
-      }
+    const bool busy = g < groups && n > 0;
+    bool ok = true;
+    for (int i = 0; busy && i < n; ++i) {
+      if (!(ok = wait_asleep(&st.s_full[g], i & 1, abort_flag, a.status, 60))) break;
       tc_fence_after();
-      uint32_t s[4][32];
+      constexpr int NC = T / 32;
+      uint32_t s[NC][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32_async(s_at + 32 * c, s[c]);
+      for (int c = 0; c < NC; ++c) tmem_ld32_async(s_at + 32 * c, s[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+      for (int c = 0; c < NC; ++c) tmem_wait_ld(s[c]);
       const int base = base_of(i);
       const bool edge = is_edge(base);
       if (edge) {
-        const int hi = pos - base;  // keys [lo, hi] and [0, sk) of the tile
-        const int low = a.window > 0 ? hi - a.window + 1 : -0x7fffffff, sk = a.sinks - base;
+        // bit k of a word: the row sees key 32 c + k of the tile
+        const int hi = pos - base;  // keys up to hi, and from low or before sk
+        const int low = a.window > 0 ? hi - a.window + 1 : 0, sk = a.sinks - base;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < NC; ++c) {
+          const uint32_t seen = low_bits(hi + 1 - 32 * c) & (~low_bits(low - 32 * c) | low_bits(sk - 32 * c));
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int k = 32 * c + j;
-            // no short circuits: they would become branches
-            s[c][j] = (int)(k <= hi) & ((int)(k >= low) | (int)(k < sk)) ? s[c][j] : 0xff800000u;
-          }
+          for (int k = 0; k < 32; ++k) s[c][k] = seen >> k & 1 ? s[c][k] : 0xff800000u;
+        }
       }
-      float mx[4];
+      float mx[NC];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < NC; ++c) {
         mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int j = 2; j < 32; j += 2)
-          mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])));
+        for (int k = 2; k < 32; k += 2)
+          mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      float top = mx[0];
+#pragma unroll
+      for (int c = 1; c < NC; ++c) top = fmaxf(top, mx[c]);
       const bool move = top > m + growth || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, move)) {
         const float corr = move ? exp2_fast((m - top) * scale2) : 1.f;
         if (move) m = top;
         l *= corr;
         if (i > 0) {  // the previous product is complete: S was issued after it
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_at + 16 * c, o);
 #pragma unroll
-          for (int c = 0; c < S::kSlabs; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_at + 32 * c, o);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-            tmem_st32(o_at + 32 * c, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+            tmem_st16(o_at + 16 * c, o);
           }
         }
       }
       const float off = m == -INFINITY ? 0.f : -m * scale2;
       const float2 scale_2 = make_float2(scale2, scale2), off_2 = make_float2(off, off);
-      float2 sum[4];
+      float2 sum[4] = {make_float2(l, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.f, 0.f);
+      for (int c = 0; c < NC; ++c) {
+        uint32_t p[16];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const uint32_t* src = s[2 * c + (j >> 4)];
-          float2 x = make_float2(__uint_as_float(src[2 * (j & 15)]), __uint_as_float(src[2 * (j & 15) + 1]));
+        for (int k = 0; k < 16; ++k) {
+          float2 x = make_float2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
           x = __ffma2_rn(x, scale_2, off_2);
           x.x = exp2_fast(x.x);
           x.y = exp2_fast(x.y);
-          sum[j & 3] = __fadd2_rn(sum[j & 3], x);
-          p[j] = pack_bf16x2(x.x, x.y);
+          sum[k & 3] = __fadd2_rn(sum[k & 3], x);
+          p[k] = pack_bf16x2(x.x, x.y);
         }
-        tmem_st32(s_at + 32 * c, p);
+        tmem_st16(s_at + 16 * c, p);
       }
       sum[0] = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
-      l += sum[0].x + sum[0].y;
+      l = sum[0].x + sum[0].y;
       tmem_wait_st();
       if (edge) {
         // was a value taken out of the tile that this row sees?
         const int stage = i % NS;
         uint64_t* full = SEP ? &st.v_full[stage] : &st.k_full[stage];
-        if (!wait_asleep(full, (i / NS) & 1, abort_flag, a.status, 61)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = wait_asleep(full, (i / NS) & 1, abort_flag, a.status, 61))) break;
         if (*reinterpret_cast<volatile int*>(&st.bad[stage])) {
-          for (int k = 0; k < kPfHalf; ++k) {
-            const int j = base + k;
-            if (j <= pos && (a.window == 0 || pos - j < a.window || j < a.sinks)) {
-              const uint4 w = bad_cols[stage * kPfHalf + k];
+          for (int k = 0; k < T; ++k) {
+            const int key = base + k;
+            if (key <= pos && (a.window == 0 || pos - key < a.window || key < a.sinks)) {
+              const uint4 w = bad_cols[stage * T + k];
               const uint32_t b[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
               for (int c = 0; c < S::kSlabs; ++c) poison[c] |= b[c];
@@ -438,30 +491,30 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&st.p_ready[half]);
+      if (lane == 0) mbar_arrive(&st.p_ready[g]);
     }
     // ---------------- result ----------------
-    for (int h = 0; ok && n > 0 && h < halves; ++h)
-      ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62);
+    // a CTA's result for the cluster lies over all groups' tiles
+    for (int h = 0; h < groups && n > 0; ++h)
+      if (h == g || ranks > 1) ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62) && ok;
     tc_fence_after();
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    __nv_bfloat16* out = a.out + ((long long)token * a.heads + head) * D;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
     float* part = reinterpret_cast<float*>(smem);
+    unsigned char* own = smem + g * S::kQGroup;  // the warp's rows, bf16, where Q was
 #pragma unroll
     for (int c = 0; c < S::kSlabs; ++c) {
       uint32_t o[32];
-      if (busy && n > 0) {
+      if (busy) {
         tmem_ld32(o_at + 32 * c, o);
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = 0;
+        for (int k = 0; k < 32; ++k) o[k] = 0;
       }
       if (poison[c]) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (poison[c] >> j & 1) o[j] = 0x7fc00000u;
+        for (int k = 0; k < 32; ++k)
+          if (poison[c] >> k & 1) o[k] = 0x7fc00000u;
       }
-      if (!ok || r >= rows) continue;
       if (ranks == 1) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -470,9 +523,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           w.y = pack_bf16x2(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
           w.z = pack_bf16x2(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
           w.w = pack_bf16x2(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
-          reinterpret_cast<uint4*>(out)[c * 4 + v] = w;
+          *reinterpret_cast<uint4*>(own + sw64_at<kGroup>(r & (kGroup - 1), c * 4 + v)) = w;
         }
-      } else {
+      } else if (n > 0) {
         // rows of D floats, 16-byte vectors exchanged by the row's low bits so
         // that the lanes' stores fall in different banks
 #pragma unroll
@@ -481,21 +534,35 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
       }
     }
+    if (ranks == 1) {
+      const int row = tile.row0 + min(r, rows - 1);
+      __nv_bfloat16* out = a.out + ((long long)(tile.first + row / group) * a.heads +
+                                    kvh * group + row % group) * D;
+      const unsigned long long at = ok && r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
+      constexpr int VR = D / 8;
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < VR; ++x) {
+        const int i = 32 * x + lane;
+        uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
+        if (dst != nullptr) dst[i % VR] = *reinterpret_cast<const uint4*>(own + sw64_at<kGroup>(quarter * 32 + i / VR, i % VR));
+      }
+    }
     st.m[r] = m * scale2;
     st.l[r] = l;
-    finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks);
+    finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks, 32 * S::kRowWarps);
     return;
   }
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp < 8 + kLoadWarps) {
+  if constexpr (NG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp < S::kRowWarps + kLoadWarps) {
     // ---------------- keys and values ----------------
-    const int lt = threadIdx.x - 256;  // 0 .. 95
+    const int lt = threadIdx.x - 32 * S::kRowWarps;  // 0 .. 95
     uint32_t raw_phase = 0;            // a bit per stage
     if constexpr (!E4M3) {
-      if (warp == 8) {
+      if (warp == S::kRowWarps) {
         bool ok = true;
-        const int box = min(1 << a.kv.page_shift, kPfHalf);  // rows of a TMA box
-        const int pieces = kPfHalf / box;
+        const int box = paged_box_rows(D, 1 << a.kv.page_shift);
+        const int pieces = T / box;
         const int beyond = a.kv.pages * a.kv.kv_heads << a.kv.page_shift;  // past the pool: zeros
         for (int i = 0; ok && i < n; ++i) {
           const int s = i % NS;
@@ -550,7 +617,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         __syncwarp();
       } else {
-        // warps 9-10: the edge tiles' values
+        // the other two warps: the edge tiles' values
         const int ct = lt - 32;
         for (int i = 0; i < n; ++i) {
           const int base = base_of(i);
@@ -561,13 +628,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           raw_phase ^= 1u << s;
           unsigned char* tile_p = smem + S::kQ + (S::kSides - 1) * S::kRing + s * S::kTile;
           bool any = false;
-          for (int k = ct; k < kPfHalf; k += 64) {
+          for (int k = ct; k < T; k += 64) {
             const bool seen = some_row_sees(base + k);
             uint32_t cols[4] = {0, 0, 0, 0};
             bool row_bad = false;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
-              uint4* p = reinterpret_cast<uint4*>(tile_p + sw64_at<D>(k, c));
+              uint4* p = reinterpret_cast<uint4*>(tile_p + sw64_at<T>(k, c));
               if (!seen) {
                 *p = make_uint4(0, 0, 0, 0);
                 continue;
@@ -586,7 +653,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             }
             // a latent's key is its value: a row that sees it has no score left
             if (!SEP && row_bad) cols[0] = cols[1] = cols[2] = cols[3] = 0xffffffffu;
-            bad_cols[s * kPfHalf + k] = make_uint4(cols[0], cols[1], cols[2], cols[3]);
+            bad_cols[s * T + k] = make_uint4(cols[0], cols[1], cols[2], cols[3]);
             any |= row_bad;
           }
           fence_async_shared();
@@ -599,7 +666,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
     } else {
       constexpr int VR = D / 16;                           // 16-byte vectors of a raw row
-      constexpr int kPer = (kPfHalf * VR + 95) / 96;       // of a thread
+      constexpr int kPer = (T * VR + 95) / 96;       // of a thread
       bool ok = true;
       uint4 raw[kPer];
       auto fetch = [&](const void* pool) {
@@ -607,7 +674,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int x = 0; x < kPer; ++x) {
           const int v = lt + 96 * x;
           raw[x] = make_uint4(0, 0, 0, 0);
-          if (v < kPfHalf * VR) {
+          if (v < T * VR) {
             const int k = v / VR, c = v - k * VR, at = st.row[k];
             if (at >= 0) raw[x] = reinterpret_cast<const uint4*>(pool)[(long long)at * VR + c];
           }
@@ -618,7 +685,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
           const int v = lt + 96 * x;
-          if (v < kPfHalf * VR) {
+          if (v < T * VR) {
             const int k = v / VR, c = v - k * VR;
             const uint32_t s2 = scale_pair(st.scale[k] >> shift & 0xff);
             const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
@@ -631,7 +698,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                 if (bits) {
                   any = true;
                   const int c8 = 2 * c + h;
-                  uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * kPfHalf + k);
+                  uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * T + k);
                   if (SEP) {
                     atomicOr(cols + (c8 >> 2), bits << (8 * (c8 & 3)));
                   } else {
@@ -643,7 +710,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                   o.w &= keep_mask(bits, 3);
                 }
               }
-              *reinterpret_cast<uint4*>(dst + sw64_at<D>(k, 2 * c + h)) = o;
+              *reinterpret_cast<uint4*>(dst + sw64_at<T>(k, 2 * c + h)) = o;
             }
           }
         }
@@ -652,7 +719,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       for (int i = 0; ok && i < n; ++i) {
         const int s = i % NS, base = base_of(i);
         const bool edge = is_edge(base);
-        for (int k = lt; k < kPfHalf; k += 96) {
+        for (int k = lt; k < T; k += 96) {
           const int j = base + k;
           int at = -1;
           if (some_row_sees(j)) {
@@ -672,7 +739,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           if (!ok) break;
           const bool check = edge && side == S::kSides - 1;
           if (check)
-            for (int k = lt; k < kPfHalf; k += 96) bad_cols[s * kPfHalf + k] = make_uint4(0, 0, 0, 0);
+            for (int k = lt; k < T; k += 96) bad_cols[s * T + k] = make_uint4(0, 0, 0, 0);
           if (check) named_sync(1, 96);
           const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, 8 * side, s, check);
           fence_async_shared();
@@ -684,59 +751,59 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == S::kMmaWarp) {
     // ---------------- matrix instructions ----------------
-    if (lane == 0 && n > 0) {
-      const uint32_t id_s = make_idesc(kPfHalf, kPfHalf);
-      const uint32_t id_o = make_idesc(kPfHalf, D) | (1u << 16);  // V: columns contiguous
-      bool ok = wait_asleep(&st.q_ready, 0, abort_flag, a.status, 65);
+    if (n > 0) {
+      const uint32_t leader = elect_one();
+      const uint32_t id_s = make_idesc(kGroup, T);
+      const uint32_t id_o = make_idesc(kGroup, D) | (1u << 16);  // V: columns contiguous
+      bool ok = true;
       auto scores = [&](int h, int s) {
-        const uint64_t qd = sw64_desc(q_u + h * S::kTile, 16), kd = sw64_desc(k_u + s * S::kTile, 16);
+        const uint32_t qd = sw64_lo(q_u + h * S::kQGroup, 16), kd = sw64_lo(k_u + s * S::kTile, 16);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 1) * S::kSlab + (k & 1) * 32) >> 4;
-          mma_bf16(tmem + kTmemS + h * 128, qd + off, kd + off, id_s, k != 0);
-        }
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(tmem + h * T, qd + ((uint32_t)((k >> 1) * S::kQSlab + (k & 1) * 32) >> 4),
+                 kd + ((uint32_t)((k >> 1) * S::kSlab + (k & 1) * 32) >> 4), id_s, k != 0, leader);
       };
       auto values = [&](int h, int s, uint32_t accumulate) {
-        const uint64_t vd = sw64_desc(v_u + s * S::kTile, S::kSlab);
+        const uint32_t vd = sw64_lo(v_u + s * S::kTile, S::kSlab);
 #pragma unroll
-        for (int k = 0; k < kPfHalf / 16; ++k)
-          mma_bf16_ts(tmem + kTmemO + h * 128, tmem + kTmemS + h * 128 + k * 8,
-                      vd + (uint32_t)(k * 1024 >> 4), id_o, accumulate | (k != 0));
+        for (int k = 0; k < T / 16; ++k)
+          mma_ts(tmem + S::kTmemO + h * D, tmem + h * T + k * 8, vd + (uint32_t)(k * 1024 >> 4), id_o,
+                 k == 0 ? accumulate : 1u, leader);
       };
-      if (ok && (ok = wait_asleep(&st.k_full[0], 0, abort_flag, a.status, 66))) {
+      if ((ok = wait_asleep(&st.k_full[0], 0, abort_flag, a.status, 66))) {
         tc_fence_after();
-        for (int h = 0; h < halves; ++h) {
+        for (int h = 0; h < groups; ++h) {
           scores(h, 0);
-          mma_commit(&st.s_full[h]);
+          commit_to(&st.s_full[h], leader);
         }
-        if (SEP) mma_commit(&st.k_empty[0]);
+        if (SEP) commit_to(&st.k_empty[0], leader);
       }
-      // The thread issues at the tensor core's pace, so what it does between
-      // the products is time lost: copies are waited for ahead of the rows.
+      // Copies are waited for ahead of the rows: what this warp does between a
+      // group's P and its next scores is time that group waits.
       for (int i = 0; ok && i < n; ++i) {
         const int s = i % NS, s1 = (i + 1) % NS;
         const bool more = i + 1 < n;
         if (SEP && !(ok = wait_asleep(&st.v_full[s], (i / NS) & 1, abort_flag, a.status, 67))) break;
         if (more && !(ok = wait_asleep(&st.k_full[s1], ((i + 1) / NS) & 1, abort_flag, a.status, 66))) break;
-        for (int h = 0; h < halves; ++h) {
+        for (int h = 0; h < groups; ++h) {
           if (!(ok = wait_asleep(&st.p_ready[h], i & 1, abort_flag, a.status, 68))) break;
           tc_fence_after();
           values(h, s, i > 0);
           if (more) {
             scores(h, s1);
-            mma_commit(&st.s_full[h]);
+            commit_to(&st.s_full[h], leader);
           } else {
-            mma_commit(&st.o_done[h]);
+            commit_to(&st.o_done[h], leader);
           }
         }
         if (!ok) break;
-        mma_commit(SEP ? &st.v_empty[s] : &st.k_empty[s]);
-        if (SEP && more) mma_commit(&st.k_empty[s1]);
+        commit_to(SEP ? &st.v_empty[s] : &st.k_empty[s], leader);
+        if (SEP && more) commit_to(&st.k_empty[s1], leader);
       }
       // all matrix instructions have finished before TMEM is freed
-      mma_commit(&st.drain);
+      commit_to(&st.drain, leader);
       mbar_drain(&st.drain, 0);
     }
     __syncwarp();
@@ -747,7 +814,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   tc_fence_after();
   // freed before the cluster waits: a CTA that waits for TMEM on this SM may
   // be the one that a peer of this cluster waits behind
-  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+  if (warp == S::kMmaWarp) tmem_dealloc(tmem, 512);
   if (ranks > 1) {
     cluster_sync();
     cluster_sync();
@@ -762,8 +829,8 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   using S = PrefillShape<D, SEP>;
   auto k = paged_prefill_kernel<D, E4M3, SEP>;
   const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
-  const long long tiles = std::min(n * ((group + kPfRows - 1) / kPfRows),
-                                   n * group / kPfRows + std::min<long long>(a.batch.batch, n));
+  const long long tiles = std::min(n * ((group + S::kRows - 1) / S::kRows),
+                                   n * group / S::kRows + std::min<long long>(a.batch.batch, n));
   // CTAs per tile while the GPU has SMs to spare
   int ranks = 1;
   while (ranks < kMaxRanks && 2 * ranks * tiles * a.kv.kv_heads <= sms) ranks *= 2;
@@ -773,7 +840,7 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
     return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);
-  cfg.blockDim = dim3(kPfThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -798,6 +865,8 @@ int launch_prefill_d(const PagedAttnArgs& a, const CUtensorMap& k, const CUtenso
 }
 
 }  // namespace
+
+int paged_prefill_box_rows(int head_dim, int page_size) { return paged_box_rows(head_dim, page_size); }
 
 int launch_paged_prefill(const PagedAttnArgs& a, const CUtensorMap& k_map,
                          const CUtensorMap& v_map, int sms, cudaStream_t stream) {
