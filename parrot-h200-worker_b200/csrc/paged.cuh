@@ -86,16 +86,19 @@ __device__ __forceinline__ int sequence_of(const PagedBatch& s, int i) {
   return lo;
 }
 
-// Keys of sequence b that the table can hold.
-__device__ __forceinline__ int context_of(const PagedBatch& s, const PagedKV& kv, int b,
-                                          int* status) {
-  const int n = s.context_len[b];
+// A context length as given, at most what the table can hold.
+__device__ __forceinline__ int clamp_context(const PagedBatch& s, const PagedKV& kv, int n,
+                                             int* status) {
   const long long most = (long long)s.table_width << kv.page_shift;
   if (n > most) {
     report_status(status, kStatusBadIndex, 51, n);
     return (int)most;
   }
   return max(n, 0);
+}
+__device__ __forceinline__ int context_of(const PagedBatch& s, const PagedKV& kv, int b,
+                                          int* status) {
+  return clamp_context(s, kv, s.context_len[b], status);
 }
 
 // Page of position p of sequence b; -1 (reported) if the table names none.

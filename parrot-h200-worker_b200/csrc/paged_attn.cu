@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
   griddep_launch();
   const Tile tile = find_tile(a.batch, group, kDecRows, blockIdx.x / ranks);
   if (tile.b < 0) return;  // the whole cluster
-  const int n = context_of(a.batch, a.kv, tile.b, a.status);
+  const int n = clamp_context(a.batch, a.kv, tile.ctx, a.status);
   const int rows = min(kDecRows, tile.n * group - tile.row0);
   const int pos0 = n - tile.n;  // position of the sequence's first batch row
   const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;

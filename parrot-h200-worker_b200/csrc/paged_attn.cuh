@@ -20,6 +20,7 @@ struct Tile {
   int first;       // batch row of the sequence's first token
   int n;           // its tokens in the batch
   int row0;        // first (token, head) row of the tile
+  int ctx;         // its context length, as given
 };
 
 // The tile with this number, sequences in order, ceil(n_b * group / rows_per)
@@ -32,7 +33,7 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int ro
     const int b = b0 + lane;
     int2 r = make_int2(0, 0);
     if (b < s.batch) r = batch_rows(s, b);
-    const int n = r.y - r.x;
+    const int n = r.y - r.x, len = b < s.batch ? s.context_len[b] : 0;
     const int mine = (int)(((long long)n * group + rows_per - 1) / rows_per);
     int upto = mine;
 #pragma unroll
@@ -47,13 +48,53 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int ro
       t.b = b0 + l;
       t.first = __shfl_sync(0xffffffffu, r.x, l);
       t.n = __shfl_sync(0xffffffffu, n, l);
+      t.ctx = __shfl_sync(0xffffffffu, len, l);
       t.row0 = (tile - base - __shfl_sync(0xffffffffu, upto - mine, l)) * rows_per;
       return t;
     }
     base += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return Tile{-1, 0, 0, 0};
+  return Tile{-1, 0, 0, 0, 0};
 }
+
+// As find_tile with the sequences' tiles taken from their ends in turn: all
+// last tiles first, which see the most keys, then those before them, so that
+// what is left to the end of the launch is short.  Up to 32 sequences (above,
+// no tile is a large part of the work, and the order is find_tile's reversed).
+__device__ __forceinline__ Tile find_tile_from_ends(const PagedBatch& s, int group, int rows_per,
+                                                    int index, int most) {
+  if (s.batch > 32) return find_tile(s, group, rows_per, most - 1 - index);
+  const int lane = threadIdx.x & 31;
+  int2 r = make_int2(0, 0);
+  int len = 0;
+  if (lane < s.batch) {
+    r = batch_rows(s, lane);
+    len = s.context_len[lane];
+  }
+  const int n = r.y - r.x;
+  const int tiles = (int)(((long long)n * group + rows_per - 1) / rows_per);
+  if (index >= (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles)) return Tile{-1, 0, 0, 0, 0};
+  // the round: the last one before which at most `index` tiles were taken
+  int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)tiles);
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((int)__reduce_add_sync(0xffffffffu, (unsigned)min(tiles, mid)) <= index) lo = mid;
+    else hi = mid;
+  }
+  const int left = index - (int)__reduce_add_sync(0xffffffffu, (unsigned)min(tiles, lo));
+  const unsigned open = __ballot_sync(0xffffffffu, tiles > lo);
+  const unsigned before = open & ((1u << lane) - 1u);
+  const unsigned hit = __ballot_sync(0xffffffffu, (open >> lane & 1) && __popc(before) == left);
+  const int l = __ffs(hit) - 1;
+  Tile t;
+  t.b = l;
+  t.first = __shfl_sync(0xffffffffu, r.x, l);
+  t.n = __shfl_sync(0xffffffffu, n, l);
+  t.ctx = __shfl_sync(0xffffffffu, len, l);
+  t.row0 = (__shfl_sync(0xffffffffu, tiles, l) - 1 - lo) * rows_per;
+  return t;
+}
+
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;

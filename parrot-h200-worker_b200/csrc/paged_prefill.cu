@@ -91,6 +91,7 @@ struct PrefillState {
   uint32_t armed_parity[2][6];
   int row[128];                // e4m3: pool row of each key of the tile, -1: zeros
   uint32_t scale[128];         // its scale bytes (key, value)
+  uint4 poison[kGroup * kMaxGroups];
   float m[kGroup * kMaxGroups], l[kGroup * kMaxGroups];  // merge
 };
 
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
   uint4* bad_cols = reinterpret_cast<uint4*>(smem + S::kQ + S::kSides * S::kRing);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ranks = a.cluster, rank = blockIdx.x % ranks;
-  const int kvh = blockIdx.y, group = a.heads / a.kv.kv_heads;
+  const int kvh = blockIdx.x / ranks % a.kv.kv_heads, group = a.heads / a.kv.kv_heads;
   volatile int* abort_flag = &st.abort;
 
   if (threadIdx.x == 0) {
@@ -328,13 +329,14 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
+  __syncthreads();
   griddep_wait();
-  // tiles in reverse: a long sequence's last tiles see the most keys
-  const Tile tile =
-      find_tile(a.batch, group, R, gridDim.x / ranks - 1 - blockIdx.x / ranks);
+  const Tile tile = find_tile_from_ends(a.batch, group, R, blockIdx.x / (ranks * a.kv.kv_heads),
+                                        gridDim.x / (ranks * a.kv.kv_heads));
   if (tile.b < 0) return;  // the whole cluster, before any wait
-  if (warp == S::kMmaWarp) tmem_alloc(&st.tmem, 512);
   const int rows = min(R, tile.n * group - tile.row0);
+  const bool loads = warp >= S::kRowWarps && warp < S::kMmaWarp;  // these need neither Q nor TMEM
+  if (warp == S::kMmaWarp) tmem_alloc(&st.tmem, 512);
   if (warp < S::kRowWarps) {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
     const int r = warp * 32 + lane, row = tile.row0 + r, head = kvh * group + row % group;
     const uint4* mine = reinterpret_cast<const uint4*>(
@@ -356,15 +358,17 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     }
     fence_async_shared();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  if (!loads) {
+    tc_fence_before();
+    named_sync(2, 32 * (S::kRowWarps + 1));
+    tc_fence_after();
+  }
   const uint32_t tmem = st.tmem;
   // not before: a kernel launched early may want TMEM, and holds it until this
   // one has finished
-  griddep_launch();
+  if (!loads) griddep_launch();
 
-  const int ctx = context_of(a.batch, a.kv, tile.b, a.status);
+  const int ctx = clamp_context(a.batch, a.kv, tile.ctx, a.status);
   const int groups = (rows + kGroup - 1) / kGroup;
   const int pos0 = ctx - tile.n;
   const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;
@@ -398,9 +402,7 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     const float scale2 = a.scale * kLog2e;
     const float growth = kGrowth / scale2;
     float m = -INFINITY, l = 0.f;
-    uint32_t poison[S::kSlabs];
-#pragma unroll
-    for (int i = 0; i < S::kSlabs; ++i) poison[i] = 0;
+    bool poison = false;  // st.poison[r]: the columns that are NaN
     const bool busy = g < groups && n > 0;
     bool ok = true;
     for (int i = 0; busy && i < n; ++i) {
@@ -478,15 +480,19 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         uint64_t* full = SEP ? &st.v_full[stage] : &st.k_full[stage];
         if (!(ok = wait_asleep(full, (i / NS) & 1, abort_flag, a.status, 61))) break;
         if (*reinterpret_cast<volatile int*>(&st.bad[stage])) {
+          uint4 cols = poison ? st.poison[r] : make_uint4(0, 0, 0, 0);
           for (int k = 0; k < T; ++k) {
             const int key = base + k;
             if (key <= pos && (a.window == 0 || pos - key < a.window || key < a.sinks)) {
               const uint4 w = bad_cols[stage * T + k];
-              const uint32_t b[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int c = 0; c < S::kSlabs; ++c) poison[c] |= b[c];
+              cols.x |= w.x;
+              cols.y |= w.y;
+              cols.z |= w.z;
+              cols.w |= w.w;
             }
           }
+          st.poison[r] = cols;
+          poison = true;
         }
       }
       tc_fence_before();
@@ -501,7 +507,9 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
     float* part = reinterpret_cast<float*>(smem);
     unsigned char* own = smem + g * S::kQGroup;  // the warp's rows, bf16, where Q was
-#pragma unroll
+    // loops, not straight lines: this runs once, and fetching its instructions
+    // is much of what it costs
+#pragma unroll 1
     for (int c = 0; c < S::kSlabs; ++c) {
       uint32_t o[32];
       if (busy) {
@@ -510,10 +518,11 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = 0;
       }
-      if (poison[c]) {
+      if (poison) {
+        const uint32_t cols = reinterpret_cast<const uint32_t*>(&st.poison[r])[c];
 #pragma unroll
         for (int k = 0; k < 32; ++k)
-          if (poison[c] >> k & 1) o[k] = 0x7fc00000u;
+          if (cols >> k & 1) o[k] = 0x7fc00000u;
       }
       if (ranks == 1) {
 #pragma unroll
@@ -541,7 +550,7 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
       const unsigned long long at = ok && r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
       constexpr int VR = D / 8;
       __syncwarp();
-#pragma unroll
+#pragma unroll 4
       for (int x = 0; x < VR; ++x) {
         const int i = 32 * x + lane;
         uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
@@ -835,11 +844,11 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   int ranks = 1;
   while (ranks < kMaxRanks && 2 * ranks * tiles * a.kv.kv_heads <= sms) ranks *= 2;
   a.cluster = ranks;
-  if (tiles * ranks > 0x7fffffffll) return -1;
+  if (tiles * ranks * a.kv.kv_heads > 0x7fffffffll) return -1;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
     return -2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);
+  cfg.gridDim = dim3((unsigned)(tiles * ranks * a.kv.kv_heads));
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
