@@ -43,15 +43,22 @@ __device__ __forceinline__ uint32_t scale_pair(int byte) {  // 2^(byte - 127) tw
   const uint32_t one = (uint32_t)byte << 7;
   return one | (one << 16);
 }
+__device__ __forceinline__ uint2 e4m3x4_numbers(uint32_t w);
 __device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t w, uint32_t scale2) {
+  uint2 r = e4m3x4_numbers(w);
+  r.x = mul_bf16x2_exact(r.x, scale2);
+  r.y = mul_bf16x2_exact(r.y, scale2);
+  return r;
+}
+__device__ __forceinline__ uint2 e4m3x4_numbers(uint32_t w) {
   constexpr uint32_t k2p120 = ((120u + 127u) << 7) * 0x10001u;
   // bytes (0, 1) and (2, 3) into the upper bytes of the halves of a register
   const uint32_t lo = __byte_perm(w, 0, 0x1404), hi = __byte_perm(w, 0, 0x3424);
   uint2 r;
   uint32_t a = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
   uint32_t b = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
-  a = mul_bf16x2_exact(mul_bf16x2_exact(a, k2p120), scale2);
-  b = mul_bf16x2_exact(mul_bf16x2_exact(b, k2p120), scale2);
+  a = mul_bf16x2_exact(a, k2p120);
+  b = mul_bf16x2_exact(b, k2p120);
   // any byte 0x7f / 0xff?  (w | 0x80..) == 0xff per byte
   const uint32_t nan = __vcmpeq4(w | 0x80808080u, 0xffffffffu);
   if (nan) {

@@ -45,6 +45,27 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same with f16 operands
+__device__ __forceinline__ void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two e4m3 numbers as a pair of f16, exact (NaN stays NaN)
+__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t w) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)w));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) != 0x7f80u; }
 
 // ---------------------------------------------------------------------------
@@ -58,6 +79,15 @@ __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) !
 // own running maximum, sum and fp32 weighted values.  The warps' results are
 // merged in shared memory, the CTAs' over distributed shared memory, in a
 // fixed order: no workspace, no second launch, no atomics.
+//
+// An e4m3 cache halves the bytes, and widening them becomes what counts.  Keys
+// go from memory to the product's registers: a thread's 8 bytes of a key are
+// its share of two products when the query's columns are permuted alike, and
+// the conversion to f16 is one instruction for two (the query goes to f16 with
+// a power of two per row that puts its largest magnitude at 2^8, so what f16
+// loses is below 2^-32 of that).  The scales multiply the scores' columns, and
+// for the values the probabilities, as powers of two exactly.  Values pass
+// through shared memory as bf16 for the transposed load.
 // ---------------------------------------------------------------------------
 constexpr int kDecWarps = 4;
 constexpr int kDecKeys = 32;
@@ -65,23 +95,22 @@ constexpr int kDecRows = 16;
 
 template <int D, bool E4M3, bool SEP>
 struct DecodeShape {
-  static constexpr int kStages = E4M3 ? 3 : 2;
+  static constexpr int kStages = 2;
   // bf16 rows are padded by 16 bytes: an odd number of 16-byte units, so the
   // eight rows of a matrix load fall in different banks
   static constexpr int kRow = 2 * D + 16;
   static constexpr int kTile = kDecKeys * kRow;
-  static constexpr int kRaw = kDecKeys * D;
-  static constexpr int kSide = E4M3 ? kRaw : kTile;
+  static constexpr int kSide = kTile;
   static constexpr int kStage = kSide * (SEP ? 2 : 1);
-  // e4m3: a bf16 tile that the chunk's keys, then its values, are expanded to
-  static constexpr int kWarp = kStage * kStages + (E4M3 ? kTile : 0);
+  // e4m3: one bf16 tile that a chunk's values are widened to
+  static constexpr int kWarp = E4M3 ? kTile : kStage * kStages;
   static constexpr int kPart = kDecRows * D * 4 + 2 * kDecRows * 4;  // a CTA's result
   static constexpr int kBytes = kWarp * kDecWarps + kPart;
   static_assert(kWarp >= kPart, "a warp's ring holds its result");
 };
 
 template <int D, bool E4M3, bool SEP>
-__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(32 * kDecWarps, D == 128 ? 2 : 3) paged_decode_kernel(PagedAttnArgs a) {
   using S = DecodeShape<D, E4M3, SEP>;
   constexpr int KS = D / 16;  // k steps of q . k
   constexpr int NT = D / 8;   // column tiles of the output
@@ -102,6 +131,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
   // the two (token, head) rows of this thread in the product's layout
   int pos[2];
   uint32_t qf[KS][4];
+  float row_scale[2];
   const __nv_bfloat16* qrow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -109,12 +139,39 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
     pos[i] = pos0 + r / group;
     qrow[i] = a.q + (long long)(tile.first + r / group) * a.q_row +
               (long long)(kvh * group + r % group) * D;
+    row_scale[i] = a.scale * kLog2e;
   }
+  if constexpr (!E4M3) {
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+    for (int k = 0; k < KS; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      qf[k][j] = *reinterpret_cast<const uint32_t*>(qrow[j & 1] + k * 16 + 2 * t + 8 * (j >> 1));
+      for (int j = 0; j < 4; ++j)
+        qf[k][j] = *reinterpret_cast<const uint32_t*>(qrow[j & 1] + k * 16 + 2 * t + 8 * (j >> 1));
+  } else {
+    // columns 32 b + 8 t .. + 7 are this thread's of products 2 b and 2 b + 1
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float amax = 0.f;
+      float f[KS / 2][8];
+#pragma unroll
+      for (int b = 0; b < KS / 2; ++b) {
+        bf16x8_to_float(*reinterpret_cast<const uint4*>(qrow[i] + 32 * b + 8 * t), f[b]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[b][e]));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // 2^(8 - exponent of amax), within fp32's normal powers
+      const int ex = amax > 0.f ? min(max((int)(__float_as_uint(amax) >> 23) - 127, -110), 120) : 8;
+      const float up = pow2(8 - ex);
+      row_scale[i] *= pow2(ex - 8);
+#pragma unroll
+      for (int b = 0; b < KS / 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          qf[2 * b + (e >> 1)][i + 2 * (e & 1)] = pack_f16x2(f[b][2 * e] * up, f[b][2 * e + 1] * up);
+    }
+  }
 
   // chunks: those of the sinks that lie before the window's first, then the
   // window's; key base of chunk c
@@ -127,10 +184,6 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
 
   unsigned char* ring = dec_smem + warp * S::kWarp;
   const uint32_t ring_u = tc::smem_u32(ring);
-  const uint32_t wide_u = ring_u + S::kStage * S::kStages;
-  uint32_t sc[S::kStages];  // e4m3: this lane's key's two scale bytes, per stage
-#pragma unroll
-  for (int i = 0; i < S::kStages; ++i) sc[i] = 0;
   // the page of this lane's key of a chunk, -1 where nobody of the tile sees it
   auto page_for = [&](int c) {
     if (c >= chunks) return -1;
@@ -138,28 +191,51 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
     const bool seen = j <= pmax && (a.window == 0 || j > pmin - a.window || j < a.sinks);
     return seen ? page_of(a.batch, a.kv, tile.b, j, a.status) : -1;
   };
-  // start the copies of chunk c into a stage; keys nobody sees become zeros
-  auto fetch = [&](int c, int page, uint32_t stage, uint32_t& scales) {
+  // bf16: start the copies of chunk c into a stage; keys nobody sees become zeros
+  auto fetch = [&](int c, int page, uint32_t stage) {
     if (c < chunks) {
-      const int j = base_of(c) + lane;
-      const int row = page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, j);
-      if constexpr (E4M3) {
-        scales = row < 0 ? 0u
-                         : (uint32_t)a.kv.key_scale[row] |
-                               (SEP ? (uint32_t)a.kv.value_scale[row] << 8 : 0u);
-      }
-      constexpr int VR = E4M3 ? D / 16 : D / 8;  // 16-byte vectors of a row
+      const int row = page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, base_of(c) + lane);
+      constexpr int VR = D / 8;  // 16-byte vectors of a row
 #pragma unroll
       for (int i = 0; i < VR; ++i) {
         const int v = lane + 32 * i, r = v / VR, cv = v - r * VR;
         const int rr = __shfl_sync(0xffffffffu, row, r);
         const long long at = ((long long)max(rr, 0) * VR + cv) * 16;
-        const uint32_t dst = ring_u + stage * S::kStage + r * (E4M3 ? D : S::kRow) + cv * 16;
+        const uint32_t dst = ring_u + stage * S::kStage + r * S::kRow + cv * 16;
         cp_async16_zfill(dst, static_cast<const char*>(a.kv.key) + at, rr >= 0);
         if (SEP) cp_async16_zfill(dst + S::kSide, static_cast<const char*>(a.kv.value) + at, rr >= 0);
       }
     }
     cp_async_commit();
+  };
+  // e4m3: chunk c into registers: this thread's keys (8 t .. 8 t + 7 of each 32
+  // columns of keys g, g + 8, ...), vectors of the values in memory order, and
+  // the scale bytes of key `lane`; zeros for keys nobody sees
+  constexpr int NB = D / 32, VR8 = D / 16;
+  uint2 kr[E4M3 ? 4 : 1][E4M3 ? NB : 1];
+  uint4 vr[E4M3 ? VR8 : 1];
+  uint32_t scales = 0;
+  auto fetch8 = [&](int c, int page) {
+    if (c >= chunks) return;
+    const int row = page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, base_of(c) + lane);
+    const void* values = SEP ? a.kv.value : a.kv.key;
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      const int rr = __shfl_sync(0xffffffffu, row, nt * 8 + g);
+      const uint2* src = reinterpret_cast<const uint2*>(a.kv.key) + (long long)max(rr, 0) * (D / 8) + t;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) kr[nt][b] = rr < 0 ? make_uint2(0u, 0u) : src[4 * b];
+    }
+#pragma unroll
+    for (int i = 0; i < VR8; ++i) {
+      const int v = lane + 32 * i, r = v / VR8, cv = v - r * VR8;
+      const int rr = __shfl_sync(0xffffffffu, row, r);
+      vr[i] = rr < 0 ? make_uint4(0u, 0u, 0u, 0u)
+                     : reinterpret_cast<const uint4*>(values)[(long long)rr * VR8 + cv];
+    }
+    scales = row < 0 ? (uint32_t)kScaleBias * 0x101u
+                     : (uint32_t)a.kv.key_scale[row] |
+                           (uint32_t)(SEP ? a.kv.value_scale : a.kv.key_scale)[row] << 8;
   };
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -168,74 +244,77 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  const float scale2 = a.scale * kLog2e;
-
-  int c = me;
-#pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s)
-    fetch(c + s * workers, page_for(c + s * workers), s, sc[s]);
-  int next_page = page_for(c + (S::kStages - 1) * workers);
-  int it = 0;
+  int c = me, it = 0;
+  int next_page = -1;
+  if constexpr (E4M3) {
+    fetch8(c, page_for(c));
+    next_page = page_for(c + workers);
+  } else {
+    fetch(c, page_for(c), 0);
+    next_page = page_for(c + workers);
+  }
   for (; c < chunks; c += workers, ++it) {
-    const int slot = it % S::kStages, fill = (it + S::kStages - 1) % S::kStages;
-    uint32_t new_sc = 0;
-    fetch(c + (S::kStages - 1) * workers, next_page, fill, new_sc);
-    if constexpr (E4M3) {
-#pragma unroll
-      for (int s = 0; s < S::kStages; ++s)
-        if (s == fill) sc[s] = new_sc;
-    }
-    next_page = page_for(c + S::kStages * workers);
-    cp_async_wait<S::kStages - 1>();
-    __syncwarp();
-    uint32_t k_u = ring_u + slot * S::kStage, v_u = SEP ? k_u + S::kSide : k_u;
-    uint32_t scales = 0;
-    if constexpr (E4M3) {
-#pragma unroll
-      for (int s = 0; s < S::kStages; ++s)
-        if (s == slot) scales = sc[s];
-    }
-    // a side's 32 rows of e4m3 numbers to bf16 values
-    auto widen = [&](uint32_t raw, int shift) {
-      constexpr int VR = D / 16;
-#pragma unroll
-      for (int i = 0; i < VR; ++i) {
-        const int v = lane + 32 * i, r = v / VR, cv = v - r * VR;
-        const uint32_t s2 = scale_pair((__shfl_sync(0xffffffffu, scales, r) >> shift) & 0xff);
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(raw + v * 16));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint2 x = e4m3x4_to_bf16(w[2 * h], s2), y = e4m3x4_to_bf16(w[2 * h + 1], s2);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(wide_u + r * S::kRow +
-                                                                        cv * 32 + h * 16),
-                       "r"(x.x), "r"(x.y), "r"(y.x), "r"(y.y)
-                       : "memory");
-        }
-      }
-      __syncwarp();
-    };
-    if constexpr (E4M3) {
-      widen(k_u, 0);
-      k_u = wide_u;
-    }
     // scores of the 16 rows and 32 keys
     float s[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    uint32_t v_u = ring_u;
+    float v_scale[4][2];  // of the keys of this thread's columns
+    if constexpr (E4M3) {
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
+      for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-      for (int k2 = 0; k2 < KS / 2; ++k2) {
-        uint32_t b[4];
-        ldmatrix_x4(b, k_u + (nt * 8 + (lane & 7)) * S::kRow + k2 * 64 + (lane >> 3) * 16);
-        mma_16816(s[nt], qf[2 * k2], b[0], b[1]);
-        mma_16816(s[nt], qf[2 * k2 + 1], b[2], b[3]);
+        for (int b = 0; b < NB; ++b) {
+          mma_16816_f16(s[nt], qf[2 * b], e4m3x2_to_f16(kr[nt][b].x), e4m3x2_to_f16(kr[nt][b].x >> 16));
+          mma_16816_f16(s[nt], qf[2 * b + 1], e4m3x2_to_f16(kr[nt][b].y), e4m3x2_to_f16(kr[nt][b].y >> 16));
+        }
+      // the values as bf16 numbers to shared memory
+#pragma unroll
+      for (int i = 0; i < VR8; ++i) {
+        const int v = lane + 32 * i, r = v / VR8, cv = v - r * VR8;
+        const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 x = e4m3x4_numbers(w[2 * h]), y = e4m3x4_numbers(w[2 * h + 1]);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(ring_u + r * S::kRow +
+                                                                        cv * 32 + h * 16),
+                       "r"(x.x), "r"(x.y), "r"(y.x), "r"(y.y)
+                       : "memory");
+        }
       }
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t b = __shfl_sync(0xffffffffu, scales, nt * 8 + 2 * t + e);
+          const float ks = __uint_as_float((b & 0xffu) << 23);
+          v_scale[nt][e] = __uint_as_float((b >> 8 & 0xffu) << 23);
+          s[nt][e] *= ks;
+          s[nt][2 + e] *= ks;
+        }
+      fetch8(c + workers, next_page);
+      next_page = page_for(c + 2 * workers);
+      __syncwarp();
+    } else {
+      const int slot = it & 1;
+      fetch(c + workers, next_page, slot ^ 1);
+      next_page = page_for(c + 2 * workers);
+      cp_async_wait<1>();
+      __syncwarp();
+      const uint32_t k_u = ring_u + slot * S::kStage;
+      v_u = SEP ? k_u + S::kSide : k_u;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int k2 = 0; k2 < KS / 2; ++k2) {
+          uint32_t b[4];
+          ldmatrix_x4(b, k_u + (nt * 8 + (lane & 7)) * S::kRow + k2 * 64 + (lane >> 3) * 16);
+          mma_16816(s[nt], qf[2 * k2], b[0], b[1]);
+          mma_16816(s[nt], qf[2 * k2 + 1], b[2], b[3]);
+        }
+    }
     const int base = base_of(c);
     const bool whole = base + kDecKeys - 1 <= pmin &&
                        (a.window == 0 || base > pmax - a.window || base + kDecKeys <= a.sinks);
@@ -246,7 +325,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
     for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[nt][j] *= scale2;
+        s[nt][j] *= row_scale[j >> 1];
         if (!whole && !sees(j >> 1, base + nt * 8 + 2 * t + (j & 1))) s[nt][j] = -INFINITY;
       }
 #pragma unroll
@@ -275,11 +354,6 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
         o[nt][2 * i + 1] *= corr;
       }
     }
-    if constexpr (E4M3 && SEP) {
-      __syncwarp();  // the keys have been read
-      widen(v_u, 8);
-    }
-    if constexpr (E4M3) v_u = wide_u;
     if (!whole && pmin != pmax) {
       // A value that is not finite would reach, as 0 * NaN in the product, the
       // rows that do not see its key.  Take such numbers out of the tile and add
@@ -339,7 +413,12 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int nt = 2 * kk + (j >> 1);
-        p[j] = tc::pack_bf16x2(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
+        float x = s[nt][2 * (j & 1)], y = s[nt][2 * (j & 1) + 1];
+        if constexpr (E4M3) {  // the values' scales, powers of two
+          x *= v_scale[nt][0];
+          y *= v_scale[nt][1];
+        }
+        p[j] = tc::pack_bf16x2(x, y);
       }
 #pragma unroll
       for (int n2 = 0; n2 < NT / 2; ++n2) {
@@ -439,13 +518,13 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(PagedAttnA
 }
 
 // CTAs per tile: as many as keep every warp two chunks or more of the longest
-// possible context, while the grid stays within about three CTAs per SM.
+// possible context, while the grid stays within about four CTAs per SM.
 int decode_ranks(const PagedAttnArgs& a, long long tiles, int sms) {
   long long keys = (long long)a.batch.table_width << a.kv.page_shift;
   if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
   const long long chunks = (keys + kDecKeys - 1) / kDecKeys;
   int ranks = 1;
-  while (ranks < 8 && chunks >= 4LL * ranks * kDecWarps && tiles * ranks * 2 <= 3LL * sms) ranks *= 2;
+  while (ranks < 8 && chunks >= 4LL * ranks * kDecWarps && tiles * ranks * 2 <= 4LL * sms) ranks *= 2;
   return ranks;
 }
 

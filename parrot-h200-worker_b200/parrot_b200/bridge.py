@@ -755,13 +755,19 @@ class PagedKV:
         if value is not None and (value.shape != key.shape or value.dtype != key.dtype):
             raise ValueError("value must match key in shape and type")
         e4m3 = key.dtype == torch.float8_e4m3fn
-        for scale, pool in ((key_scale, key), (value_scale, value)):
-            if (scale is not None) != (e4m3 and pool is not None):
-                raise ValueError("8-bit pools need their scales, bf16 pools have none")
-            if scale is not None and (scale.shape != key.shape[:3] or scale.dtype != torch.uint8):
-                raise ValueError("scales must be uint8 [pages, kv heads, page size]")
-        for t in (key, value, key_scale, value_scale):
-            if t is not None and (t.device != key.device or not t.is_contiguous()):
+        pools = (key,) if value is None else (key, value)
+        if e4m3:
+            if key_scale is None or (value_scale is None) != (value is None):
+                raise ValueError("8-bit pools need their scales")
+            for scale in (key_scale,) if value is None else (key_scale, value_scale):
+                if scale.shape != key.shape[:3] or scale.dtype != torch.uint8:
+                    raise ValueError("scales must be uint8 [pages, kv heads, page size]")
+                pools += (scale,)
+        elif key_scale is not None or value_scale is not None:
+            raise ValueError("bf16 pools have no scales")
+        where = key.get_device()
+        for t in pools:
+            if t.get_device() != where or not t.is_contiguous():
                 raise ValueError("the pools and scales must be contiguous, on one device")
         self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
         self.struct = _lib.PagedKVStruct(
@@ -800,34 +806,48 @@ def _serving_device(dev: torch.device, what: str) -> torch.device:
     return dev
 
 
+# the current stream's handle without the Stream object that
+# torch.cuda.current_stream() builds around it (2 us of a 15 us call)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
 def _on_device(dev: torch.device, what: str, fn, args) -> None:
     """``fn(*args, stream)`` with ``dev`` current, on its current stream."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, stream)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
+
+
+def _int_list(t: Tensor, index: int) -> Tensor:
+    if t.dtype is not torch.int32 or t.get_device() != index:
+        raise ValueError("page_table, query_start and context_len must be int32, on the cache's device")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _paged_batch(kv: PagedKV, page_table: Tensor, query_start: Tensor | None, context_len: Tensor,
                  tokens: int):
     """(struct, the tensors it points into)."""
-    dev = kv.key.device
-    if page_table.ndim != 2 or context_len.ndim != 1 or page_table.shape[0] != context_len.shape[0]:
+    index = kv.key.get_device()
+    length = _int_list(context_len, index)
+    table = _int_list(page_table, index)
+    if table.ndim != 2 or length.ndim != 1:
         raise ValueError("page_table must be [sequences, pages] and context_len [sequences]")
-    if query_start is not None and query_start.shape != (context_len.shape[0] + 1,):
-        raise ValueError("query_start must be [sequences + 1]")
-    for t in (page_table, context_len) if query_start is None else (page_table, context_len, query_start):
-        if t.dtype != torch.int32 or t.device != dev:
-            raise ValueError(f"page_table, query_start and context_len must be int32 on {dev}")
-    table, length = page_table.contiguous(), context_len.contiguous()
-    start = None if query_start is None else query_start.contiguous()
+    n, width = table.shape
+    if length.shape[0] != n:
+        raise ValueError("page_table must be [sequences, pages] and context_len [sequences]")
+    start = None
+    if query_start is not None:
+        start = _int_list(query_start, index)
+        if start.ndim != 1 or start.shape[0] != n + 1:
+            raise ValueError("query_start must be [sequences + 1]")
     return _lib.PagedBatchStruct(table.data_ptr(), None if start is None else start.data_ptr(),
-                                 length.data_ptr(), table.shape[0], table.shape[1], tokens), \
-        (table, start, length)
+                                 length.data_ptr(), n, width, tokens), (table, start, length)
 
 
 def _status_ptr(status: Tensor | None, dev) -> int | None:
@@ -839,11 +859,15 @@ def _status_ptr(status: Tensor | None, dev) -> int | None:
     return status.data_ptr()
 
 
-def _row_view(t: Tensor) -> Tensor:
-    """``t`` [rows, width] with unit column stride and 16-byte rows (a copy if need be)."""
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16 or t.stride(0) < t.shape[1]:
+def _rows_of(t: Tensor) -> tuple[Tensor, int]:
+    """``t`` [rows, width] with 16-byte rows (a copy if need be), and its row stride."""
+    stride, step = t.stride()
+    if step != 1 or stride % 8 or t.data_ptr() % 16 or stride < t.shape[1]:
         t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        stride = t.shape[1]
+    return t, stride
 
 
 def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start: Tensor,
@@ -872,7 +896,7 @@ def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start:
         raise ValueError(f"qkv rows must be {width} wide, got {qkv.shape[1]}")
     tokens = qkv.shape[0]
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
-    qkv = _row_view(qkv)
+    qkv, stride = _rows_of(qkv)
     cos = sin = None
     if rope is not None:
         cos, sin = rope
@@ -880,10 +904,9 @@ def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start:
             if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous() or \
                     t.ndim != 2 or t.shape[1] * 2 != s.head_dim or t.shape != cos.shape:
                 raise ValueError("rope tables must be contiguous fp32 [positions, head_dim / 2]")
-    out = torch.empty((tokens, n_heads, s.head_dim), device=dev, dtype=torch.bfloat16) \
-        if n_heads else None
+    out = qkv.new_empty((tokens, n_heads, s.head_dim)) if n_heads else None
     _on_device(dev, "parrot_paged_append_bf16", _lib.load().parrot_paged_append_bf16, (
-        s, batch, qkv.data_ptr(), max(qkv.stride(0), width), n_heads,
+        s, batch, qkv.data_ptr(), max(stride, width), n_heads,
         None if out is None or tokens == 0 else out.data_ptr(),
         None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
         0 if cos is None else cos.shape[0], _status_ptr(status, dev)))
@@ -940,15 +963,19 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
     if heads % s.n_kv_heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
-    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
-        q = q.contiguous()
-    q2 = _row_view(q.view(tokens, heads * dim) if q.is_contiguous() else
-                   q.as_strided((tokens, heads * dim), (q.stride(0), 1)))
-    out = torch.empty((tokens, heads, dim), device=dev, dtype=torch.bfloat16)
+    width = heads * dim
+    if q.is_contiguous() and q.data_ptr() % 16 == 0:
+        rows, stride = q, width
+        out = torch.empty_like(q)
+    else:
+        if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
+            q = q.contiguous()
+        rows, stride = _rows_of(q.as_strided((tokens, width), (q.stride(0), 1)))
+        out = q.new_empty((tokens, heads, dim))
     if tokens:
         _on_device(dev, "parrot_paged_attention_bf16", _lib.load().parrot_paged_attention_bf16, (
-            s, batch, q2.data_ptr(), max(q2.stride(0), heads * dim), out.data_ptr(), heads,
-            window, sinks, dim ** -0.5 if scale is None else scale, _status_ptr(status, dev)))
+            s, batch, rows.data_ptr(), max(stride, width), out.data_ptr(), heads, window, sinks,
+            dim ** -0.5 if scale is None else scale, _status_ptr(status, dev)))
     return out
 
 
@@ -978,12 +1005,14 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
     if logits.stride(1) != 1 or logits.stride(0) < vocab:
         logits = logits.contiguous()
 
+    index = dev.index
+
     def param(v, name, dtype):
         if not isinstance(v, Tensor):
             return None, v
-        if v.shape != (rows,) or v.dtype != dtype or v.device != dev:
+        if v.ndim != 1 or v.shape[0] != rows or v.dtype is not dtype or v.get_device() != index:
             raise ValueError(f"{name} must be a number or {dtype} [{rows}] on {dev}")
-        return v.contiguous(), 0
+        return v if v.is_contiguous() else v.contiguous(), 0
 
     uniform, _ = param(uniform, "uniform", torch.float32)
     if uniform is None:
@@ -993,7 +1022,7 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
     p, p_all = param(top_p, "top_p", torch.float32)
     m, m_all = param(min_p, "min_p", torch.float32)
     ids = torch.empty((rows, 1), device=dev, dtype=torch.int64)
-    logprobs = torch.empty(rows, device=dev, dtype=torch.float32)
+    logprobs = torch.empty_like(uniform)
 
     def ptr(v):
         return None if v is None else v.data_ptr()
