@@ -43,32 +43,45 @@ __device__ __forceinline__ uint32_t scale_pair(int byte) {  // 2^(byte - 127) tw
   const uint32_t one = (uint32_t)byte << 7;
   return one | (one << 16);
 }
-__device__ __forceinline__ uint2 e4m3x4_numbers(uint32_t w);
-__device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t w, uint32_t scale2) {
-  uint2 r = e4m3x4_numbers(w);
-  r.x = mul_bf16x2_exact(r.x, scale2);
-  r.y = mul_bf16x2_exact(r.y, scale2);
-  return r;
-}
-__device__ __forceinline__ uint2 e4m3x4_numbers(uint32_t w) {
+// Without the scale, and with NaN as 480: for numbers known not to be NaN.
+__device__ __forceinline__ uint2 e4m3x4_finite(uint32_t w) {
   constexpr uint32_t k2p120 = ((120u + 127u) << 7) * 0x10001u;
   // bytes (0, 1) and (2, 3) into the upper bytes of the halves of a register
   const uint32_t lo = __byte_perm(w, 0, 0x1404), hi = __byte_perm(w, 0, 0x3424);
   uint2 r;
-  uint32_t a = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
-  uint32_t b = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
-  a = mul_bf16x2_exact(a, k2p120);
-  b = mul_bf16x2_exact(b, k2p120);
-  // any byte 0x7f / 0xff?  (w | 0x80..) == 0xff per byte
-  const uint32_t nan = __vcmpeq4(w | 0x80808080u, 0xffffffffu);
-  if (nan) {
-    if (nan & 0x000000ffu) a |= 0x00007fffu;
-    if (nan & 0x0000ff00u) a |= 0x7fff0000u;
-    if (nan & 0x00ff0000u) b |= 0x00007fffu;
-    if (nan & 0xff000000u) b |= 0x7fff0000u;
+  r.x = mul_bf16x2_exact((lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u), k2p120);
+  r.y = mul_bf16x2_exact((hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u), k2p120);
+  return r;
+}
+// A byte of w that is NaN (0x7f or 0xff) sets its top bit here, and no other does.
+__device__ __forceinline__ uint32_t e4m3_nan_bits(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint2 e4m3_put_nan(uint2 r, uint32_t nan) {
+  if (nan & 0x00000080u) r.x |= 0x00007fffu;
+  if (nan & 0x00008000u) r.x |= 0x7fff0000u;
+  if (nan & 0x00800000u) r.y |= 0x00007fffu;
+  if (nan & 0x80000000u) r.y |= 0x7fff0000u;
+  return r;
+}
+// Sixteen numbers as bf16 (two vectors).
+__device__ __forceinline__ void e4m3x16_numbers(const uint4& v, uint4 (&out)[2]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint2 r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = e4m3x4_finite(w[i]);
+  if (e4m3_nan_bits(v.x) | e4m3_nan_bits(v.y) | e4m3_nan_bits(v.z) | e4m3_nan_bits(v.w)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = e4m3_put_nan(r[i], e4m3_nan_bits(w[i]));
   }
-  r.x = a;
-  r.y = b;
+  out[0] = make_uint4(r[0].x, r[0].y, r[1].x, r[1].y);
+  out[1] = make_uint4(r[2].x, r[2].y, r[3].x, r[3].y);
+}
+__device__ __forceinline__ uint2 e4m3x4_to_bf16(uint32_t w, uint32_t scale2) {
+  uint2 r = e4m3x4_finite(w);
+  if (const uint32_t nan = e4m3_nan_bits(w)) r = e4m3_put_nan(r, nan);
+  r.x = mul_bf16x2_exact(r.x, scale2);
+  r.y = mul_bf16x2_exact(r.y, scale2);
   return r;
 }
 

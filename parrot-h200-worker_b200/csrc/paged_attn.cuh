@@ -23,6 +23,23 @@ struct Tile {
   int ctx;         // its context length, as given
 };
 
+// Rows of a tile as tokens and heads of the group: one division a tile, and for
+// a row a product with the reciprocal, exact for so small numbers.
+struct RowMap {
+  int group, token0, rest;
+  float inverse;
+  __device__ __forceinline__ RowMap(int row0, int g) : group(g) {
+    token0 = row0 / g;
+    rest = row0 - token0 * g;
+    inverse = 1.f / (float)g;
+  }
+  // (token of the sequence's rows, head of the group) of row r of the tile, r < 4096
+  __device__ __forceinline__ int2 operator()(int r) const {
+    const int x = rest + r, q = (int)(((float)x + 0.5f) * inverse);
+    return make_int2(token0 + q, x - q * group);
+  }
+};
+
 // The tile with this number, sequences in order, ceil(n_b * group / rows_per)
 // tiles each.  A whole warp calls; 32 sequences a step, their lengths loaded
 // side by side.

@@ -89,8 +89,8 @@ struct PrefillState {
   int bad[6];
   uint64_t* armed[2][6];       // the barrier of each stage's last copy, and its phase
   uint32_t armed_parity[2][6];
-  int row[128];                // e4m3: pool row of each key of the tile, -1: zeros
-  uint32_t scale[128];         // its scale bytes (key, value)
+  int row[2][128];             // e4m3: pool row of each key of two tiles, -1: zeros
+  uint32_t scale[2][128];      // their scale bytes (key, value)
   uint4 poison[kGroup * kMaxGroups];
   float m[kGroup * kMaxGroups], l[kGroup * kMaxGroups];  // merge
 };
@@ -143,18 +143,6 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31]), "r"(addr)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
@@ -674,36 +662,55 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         }
       }
     } else {
-      constexpr int VR = D / 16;                           // 16-byte vectors of a raw row
-      constexpr int kPer = (T * VR + 95) / 96;       // of a thread
-      bool ok = true;
+      // A unit is one side of a tile.  Its raw vectors are loaded while the unit
+      // before is widened, and the list of a tile's rows while the tile before is
+      // in work, so that no load is waited for where it is issued.
+      constexpr int VR = D / 16;                        // 16-byte vectors of a raw row
+      constexpr int kPer = (T * VR + 95) / 96;          // of a thread
       uint4 raw[kPer];
-      auto fetch = [&](const void* pool) {
+      auto rows_of = [&](int i, int list) {  // into st.row[list], st.scale[list]
+        if (i >= n) return;
+        for (int k = lt; k < T; k += 96) {
+          const int j = base_of(i) + k;
+          int at = -1;
+          if (some_row_sees(j)) {
+            const int page = page_of(a.batch, a.kv, tile.b, j, a.status);
+            if (page >= 0) at = (int)pool_row(a.kv, page, kvh, j);
+          }
+          st.row[list][k] = at;
+          st.scale[list][k] = at < 0 ? 0u : (uint32_t)a.kv.key_scale[at] |
+                                                (SEP ? (uint32_t)a.kv.value_scale[at] << 8 : 0u);
+        }
+      };
+      auto fetch = [&](int i, int side) {
+        if (i >= n) return;
+        const uint4* pool = reinterpret_cast<const uint4*>(side ? a.kv.value : a.kv.key);
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          const int v = lt + 96 * x;
-          raw[x] = make_uint4(0, 0, 0, 0);
-          if (v < T * VR) {
-            const int k = v / VR, c = v - k * VR, at = st.row[k];
-            if (at >= 0) raw[x] = reinterpret_cast<const uint4*>(pool)[(long long)at * VR + c];
+          const int v = lt + 96 * x, k = v / VR;
+          if (T * VR % 96 == 0 || v < T * VR) {
+            const int at = st.row[i & 1][k];
+            raw[x] = at >= 0 ? pool[(long long)at * VR + (v - k * VR)] : make_uint4(0, 0, 0, 0);
           }
         }
       };
-      auto widen = [&](unsigned char* dst, int shift, int s, bool check) {
+      auto widen = [&](unsigned char* dst, int list, int shift, int s, bool check) {
         bool any = false;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          const int v = lt + 96 * x;
-          if (v < T * VR) {
-            const int k = v / VR, c = v - k * VR;
-            const uint32_t s2 = scale_pair(st.scale[k] >> shift & 0xff);
-            const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+          const int v = lt + 96 * x, k = v / VR, c = v - k * VR;
+          if (T * VR % 96 == 0 || v < T * VR) {
+            const uint32_t s2 = scale_pair(st.scale[list][k] >> shift & 0xff);
+            uint4 o[2];
+            e4m3x16_numbers(raw[x], o);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint2 y = e4m3x4_to_bf16(w[2 * h], s2), z = e4m3x4_to_bf16(w[2 * h + 1], s2);
-              uint4 o = make_uint4(y.x, y.y, z.x, z.y);
+              o[h].x = mul_bf16x2_exact(o[h].x, s2);
+              o[h].y = mul_bf16x2_exact(o[h].y, s2);
+              o[h].z = mul_bf16x2_exact(o[h].z, s2);
+              o[h].w = mul_bf16x2_exact(o[h].w, s2);
               if (check) {
-                const uint32_t bits = not_finite8(o);
+                const uint32_t bits = not_finite8(o[h]);
                 if (bits) {
                   any = true;
                   const int c8 = 2 * c + h;
@@ -713,51 +720,47 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
                   } else {
                     for (int q = 0; q < 4; ++q) atomicOr(cols + q, 0xffffffffu);
                   }
-                  o.x &= keep_mask(bits, 0);
-                  o.y &= keep_mask(bits, 1);
-                  o.z &= keep_mask(bits, 2);
-                  o.w &= keep_mask(bits, 3);
+                  o[h].x &= keep_mask(bits, 0);
+                  o[h].y &= keep_mask(bits, 1);
+                  o[h].z &= keep_mask(bits, 2);
+                  o[h].w &= keep_mask(bits, 3);
                 }
               }
-              *reinterpret_cast<uint4*>(dst + sw64_at<T>(k, 2 * c + h)) = o;
+              *reinterpret_cast<uint4*>(dst + sw64_at<T>(k, 2 * c + h)) = o[h];
             }
           }
         }
         return any;
       };
+      rows_of(0, 0);
+      named_sync(1, 96);
+      fetch(0, 0);
+      rows_of(1, 1);
+      bool ok = true;
       for (int i = 0; ok && i < n; ++i) {
-        const int s = i % NS, base = base_of(i);
-        const bool edge = is_edge(base);
-        for (int k = lt; k < T; k += 96) {
-          const int j = base + k;
-          int at = -1;
-          if (some_row_sees(j)) {
-            const int page = page_of(a.batch, a.kv, tile.b, j, a.status);
-            if (page >= 0) at = (int)pool_row(a.kv, page, kvh, j);
-          }
-          st.row[k] = at;
-          st.scale[k] = at < 0 ? 0u : (uint32_t)a.kv.key_scale[at] |
-                                          (SEP ? (uint32_t)a.kv.value_scale[at] << 8 : 0u);
-        }
-        named_sync(1, 96);
+        const int s = i % NS;
+        const bool edge = is_edge(base_of(i));
         for (int side = 0; side < S::kSides; ++side) {
-          fetch(side ? a.kv.value : a.kv.key);
-          uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
-          bool mine = i < NS || wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
-          ok = !named_or(1, 96, !mine);  // all 96 stop together
-          if (!ok) break;
           const bool check = edge && side == S::kSides - 1;
           if (check)
             for (int k = lt; k < T; k += 96) bad_cols[s * T + k] = make_uint4(0, 0, 0, 0);
-          if (check) named_sync(1, 96);
-          const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, 8 * side, s, check);
+          uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
+          const bool mine = i < NS || wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
+          ok = !named_or(1, 96, !mine);  // all 96 stop together; the lists are complete
+          if (!ok) break;
+          const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, i & 1, 8 * side, s, check);
           fence_async_shared();
+          // the next unit's loads, on their way while the others finish
+          if (side + 1 < S::kSides) fetch(i, side + 1);
+          else fetch(i + 1, 0);
           const bool found = named_or(1, 96, any);
           if (lt == 0) {
             if (check) st.bad[s] = found;
             mbar_arrive(side ? &st.v_full[s] : &st.k_full[s]);
           }
         }
+        // every thread is past this tile's list
+        if (ok) rows_of(i + 2, i & 1);
       }
     }
   } else if (warp == S::kMmaWarp) {
