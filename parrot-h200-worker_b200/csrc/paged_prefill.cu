@@ -19,11 +19,11 @@
 // computed early (152 us); with steps of 64 keys over two S blocks a group
 // (146 us); with two threads a row (145 us).
 //
-// Warps: the groups' rows first, then three that bring K and V and one that
-// issues the matrix instructions.  A bf16 cache comes by TMA, a page's rows of
+// Warps: the groups' rows first, then three (seven for e4m3) that bring K and V
+// and one that issues the matrix instructions.  A bf16 cache comes by TMA, a page's rows of
 // 32 columns at a time into a 64-byte-swizzled tile (three boxes for a 96-wide
 // head); an e4m3 cache is read, widened and stored to the same tiles by the
-// three warps.
+// seven.
 //
 // Tiles at an edge of what the rows see (the diagonal, the window's start, the
 // sinks) pass through two of the three first: in a product 0 * NaN would carry a
@@ -45,7 +45,6 @@ using namespace tc;
 
 constexpr int kGroup = 128;             // rows of a group
 constexpr int kMaxGroups = 3;
-constexpr int kLoadWarps = 3;
 constexpr int kMaxRanks = 8;
 constexpr float kGrowth = 8.f;          // log2 of the growth of a maximum let through
 
@@ -57,11 +56,18 @@ __host__ __device__ constexpr int paged_box_rows(int d, int page) {
   return page < tile_keys(d) ? page : tile_keys(d);
 }
 
-template <int D, bool SEP>
+template <int D, bool E4M3, bool SEP>
 struct PrefillShape {
   static constexpr int kGroups = tile_groups(D), kKeys = tile_keys(D);
   static constexpr int kRows = kGroup * kGroups, kRowWarps = 4 * kGroups;
+  static constexpr int kLoadWarps = E4M3 ? 7 : 3;  // widening takes more
   static constexpr int kMmaWarp = kRowWarps + kLoadWarps, kThreads = 32 * (kMmaWarp + 1);
+  // Registers of a rows' thread and of the others: their sum stays within the
+  // launch's, 65536 / kThreads rounded down to 8 each (0: no split).
+  static constexpr int kRowRegs = E4M3 ? (kGroups == 2 ? 184 : 120) : kGroups == 2 ? 208 : 0;
+  static constexpr int kOtherRegs = E4M3 ? (kGroups == 2 ? 72 : 56) : 88;
+  static_assert(kRowRegs == 0 || (kRowRegs * kRowWarps + kOtherRegs * (kLoadWarps + 1)) * 32 <=
+                                     65536 / kThreads / 8 * 8 * kThreads, "register split");
   // TMEM columns: S (and P over it) of group g at g * kKeys, O behind
   static constexpr uint32_t kTmemO = kGroups * kKeys;
   static_assert(kGroups * (kKeys + D) <= 512, "S and O of all groups");
@@ -281,10 +287,10 @@ __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState
 }  // namespace
 
 template <int D, bool E4M3, bool SEP>
-__global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
+__global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     paged_prefill_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map) {
-  using S = PrefillShape<D, SEP>;
+  using S = PrefillShape<D, E4M3, SEP>;
   constexpr int NS = S::kStages, T = S::kKeys, NG = S::kGroups, R = S::kRows;
   extern __shared__ unsigned char pf_raw[];
   __shared__ PrefillState st;
@@ -381,8 +387,8 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
 
   if (warp < S::kRowWarps) {
     // ---------------- rows ----------------
-    // a row of 128 keys is 128 registers: 8 warps x 208 + 4 x 88 = 12 x 168 of launch
-    if constexpr (NG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (S::kRowRegs > 0)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kRowRegs));
     const int g = warp >> 2, quarter = warp & 3, r = warp * 32 + lane;
     const int pos = pos0 + (tile.row0 + min(r, rows - 1)) / group;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -550,10 +556,11 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
     finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks, 32 * S::kRowWarps);
     return;
   }
-  if constexpr (NG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp < S::kRowWarps + kLoadWarps) {
+  if constexpr (S::kRowRegs > 0)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
+  if (warp < S::kRowWarps + S::kLoadWarps) {
     // ---------------- keys and values ----------------
-    const int lt = threadIdx.x - 32 * S::kRowWarps;  // 0 .. 95
+    const int lt = threadIdx.x - 32 * S::kRowWarps;
     uint32_t raw_phase = 0;            // a bit per stage
     if constexpr (!E4M3) {
       if (warp == S::kRowWarps) {
@@ -665,12 +672,13 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
       // A unit is one side of a tile.  Its raw vectors are loaded while the unit
       // before is widened, and the list of a tile's rows while the tile before is
       // in work, so that no load is waited for where it is issued.
+      constexpr int LT = 32 * S::kLoadWarps;
       constexpr int VR = D / 16;                        // 16-byte vectors of a raw row
-      constexpr int kPer = (T * VR + 95) / 96;          // of a thread
+      constexpr int kPer = (T * VR + LT - 1) / LT;          // of a thread
       uint4 raw[kPer];
       auto rows_of = [&](int i, int list) {  // into st.row[list], st.scale[list]
         if (i >= n) return;
-        for (int k = lt; k < T; k += 96) {
+        for (int k = lt; k < T; k += LT) {
           const int j = base_of(i) + k;
           int at = -1;
           if (some_row_sees(j)) {
@@ -687,8 +695,8 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         const uint4* pool = reinterpret_cast<const uint4*>(side ? a.kv.value : a.kv.key);
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          const int v = lt + 96 * x, k = v / VR;
-          if (T * VR % 96 == 0 || v < T * VR) {
+          const int v = lt + LT * x, k = v / VR;
+          if (T * VR % LT == 0 || v < T * VR) {
             const int at = st.row[i & 1][k];
             raw[x] = at >= 0 ? pool[(long long)at * VR + (v - k * VR)] : make_uint4(0, 0, 0, 0);
           }
@@ -698,8 +706,8 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         bool any = false;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-          const int v = lt + 96 * x, k = v / VR, c = v - k * VR;
-          if (T * VR % 96 == 0 || v < T * VR) {
+          const int v = lt + LT * x, k = v / VR, c = v - k * VR;
+          if (T * VR % LT == 0 || v < T * VR) {
             const uint32_t s2 = scale_pair(st.scale[list][k] >> shift & 0xff);
             uint4 o[2];
             e4m3x16_numbers(raw[x], o);
@@ -733,7 +741,7 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         return any;
       };
       rows_of(0, 0);
-      named_sync(1, 96);
+      named_sync(1, LT);
       fetch(0, 0);
       rows_of(1, 1);
       bool ok = true;
@@ -743,17 +751,17 @@ __global__ void __launch_bounds__(PrefillShape<D, SEP>::kThreads, 1)
         for (int side = 0; side < S::kSides; ++side) {
           const bool check = edge && side == S::kSides - 1;
           if (check)
-            for (int k = lt; k < T; k += 96) bad_cols[s * T + k] = make_uint4(0, 0, 0, 0);
+            for (int k = lt; k < T; k += LT) bad_cols[s * T + k] = make_uint4(0, 0, 0, 0);
           uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
           const bool mine = i < NS || wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
-          ok = !named_or(1, 96, !mine);  // all 96 stop together; the lists are complete
+          ok = !named_or(1, LT, !mine);  // all stop together; the lists are complete
           if (!ok) break;
           const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, i & 1, 8 * side, s, check);
           fence_async_shared();
           // the next unit's loads, on their way while the others finish
           if (side + 1 < S::kSides) fetch(i, side + 1);
           else fetch(i + 1, 0);
-          const bool found = named_or(1, 96, any);
+          const bool found = named_or(1, LT, any);
           if (lt == 0) {
             if (check) st.bad[s] = found;
             mbar_arrive(side ? &st.v_full[s] : &st.k_full[s]);
@@ -838,14 +846,13 @@ namespace {
 template <int D, bool E4M3, bool SEP>
 int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map, int sms,
                    cudaStream_t stream) {
-  using S = PrefillShape<D, SEP>;
+  using S = PrefillShape<D, E4M3, SEP>;
   auto k = paged_prefill_kernel<D, E4M3, SEP>;
   const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
   const long long tiles = std::min(n * ((group + S::kRows - 1) / S::kRows),
                                    n * group / S::kRows + std::min<long long>(a.batch.batch, n));
   // CTAs per tile while the GPU has SMs to spare
-  int ranks = 1;
-  while (ranks < kMaxRanks && 2 * ranks * tiles * a.kv.kv_heads <= sms) ranks *= 2;
+  const int ranks = (int)std::max(1LL, std::min<long long>(kMaxRanks, sms / (tiles * a.kv.kv_heads)));
   a.cluster = ranks;
   if (tiles * ranks * a.kv.kv_heads > 0x7fffffffll) return -1;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
