@@ -13,6 +13,8 @@ The hot path runs in ``libparrot_b200.so`` (C ABI: ``include/parrot_b200.h``);
 """
 from .model import (Block, DepthMix, GenerationState, GlobalMLA, LocalGQA, LocalKVCache,
                     MLALatentCache, ModelConfig, ModelOutput, MoE, Parrot, RMSNorm, SwiGLU)
+from .paged import PagedState
 
 __all__ = ["Block", "DepthMix", "GenerationState", "GlobalMLA", "LocalGQA", "LocalKVCache",
-           "MLALatentCache", "ModelConfig", "ModelOutput", "MoE", "Parrot", "RMSNorm", "SwiGLU"]
+           "MLALatentCache", "ModelConfig", "ModelOutput", "MoE", "PagedState",
+           "Parrot", "RMSNorm", "SwiGLU"]

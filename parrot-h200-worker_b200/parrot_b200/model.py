@@ -25,6 +25,7 @@ from torch.nn import functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from . import bridge
+from .paged import PagedBatch, PagedState, padded_rows
 
 # Decode attends over a key length that grows by one every step.  The cuDNN
 # SDPA backend builds an execution plan per new shape, so decode keeps to the
@@ -279,6 +280,23 @@ class LocalGQA(nn.Module):
         return out if addend is None else addend + out
 
 
+    def extend(self, x: Tensor, kv: bridge.PagedKV, batch: PagedBatch, sinks: int) -> Tensor:
+        """New tokens of a ragged batch ``x`` [1, rows, dim] over the paged cache: rotated,
+        appended and attended (the window, and the first ``sinks`` tokens behind it)."""
+        c = self.cfg
+        rows = x.shape[1]
+        w = _packed(self, "_qkv_weight", (self.q.weight, self.k.weight, self.v.weight))
+        qkv = F.linear(x[0], w)
+        q = bridge.b200_paged_append(kv, qkv, batch.page_table, batch.query_start,
+                                     batch.context_len, c.n_heads,
+                                     rope=_rope_tables(c, x.device, torch.float32))
+        y = bridge.b200_paged_attention(q, kv, batch.page_table, batch.query_start,
+                                        batch.context_len, window=c.window_size, sinks=sinks)
+        if batch.tokens < rows:
+            y[batch.tokens:] = 0  # rows of no sequence
+        return self.out(y.view(1, rows, -1))
+
+
 class GlobalMLA(nn.Module):
     """NoPE joint-latent attention (``model.py:331-432``), PyTorch SDPA."""
 
@@ -372,6 +390,22 @@ class GlobalMLA(nn.Module):
         ctx = ctx.transpose(1, 2).reshape(b, 1, c.n_heads * c.kv_latent_dim)
         out = F.linear(ctx, ao).to(x.dtype)
         return out if addend is None else addend + out
+
+
+    def extend(self, x: Tensor, kv: bridge.PagedKV, batch: PagedBatch, sinks: int) -> Tensor:
+        """New tokens of a ragged batch ``x`` [1, rows, dim] over the paged latent cache, by the
+        absorbed weights (every earlier token is visible: no window, no sinks)."""
+        c = self.cfg
+        rows = x.shape[1]
+        aq, ao = self._absorbed()
+        bridge.b200_paged_append(kv, self.kv_down(x[0]), batch.page_table, batch.query_start,
+                                 batch.context_len, 0)
+        q = F.linear(x[0], aq).view(rows, c.n_heads, c.kv_latent_dim)
+        y = bridge.b200_paged_attention(q, kv, batch.page_table, batch.query_start,
+                                        batch.context_len, scale=c.head_dim ** -0.5)
+        if batch.tokens < rows:
+            y[batch.tokens:] = 0
+        return F.linear(y.view(1, rows, -1), ao)
 
 
 class SwiGLU(nn.Module):
@@ -707,6 +741,82 @@ class Parrot(nn.Module):
     def decode_next(self, input_ids: Tensor, state: GenerationState):
         """Append one token and return the next greedy token (``model.py:927-931``)."""
         return self.decode_step(input_ids, state, _next_token_only=True)
+
+    def paged_state(self, sequences: int, pages: int, page_size: int = 64,
+                    kv_dtype: torch.dtype = torch.bfloat16, sink_tokens: int = 0) -> PagedState:
+        """A paged cache for ``extend``: ``pages`` pages of ``page_size`` tokens shared by up to
+        ``sequences`` sequences, bf16 or 8-bit (``torch.float8_e4m3fn``, one scale a row).
+        ``sink_tokens``: that many first tokens stay visible behind the local layers' window."""
+        return PagedState(self.config, sequences, pages, page_size, kv_dtype, sink_tokens,
+                          self.embedding.weight.device,
+                          [isinstance(b.attention, LocalGQA) for b in self.blocks])
+
+    @torch.inference_mode()
+    def extend(self, input_ids: Tensor, counts, state: PagedState, sequences=None) -> Tensor:
+        """Append ``counts[i]`` tokens to sequence ``sequences[i]`` (default: 0, 1, ...) of
+        ``state``.  ``input_ids`` [sum(counts)]: the new tokens, sequence by sequence.  Returns
+        the logits [with new tokens, vocab] after each of those sequences' last token."""
+        cfg = self.config
+        if self.training:
+            raise RuntimeError("extend requires model.eval()")
+        if len(state.layers) != cfg.n_layers:
+            raise ValueError("Paged state does not match model depth")
+        counts = [int(n) for n in counts]
+        sequences = list(range(len(counts))) if sequences is None else list(sequences)
+        if input_ids.ndim != 1 or input_ids.shape[0] != sum(counts):
+            raise ValueError("input_ids must be [sum(counts)]")
+        batch = state.batch(sequences, counts)
+        rows = padded_rows(batch.tokens)
+        if rows > batch.tokens:
+            input_ids = F.pad(input_ids, (0, rows - batch.tokens))
+        x = self.embedding(input_ids.to(state.device))[None]
+        attnres = cfg.residual == "attnres"
+        res = _Residuals(x, cfg.depth_block_size)
+        index = 0
+        for block, kv in zip(self.blocks, state.layers):
+            h = res.mix(self.depth_mix[index], block.attention_norm) if attnres \
+                else block.attention_norm(x)
+            delta = block.attention.extend(h, kv, batch, state.sink_tokens)
+            if attnres:
+                res.add_delta(delta)
+                res.end_module(index)
+            else:
+                x = x + delta
+            index += 1
+            h = res.mix(self.depth_mix[index], block.moe_norm, block.moe) if attnres \
+                else block.moe_norm(x)
+            out = block.moe.inference(h, direct=False, addend=res.partial if attnres else x,
+                                      defer_combine=attnres)
+            if attnres:
+                res.set_partial(out)
+                res.end_module(index)
+            else:
+                x = out
+            index += 1
+        h = res.mix(self.depth_mix[-1], self.final_norm) if attnres else self.final_norm(x)
+        state.advance(sequences, counts)
+        last, at = [], 0
+        for n in counts:
+            at += n
+            if n:
+                last.append(at - 1)
+        return F.linear(h[0, last], self.embedding.weight)
+
+    @staticmethod
+    @torch.inference_mode()
+    def sample(logits: Tensor, uniform: Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Draw a token per row of ``logits`` from the given random numbers:
+        ``(ids [rows, 1], log-probabilities [rows])``; see ``bridge.b200_sample``."""
+        return bridge.b200_sample(logits, uniform, temperature, top_k, top_p, min_p)
+
+    @torch.inference_mode()
+    def decode_sample(self, input_ids: Tensor, state: GenerationState, uniform: Tensor,
+                      temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """``decode_next`` with a draw in the place of the largest logit:
+        ``(ids [batch, 1], log-probabilities [batch], state)``."""
+        logits, state = self.decode_step(input_ids, state)
+        ids, logp = bridge.b200_sample(logits, uniform, temperature, top_k, top_p, min_p)
+        return ids, logp, state
 
     def capture_decode(self, state: GenerationState, next_token_only: bool = False):
         """CUDA-graph replay of ``decode_step`` (or ``decode_next``) on ``state``.

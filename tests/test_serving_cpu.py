@@ -152,3 +152,60 @@ def test_the_sampling_definition_on_a_row_by_hand():
     assert sample_row(x, 0.9, 1.0, 0, float(1 / w.sum()) - 1e-6, 0.0)[0] == 1
     assert sample_row(x, 0.9, 1.0, 0, float(1 / w.sum()) + 1e-6, 0.0)[0] == 3
     assert sample_row(x, 0.999, 1.0, 0, 1.0, 0.5)[0] == 3
+
+
+# ---------------------------------------------------------------------------- the paged state
+def _state(**kw):
+    from parrot_b200 import ModelConfig, PagedState
+    cfg = ModelConfig(dim=128, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=32, kv_latent_dim=32, n_experts=8,
+                      expert_dim=128, shared_expert_dim=64, window_size=64, max_seq_len=100, global_every=2)
+    d = dict(sequences=3, pages=8, page_size=16, kv_dtype=torch.bfloat16, sink_tokens=0)
+    d.update(kw)
+    return PagedState(cfg, d["sequences"], d["pages"], d["page_size"], d["kv_dtype"], d["sink_tokens"], "cpu",
+                      [True, False])
+
+
+def test_paged_state_hands_out_pages_and_takes_them_back():
+    s = _state(kv_dtype=E4M3)
+    assert [kv.key.shape for kv in s.layers] == [(8, 2, 16, 32), (8, 1, 16, 32)]
+    assert s.layers[0].value is not None and s.layers[1].value is None and s.layers[1].value_scale is None
+    b = s.batch([2, 0], [17, 16])
+    assert b.tokens == 33 and b.query_start.tolist() == [0, 17, 33] and b.context_len.tolist() == [17, 16]
+    assert b.page_table.tolist() == [s.pages_of(2), s.pages_of(0) + [-1]]
+    s.advance([2, 0], [17, 16])
+    assert s.lengths == [16, 0, 17] and s.free_pages == 5
+    b = s.batch([0, 2], [1, 0])
+    assert b.page_table.shape == (2, 2) and b.context_len.tolist() == [17, 17]
+    s.advance([0, 2], [1, 0])
+    owned = s.pages_of(0) + s.pages_of(2)
+    assert len(set(owned)) == 4 and s.free_pages == 4
+    with pytest.raises(RuntimeError, match="free pages"):
+        s.batch([1], [65])
+    assert s.free_pages == 4 and s.pages_of(1) == []        # all or none
+    s.release(2)
+    assert s.free_pages == 6 and s.lengths == [17, 0, 0]
+    s.batch([1], [65])
+    assert s.free_pages == 1
+
+
+@pytest.mark.parametrize("seqs,counts", [([0], [101]), ([0, 0], [1, 1]), ([3], [1]), ([-1], [1]), ([0], [0]),
+                                         ([0], [-1]), ([0, 1], [1]), ([], [])])
+def test_paged_state_refuses_bad_steps(seqs, counts):
+    s = _state(pages=20)
+    with pytest.raises(ValueError):
+        s.batch(seqs, counts)
+    assert s.free_pages == 20
+
+
+@pytest.mark.parametrize("kw", [dict(sequences=0), dict(pages=0), dict(page_size=24), dict(kv_dtype=torch.float16),
+                                dict(sink_tokens=-1)])
+def test_paged_state_refuses_bad_sizes(kw):
+    with pytest.raises(ValueError):
+        _state(**kw)
+
+
+def test_padded_rows_are_few_and_near():
+    from parrot_b200.paged import padded_rows
+    sizes = [padded_rows(n) for n in range(1, 4097)]
+    assert all(n <= p <= n * 1.25 for n, p in enumerate(sizes, 1)) and sizes == sorted(sizes)
+    assert len(set(sizes)) <= 16 + 4 * 8 + 1 and padded_rows(4096) == 4096
