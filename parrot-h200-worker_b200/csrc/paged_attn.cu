@@ -81,13 +81,16 @@ __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) !
 // fixed order: no workspace, no second launch, no atomics.
 //
 // An e4m3 cache halves the bytes, and widening them becomes what counts.  Keys
-// go from memory to the product's registers: a thread's 8 bytes of a key are
-// its share of two products when the query's columns are permuted alike, and
-// the conversion to f16 is one instruction for two (the query goes to f16 with
-// a power of two per row that puts its largest magnitude at 2^8, so what f16
-// loses is below 2^-32 of that).  The scales multiply the scores' columns, and
-// for the values the probabilities, as powers of two exactly.  Values pass
-// through shared memory as bf16 for the transposed load.
+// and values go from memory straight to the products' registers as f16, one
+// conversion instruction for two numbers: a thread's 8 bytes of a key are its
+// share of two products when the query's columns are permuted alike, and its 4
+// bytes of four keys' values, transposed by byte permutations, its share of
+// four column tiles when the output's columns are.  The query goes to f16 with a
+// power of two per row that puts its largest magnitude at 2^8 (what f16 loses is
+// below 2^-32 of that); the keys' scales multiply the scores.  The values'
+// scales multiply the probabilities, w = p 2^e, and these go to f16 relative to
+// a power of two W per row above all its w so far, at 2^14 W^-1: 11 bits down to
+// 2^-28 W, nothing lost above 2^-39 W.
 // ---------------------------------------------------------------------------
 constexpr int kDecWarps = 4;
 constexpr int kDecKeys = 32;
@@ -102,8 +105,8 @@ struct DecodeShape {
   static constexpr int kTile = kDecKeys * kRow;
   static constexpr int kSide = kTile;
   static constexpr int kStage = kSide * (SEP ? 2 : 1);
-  // e4m3: one bf16 tile that a chunk's values are widened to
-  static constexpr int kWarp = E4M3 ? kTile : kStage * kStages;
+  static constexpr int kPoison = kDecRows * 16;  // e4m3: columns of each row that are NaN
+  static constexpr int kWarp = E4M3 ? kDecRows * D * 4 + 2 * kDecRows * 4 + kPoison : kStage * kStages;
   static constexpr int kPart = kDecRows * D * 4 + 2 * kDecRows * 4;  // a CTA's result
   static constexpr int kBytes = kWarp * kDecWarps + kPart;
   static_assert(kWarp >= kPart, "a warp's ring holds its result");
@@ -209,16 +212,17 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
     cp_async_commit();
   };
   // e4m3: chunk c into registers: this thread's keys (8 t .. 8 t + 7 of each 32
-  // columns of keys g, g + 8, ...), vectors of the values in memory order, and
-  // the scale bytes of key `lane`; zeros for keys nobody sees
-  constexpr int NB = D / 32, VR8 = D / 16;
+  // columns of keys g, g + 8, ...), its values (4 g .. 4 g + 3 of each 32 columns
+  // of keys 8 i + 2 t and + 1), and the scale bytes of key `lane`; zeros for keys
+  // nobody sees
+  constexpr int NB = D / 32;
   uint2 kr[E4M3 ? 4 : 1][E4M3 ? NB : 1];
-  uint4 vr[E4M3 ? VR8 : 1];
+  uint32_t vr[E4M3 ? 8 : 1][E4M3 ? NB : 1];
   uint32_t scales = 0;
-  auto fetch8 = [&](int c, int page) {
-    if (c >= chunks) return;
-    const int row = page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, base_of(c) + lane);
-    const void* values = SEP ? a.kv.value : a.kv.key;
+  auto row_for = [&](int c, int page) {
+    return c >= chunks || page < 0 ? -1 : (int)pool_row(a.kv, page, kvh, base_of(c) + lane);
+  };
+  auto fetch_keys = [&](int row) {
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
       const int rr = __shfl_sync(0xffffffffu, row, nt * 8 + g);
@@ -226,17 +230,27 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
 #pragma unroll
       for (int b = 0; b < NB; ++b) kr[nt][b] = rr < 0 ? make_uint2(0u, 0u) : src[4 * b];
     }
-#pragma unroll
-    for (int i = 0; i < VR8; ++i) {
-      const int v = lane + 32 * i, r = v / VR8, cv = v - r * VR8;
-      const int rr = __shfl_sync(0xffffffffu, row, r);
-      vr[i] = rr < 0 ? make_uint4(0u, 0u, 0u, 0u)
-                     : reinterpret_cast<const uint4*>(values)[(long long)rr * VR8 + cv];
-    }
     scales = row < 0 ? (uint32_t)kScaleBias * 0x101u
                      : (uint32_t)a.kv.key_scale[row] |
                            (uint32_t)(SEP ? a.kv.value_scale : a.kv.key_scale)[row] << 8;
   };
+  auto fetch_values = [&](int row) {
+    const void* values = SEP ? a.kv.value : a.kv.key;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int rr = __shfl_sync(0xffffffffu, row, (i >> 1) * 8 + 2 * t + (i & 1));
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(values) + (long long)max(rr, 0) * (D / 4) + g;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) vr[i][b] = rr < 0 ? 0u : src[8 * b];
+    }
+  };
+  uint32_t* poison = reinterpret_cast<uint32_t*>(ring + S::kWarp - (E4M3 ? S::kPoison : 0));  // [row][4]
+  if constexpr (E4M3) {
+    poison[lane] = poison[lane + 32] = 0;
+    __syncwarp();
+  }
+  float top_w[2] = {0.f, 0.f};        // e4m3: W of each row, 0 before its first
+  const bool two = rows > 8;          // whether rows g + 8 exist
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[NT][4];
@@ -246,8 +260,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
   int c = me, it = 0;
   int next_page = -1;
+  [[maybe_unused]] int next_row = -1;
   if constexpr (E4M3) {
-    fetch8(c, page_for(c));
+    const int row = row_for(c, page_for(c));
+    fetch_keys(row);
+    fetch_values(row);
     next_page = page_for(c + workers);
   } else {
     fetch(c, page_for(c), 0);
@@ -260,8 +277,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-    uint32_t v_u = ring_u;
-    float v_scale[4][2];  // of the keys of this thread's columns
+    [[maybe_unused]] uint32_t v_u = ring_u;
+    [[maybe_unused]] float v_scale[4][2];  // of the keys of this thread's columns
     if constexpr (E4M3) {
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt)
@@ -270,19 +287,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
           mma_16816_f16(s[nt], qf[2 * b], e4m3x2_to_f16(kr[nt][b].x), e4m3x2_to_f16(kr[nt][b].x >> 16));
           mma_16816_f16(s[nt], qf[2 * b + 1], e4m3x2_to_f16(kr[nt][b].y), e4m3x2_to_f16(kr[nt][b].y >> 16));
         }
-      // the values as bf16 numbers to shared memory
-#pragma unroll
-      for (int i = 0; i < VR8; ++i) {
-        const int v = lane + 32 * i, r = v / VR8, cv = v - r * VR8;
-        uint4 w[2];
-        e4m3x16_numbers(vr[i], w);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(ring_u + r * S::kRow +
-                                                                        cv * 32 + h * 16),
-                       "r"(w[h].x), "r"(w[h].y), "r"(w[h].z), "r"(w[h].w)
-                       : "memory");
-      }
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
@@ -293,9 +297,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
           s[nt][e] *= ks;
           s[nt][2 + e] *= ks;
         }
-      fetch8(c + workers, next_page);
+      // the next chunk's keys come while this one is worked on, its values while
+      // those keys are multiplied
+      next_row = row_for(c + workers, next_page);
+      fetch_keys(next_row);
       next_page = page_for(c + 2 * workers);
-      __syncwarp();
     } else {
       const int slot = it & 1;
       fetch(c + workers, next_page, slot ^ 1);
@@ -327,9 +333,14 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
         s[nt][j] *= row_scale[j >> 1];
         if (!whole && !sees(j >> 1, base + nt * 8 + 2 * t + (j & 1))) s[nt][j] = -INFINITY;
       }
-    float corr[2];
+    float corr[2] = {1.f, 1.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !two) {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) s[nt][2] = s[nt][3] = 0.f;
+        continue;
+      }
       float mx = m[i];
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * i], s[nt][2 * i + 1]));
@@ -349,6 +360,31 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
         }
       l[i] = fmaf(l[i], corr[i], sum);  // this thread's columns; the quad is summed at the end
     }
+    if constexpr (E4M3) {
+      float most[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[nt][2 * i + e] *= v_scale[nt][e];
+            most[i] = fmaxf(most[i], s[nt][2 * i + e]);
+          }
+      if (__any_sync(0xffffffffu, most[0] >= top_w[0] || (two && most[1] >= top_w[1]))) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
+          most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
+          if (most[i] > 0.f && most[i] >= top_w[i]) {
+            // the power of two above it (at least 2^-100: its reciprocal is finite)
+            const float w = fmaxf(__uint_as_float((__float_as_uint(most[i]) & 0x7f800000u) + 0x00800000u), pow2(-100));
+            corr[i] *= top_w[i] / w;
+            top_w[i] = w;
+          }
+        }
+      }
+    }
     if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -358,81 +394,131 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
         o[nt][3] *= corr[1];
       }
     }
-    if (!whole && pmin != pmax) {
-      // A value that is not finite would reach, as 0 * NaN in the product, the
-      // rows that do not see its key.  Take such numbers out of the tile and add
-      // them to the rows that see them.
-      unsigned bad_row = 0;
-#pragma unroll 1
-      for (int i = 0; i < D / 2; ++i) {
-        uint32_t w;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(v_u + lane * S::kRow + i * 4));
-        bad_row |= !finite_bf16(w) || !finite_bf16(w >> 16);
+    if constexpr (E4M3) {
+      if (!whole && pmin != pmax) {
+        // As below: a NaN among the values is taken out, and noted for the rows
+        // that see its key.
+        uint32_t some = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) some |= e4m3_nan_bits(vr[i][b]);
+        if (__any_sync(0xffffffffu, some != 0)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t nan = e4m3_nan_bits(vr[i][b]);
+              if (nan == 0) continue;
+              const uint32_t cols = ((nan >> 7 & 1) | (nan >> 14 & 2) | (nan >> 21 & 4) | (nan >> 28 & 8)) << (4 * g);
+              const int j = base + (i >> 1) * 8 + 2 * t + (i & 1);
+              for (int r = 0; r < rows; ++r) {
+                const int at = pos0 + map(r).x;
+                if (j <= at && (a.window == 0 || at - j < a.window || j < a.sinks))
+                  atomicOr(poison + r * 4 + b, cols);
+              }
+              vr[i][b] &= ~((nan >> 7) * 0xffu);
+            }
+        }
       }
-      const unsigned bad = __ballot_sync(0xffffffffu, bad_row);
-      if (bad) {
-        for (unsigned left = bad; left; left &= left - 1) {
-          const int j = __ffs(left) - 1;  // key base + j: column tile j / 8, thread (j % 8) / 2
-          const int src = (lane & ~3) | ((j & 7) >> 1);
+      float up[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float p = 0.f;
+      for (int i = 0; i < 2; ++i)  // 2^14 / W
+        up[i] = top_w[i] > 0.f ? __uint_as_float((268u << 23) - __float_as_uint(top_w[i])) : 0.f;
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-              if (nt == j >> 3) p = j & 1 ? s[nt][2 * i + 1] : s[nt][2 * i];
-            p = __shfl_sync(0xffffffffu, p, src);
-            const bool vis = sees(i, base + j);
+      for (int kk = 0; kk < 2; ++kk) {
+        uint32_t p[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t w;
-              asm volatile("ld.shared.u32 %0, [%1];"
-                           : "=r"(w)
-                           : "r"(v_u + j * S::kRow + (nt * 8 + 2 * t) * 2));
-              const float2 v = bf16x2_to_float2(w);
-              if (vis && !finite_bf16(w)) o[nt][2 * i] = fmaf(p, v.x, o[nt][2 * i]);
-              if (vis && !finite_bf16(w >> 16)) o[nt][2 * i + 1] = fmaf(p, v.y, o[nt][2 * i + 1]);
+        for (int j = 0; j < 4; ++j) {
+          const int nt = 2 * kk + (j >> 1);
+          p[j] = pack_f16x2(s[nt][2 * (j & 1)] * up[j & 1], s[nt][2 * (j & 1) + 1] * up[j & 1]);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          // four keys' bytes of four columns, transposed
+          const uint32_t w0 = vr[4 * kk][b], w1 = vr[4 * kk + 1][b], w2 = vr[4 * kk + 2][b], w3 = vr[4 * kk + 3][b];
+          const uint32_t t0 = __byte_perm(w0, w1, 0x5140), t1 = __byte_perm(w0, w1, 0x7362);
+          const uint32_t t2 = __byte_perm(w2, w3, 0x5140), t3 = __byte_perm(w2, w3, 0x7362);
+          // t0: columns 0 (low half) and 1 of keys 0, 1; t2: of keys 2, 3
+          mma_16816_f16(o[4 * b], p, e4m3x2_to_f16(t0), e4m3x2_to_f16(t2));
+          mma_16816_f16(o[4 * b + 1], p, e4m3x2_to_f16(t0 >> 16), e4m3x2_to_f16(t2 >> 16));
+          mma_16816_f16(o[4 * b + 2], p, e4m3x2_to_f16(t1), e4m3x2_to_f16(t3));
+          mma_16816_f16(o[4 * b + 3], p, e4m3x2_to_f16(t1 >> 16), e4m3x2_to_f16(t3 >> 16));
+        }
+      }
+      fetch_values(next_row);
+    } else {
+      if (!whole && pmin != pmax) {
+        // A value that is not finite would reach, as 0 * NaN in the product, the
+        // rows that do not see its key.  Take such numbers out of the tile and add
+        // them to the rows that see them.
+        unsigned bad_row = 0;
+#pragma unroll 1
+        for (int i = 0; i < D / 2; ++i) {
+          uint32_t w;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(v_u + lane * S::kRow + i * 4));
+          bad_row |= !finite_bf16(w) || !finite_bf16(w >> 16);
+        }
+        const unsigned bad = __ballot_sync(0xffffffffu, bad_row);
+        if (bad) {
+          for (unsigned left = bad; left; left &= left - 1) {
+            const int j = __ffs(left) - 1;  // key base + j: column tile j / 8, thread (j % 8) / 2
+            const int src = (lane & ~3) | ((j & 7) >> 1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float p = 0.f;
+#pragma unroll
+              for (int nt = 0; nt < 4; ++nt)
+                if (nt == j >> 3) p = j & 1 ? s[nt][2 * i + 1] : s[nt][2 * i];
+              p = __shfl_sync(0xffffffffu, p, src);
+              const bool vis = sees(i, base + j);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                uint32_t w;
+                asm volatile("ld.shared.u32 %0, [%1];"
+                             : "=r"(w)
+                             : "r"(v_u + j * S::kRow + (nt * 8 + 2 * t) * 2));
+                const float2 v = bf16x2_to_float2(w);
+                if (vis && !finite_bf16(w)) o[nt][2 * i] = fmaf(p, v.x, o[nt][2 * i]);
+                if (vis && !finite_bf16(w >> 16)) o[nt][2 * i + 1] = fmaf(p, v.y, o[nt][2 * i + 1]);
+              }
             }
           }
-        }
-        __syncwarp();
-        if (bad_row) {
+          __syncwarp();
+          if (bad_row) {
 #pragma unroll 1
-          for (int i = 0; i < D / 2; ++i) {
-            const uint32_t at = v_u + lane * S::kRow + i * 4;
-            uint32_t w;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
-            if (!finite_bf16(w)) w &= 0xffff0000u;
-            if (!finite_bf16(w >> 16)) w &= 0x0000ffffu;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+            for (int i = 0; i < D / 2; ++i) {
+              const uint32_t at = v_u + lane * S::kRow + i * 4;
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+              if (!finite_bf16(w)) w &= 0xffff0000u;
+              if (!finite_bf16(w >> 16)) w &= 0x0000ffffu;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    // weighted values: the probabilities rounded to bf16, as the matrix
-    // instructions take them (half a step of 2^-8 relative each, unbiased)
+      // weighted values: the probabilities rounded to bf16, as the matrix
+      // instructions take them (half a step of 2^-8 relative each, unbiased)
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      uint32_t p[4];
+      for (int kk = 0; kk < 2; ++kk) {
+        uint32_t p[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int nt = 2 * kk + (j >> 1);
-        float x = s[nt][2 * (j & 1)], y = s[nt][2 * (j & 1) + 1];
-        if constexpr (E4M3) {  // the values' scales, powers of two
-          x *= v_scale[nt][0];
-          y *= v_scale[nt][1];
+        for (int j = 0; j < 4; ++j) {
+          const int nt = 2 * kk + (j >> 1);
+          p[j] = tc::pack_bf16x2(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
         }
-        p[j] = tc::pack_bf16x2(x, y);
-      }
 #pragma unroll
-      for (int n2 = 0; n2 < NT / 2; ++n2) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, v_u + (kk * 16 + (lane & 15)) * S::kRow + n2 * 32 + (lane >> 4) * 16);
-        mma_16816(o[2 * n2], p, b[0], b[1]);
-        mma_16816(o[2 * n2 + 1], p, b[2], b[3]);
+        for (int n2 = 0; n2 < NT / 2; ++n2) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, v_u + (kk * 16 + (lane & 15)) * S::kRow + n2 * 32 + (lane >> 4) * 16);
+          mma_16816(o[2 * n2], p, b[0], b[1]);
+          mma_16816(o[2 * n2 + 1], p, b[2], b[3]);
+        }
       }
+      __syncwarp();  // the stage may be filled again
     }
-    __syncwarp();  // the stage may be filled again
   }
   cp_async_wait<0>();
   __syncwarp();
@@ -447,10 +533,32 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = g + 8 * i;
+    if constexpr (E4M3) {
+      // O is relative to W 2^-14; column tiles 4 b + q hold columns 32 b + 4 n + q
+      const float back = top_w[i] * pow2(-14);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      *reinterpret_cast<float2*>(mine + r * D + nt * 8 + 2 * t) =
-          make_float2(o[nt][2 * i], o[nt][2 * i + 1]);
+      for (int b = 0; b < NB; ++b) {
+        float f[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f[q] = o[4 * b + q][2 * i] * back;
+          f[4 + q] = o[4 * b + q][2 * i + 1] * back;
+        }
+        if (const uint32_t cols = poison[r * 4 + b] >> (8 * t) & 0xffu) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (cols >> q & 1) f[q] = NAN;
+        }
+        float4* dst = reinterpret_cast<float4*>(mine + r * D + 32 * b + 8 * t);
+        dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+        dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        *reinterpret_cast<float2*>(mine + r * D + nt * 8 + 2 * t) =
+            make_float2(o[nt][2 * i], o[nt][2 * i + 1]);
+    }
     if (t == 0) {
       mine[kDecRows * D + r] = m[i];
       mine[kDecRows * D + kDecRows + r] = l[i];
