@@ -245,9 +245,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
   };
 
   uint32_t top = 0, low = 0xffffffffu;  // the largest key, and the least but 0
-  for (int v = v0 + lane; v < v1; v += 32) {
-    uint32_t ky[N];
-    fetch(v, ky);
+  auto take = [&](int v, const uint32_t (&ky)[N]) {
     if (staged) {
       uint4 w;
       Key* e = reinterpret_cast<Key*>(&w);
@@ -260,6 +258,27 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
       top = max(top, ky[i]);
       low = min(low, ky[i] - 1);  // key 0 wraps round
     }
+  };
+  int v = v0 + lane;
+  if (aligned) {  // four vectors on their way at once
+    for (; v + 96 < v1 && (v + 97) * N <= V; v += 128) {
+      uint4 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint4*>(logits)[v + 32 * j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T* e = reinterpret_cast<const T*>(&w[j]);
+        uint32_t ky[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) ky[i] = key_of(plus_zero(e[i]));
+        take(v + 32 * j, ky);
+      }
+    }
+  }
+  for (; v < v1; v += 32) {
+    uint32_t ky[N];
+    fetch(v, ky);
+    take(v, ky);
   }
   if (x == 0) s.pick = V;
   top = block_max(top, s);
@@ -342,6 +361,19 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
       for (int i = 0; i < N; ++i) f(ky[i]);
     }
   };
+  // f(keys of 32 lanes) for each element whose test holds in some lane: after a
+  // filter few do, and the rest need no exponentials
+  auto each_where = [&](auto test, auto f) {
+    for (int v = v0 + lane; v - lane < v1; v += 32) {
+      uint32_t ky[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) ky[i] = 0;
+      if (v < v1) load(v, ky);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (__any_sync(0xffffffffu, test(ky[i]))) f(ky[i]);
+    }
+  };
   auto clear_hist = [&]() {
     __syncthreads();
     for (int i = x; i < 2 * kBins; i += kSampleThreads) hist_lo[i] = 0;
@@ -370,13 +402,31 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
     }
     __syncthreads();
   };
+  // The keys of a step: bin_of does not increase with the key, so they are a
+  // range, found by 32 lanes trying 32 keys at a time.
+  auto last_key = [&](int bin) {  // the largest key with bin_of(key) >= bin, at least `low`
+    uint32_t lo = low, hi = top;
+    while (lo < hi) {
+      const uint32_t part = (hi - lo) / 32 + 1;
+      const uint32_t ky = lo + part * (lane + 1);
+      const unsigned in = __ballot_sync(0xffffffffu, ky <= hi && ky > lo && bin_of(ky) >= bin);
+      const uint32_t n = __popc(in);  // a run of the first lanes
+      hi = min(hi, lo + part * (n + 1) - 1);
+      lo = lo + part * n;
+    }
+    return lo;
+  };
   // the cluster's keys of s.bin above `floor_key` to the first CTA's list
   auto make_list = [&](uint32_t floor_key, bool with_mass) {
     const int bin = s.bin;
+    uint32_t from = bin + 1 < kBins ? last_key(bin + 1) : low - 1;
+    if (bin + 1 < kBins && from == low && bin_of(low) <= bin) from = low - 1;
+    from = max(from, floor_key);
+    const uint32_t upto = last_key(bin);
     const uint32_t count = tc::mapa_shared(&s.listed, 0);
     const uint32_t key_at = tc::mapa_shared(list_key, 0), mass_at = tc::mapa_shared(list_mass, 0);
     each([&](uint32_t ky) {
-      if (ky > floor_key && bin_of(ky) == bin) {
+      if (ky > from && ky <= upto) {
         const uint32_t at = atom_cluster_inc(count);
         if (at < kList) {
           st_cluster_u32(key_at + at * 4, ky);
@@ -459,22 +509,31 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
     if (k > 0 && k < V) exchange(0, 0, s);  // the histograms and the list have been read
     clear_hist();
     u64 at_cut = 0;
-    for (int v = v0 + lane; v < v1; v += 32) {
-      uint32_t ky[N];
-      u64 w[N];
-      load(v, ky);
+    auto add = [&](uint32_t ky, u64 w) {
+      const uint32_t lo = (uint32_t)w;
+      const int bin = bin_of(ky);
+      const uint32_t old = atomicAdd(&hist_lo[bin], lo);
+      const uint32_t up = (uint32_t)(w >> 32) + (old + lo < lo ? 1u : 0u);
+      if (up) atomicAdd(&hist_hi[bin], up);
+    };
+    if (cut > 1) {
+      each_where([&](uint32_t ky) { return ky >= cut; }, [&](uint32_t ky) {
+        const u64 w = mass(ky);
+        if (ky > cut) add(ky, w);
+        at_cut += ky == cut;
+      });
+    } else {
+      for (int v = v0 + lane; v < v1; v += 32) {
+        uint32_t ky[N];
+        u64 w[N];
+        load(v, ky);
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = mass(ky[i]);
+        for (int i = 0; i < N; ++i) w[i] = mass(ky[i]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (ky[i] > cut && w[i] != 0) {
-          const uint32_t lo = (uint32_t)w[i];
-          const int bin = bin_of(ky[i]);
-          const uint32_t old = atomicAdd(&hist_lo[bin], lo);
-          const uint32_t up = (uint32_t)(w[i] >> 32) + (old + lo < lo ? 1u : 0u);
-          if (up) atomicAdd(&hist_hi[bin], up);
+        for (int i = 0; i < N; ++i) {
+          if (ky[i] > cut && w[i] != 0) add(ky[i], w[i]);
+          at_cut += ky[i] == cut;
         }
-        at_cut += ky[i] == cut;
       }
     }
     exchange(block_sum(at_cut, s), 0, s);
@@ -578,11 +637,19 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
 
   // each warp's kept mass: of the tokens at the cut, the first `ties` by index
   u64 mine = 0, eq = 0;
-  each([&](uint32_t ky) {
-    const u64 w = kept(ky);
-    mine += ky > cut ? w : 0;
-    eq += ky == cut;
-  });
+  if (cut > 1) {
+    each_where([&](uint32_t ky) { return ky >= cut; }, [&](uint32_t ky) {
+      const u64 w = kept(ky);
+      mine += ky > cut ? w : 0;
+      eq += ky == cut;
+    });
+  } else {
+    each([&](uint32_t ky) {
+      const u64 w = kept(ky);
+      mine += ky > cut ? w : 0;
+      eq += ky == cut;
+    });
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -616,7 +683,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
   const u64 upto_w = base + warp_upto(sum_w, lane);
   const unsigned past = __ballot_sync(0xffffffffu, lane < kSampleWarps && upto_w > target);
   if (target < base || warp != __ffs(past) - 1) return;
-  // the drawn token is in this warp's part
+  // the drawn token is in this warp's part; its logarithm by (l - max l) / T, which
+  // needs no second logarithm
+  const double log_total = log((double)total * (1.0 / (double)(1ull << kMassBits)));
+  auto log_mass = [&](uint32_t ky) {
+    return ky == top ? 0.0 : ((double)value_of(ky, T()) - (double)top_v) / (double)temp;
+  };
   u64 run = __shfl_sync(0xffffffffu, upto_w - sum_w, warp);
   u64 eq_run = __shfl_sync(0xffffffffu, eq_before_w, warp);
   for (int vb = v0; vb < v1; vb += 32) {
@@ -644,7 +716,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (r <= target && target < r + w[i])
-          finish(v * N + i, (float)log((double)w[i] / (double)total));
+          finish(v * N + i, (float)(log_mass(ky[i]) - log_total));
         r += w[i];
       }
     }
