@@ -114,39 +114,62 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppen
 }
 
 // Sequence b's rows as dense [B, KVH, max_len, D] bf16; zeros past its
-// context.  A thread writes one 16-byte vector and reads as much (bf16) or
-// half (e4m3) from the page.
-template <bool E4M3>
-__global__ void __launch_bounds__(256) paged_gather_kernel(PagedGatherArgs a) {
+// context.  A CTA writes 64 or 128 rows; a thread asks for all of its vectors
+// (16 bytes of bf16, 8 of e4m3) before it stores the first.
+constexpr int kGatherThreads = 256;
+__host__ __device__ constexpr int gather_rows(int d) { return d <= 64 ? 128 : 64; }
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(kGatherThreads) paged_gather_kernel(PagedGatherArgs a) {
+  constexpr int NV = D / 8;  // vectors of a row
+  constexpr int U = gather_rows(D) * NV / kGatherThreads;
+  static_assert(U * kGatherThreads == gather_rows(D) * NV, "whole vectors per thread");
   griddep_wait();
   griddep_launch();
-  const int nv = a.kv.head_dim >> 3;
   const int b = blockIdx.z, h = blockIdx.y % a.kv.kv_heads;
   const bool is_k = blockIdx.y < (unsigned)a.kv.kv_heads;
   const int n = min(context_of(a.batch, a.kv, b, a.status), a.max_len);
   const void* pool = is_k ? a.kv.key : a.kv.value;
   const uint8_t* scale = is_k ? a.kv.key_scale : a.kv.value_scale;
+  const long long p0 = (long long)blockIdx.x * gather_rows(D);
   uint4* out = reinterpret_cast<uint4*>(is_k ? a.key_out : a.value_out) +
-               ((long long)b * a.kv.kv_heads + h) * a.max_len * nv;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-       i < (long long)a.max_len * nv; i += (long long)gridDim.x * blockDim.x) {
-    const int p = (int)(i / nv), c = (int)(i - (long long)p * nv);
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (p < n) {
-      const int page = page_of(a.batch, a.kv, b, p, a.status);
-      if (page >= 0) {
-        const long long r = pool_row(a.kv, page, h, p);
-        if constexpr (E4M3) {
-          const uint2 w = *(reinterpret_cast<const uint2*>(pool) + r * nv + c);
-          const uint32_t s2 = scale_pair(scale[r]);
-          const uint2 lo = e4m3x4_to_bf16(w.x, s2), hi = e4m3x4_to_bf16(w.y, s2);
-          v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        } else {
-          v = *(reinterpret_cast<const uint4*>(pool) + r * nv + c);
-        }
-      }
+               (((long long)b * a.kv.kv_heads + h) * a.max_len + p0) * NV;
+  const int left = (int)min((long long)gather_rows(D), a.max_len - p0);
+  long long row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int p = (threadIdx.x + u * kGatherThreads) / NV;
+    row[u] = -1;
+    if (p0 + p < n) {
+      const int page = page_of(a.batch, a.kv, b, (int)p0 + p, a.status);
+      if (page >= 0) row[u] = pool_row(a.kv, page, h, (int)p0 + p);
     }
-    out[i] = v;
+  }
+  uint4 v[U];
+  uint32_t s2[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int c = (threadIdx.x + u * kGatherThreads) % NV;
+    v[u] = make_uint4(0u, 0u, 0u, 0u);
+    s2[u] = 0u;
+    if (row[u] < 0) continue;
+    if constexpr (E4M3) {
+      const uint2 w = reinterpret_cast<const uint2*>(pool)[row[u] * NV + c];
+      v[u].x = w.x, v[u].y = w.y;
+      s2[u] = scale[row[u]];
+    } else {
+      v[u] = reinterpret_cast<const uint4*>(pool)[row[u] * NV + c];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = threadIdx.x + u * kGatherThreads;
+    if (E4M3 && row[u] >= 0) {
+      const uint32_t pair = scale_pair(s2[u]);
+      const uint2 lo = e4m3x4_to_bf16(v[u].x, pair), hi = e4m3x4_to_bf16(v[u].y, pair);
+      v[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    if (i / NV < left) out[i] = v[u];
   }
 }
 
@@ -172,14 +195,23 @@ int launch_paged_append(const PagedAppendArgs& a, cudaStream_t stream) {
   return -1;
 }
 
-int launch_paged_gather(const PagedGatherArgs& a, cudaStream_t stream) {
-  const int nv = a.kv.head_dim >> 3;
-  const long long blocks = ((long long)a.max_len * nv + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 65535 ? blocks : 65535),
+template <int D>
+static int launch_gather_d(const PagedGatherArgs& a, cudaStream_t stream) {
+  const dim3 grid((unsigned)(((long long)a.max_len + gather_rows(D) - 1) / gather_rows(D)),
                   (unsigned)(a.kv.kv_heads * (a.kv.value != nullptr ? 2 : 1)),
                   (unsigned)a.batch.batch);
-  auto k = a.kv.key_scale != nullptr ? paged_gather_kernel<true> : paged_gather_kernel<false>;
-  return launch_pdl(k, grid, dim3(256), 0, stream, a) == cudaSuccess ? 0 : -2;
+  auto k = a.kv.key_scale != nullptr ? paged_gather_kernel<D, true> : paged_gather_kernel<D, false>;
+  return launch_pdl(k, grid, dim3(kGatherThreads), 0, stream, a) == cudaSuccess ? 0 : -2;
+}
+
+int launch_paged_gather(const PagedGatherArgs& a, cudaStream_t stream) {
+  switch (a.kv.head_dim) {
+    case 32: return launch_gather_d<32>(a, stream);
+    case 64: return launch_gather_d<64>(a, stream);
+    case 96: return launch_gather_d<96>(a, stream);
+    case 128: return launch_gather_d<128>(a, stream);
+  }
+  return -1;
 }
 
 }  // namespace parrot
