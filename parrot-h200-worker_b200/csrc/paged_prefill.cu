@@ -60,14 +60,22 @@ template <int D, bool E4M3, bool SEP>
 struct PrefillShape {
   static constexpr int kGroups = tile_groups(D), kKeys = tile_keys(D);
   static constexpr int kRows = kGroup * kGroups, kRowWarps = 4 * kGroups;
-  static constexpr int kLoadWarps = E4M3 ? 7 : 3;  // widening takes more
-  static constexpr int kMmaWarp = kRowWarps + kLoadWarps, kThreads = 32 * (kMmaWarp + 1);
-  // Registers of a rows' thread and of the others: their sum stays within the
-  // launch's, 65536 / kThreads rounded down to 8 each (0: no split).
-  static constexpr int kRowRegs = E4M3 ? (kGroups == 2 ? 184 : 120) : kGroups == 2 ? 208 : 0;
-  static constexpr int kOtherRegs = E4M3 ? (kGroups == 2 ? 72 : 56) : 88;
-  static_assert(kRowRegs == 0 || (kRowRegs * kRowWarps + kOtherRegs * (kLoadWarps + 1)) * 32 <=
-                                     65536 / kThreads / 8 * 8 * kThreads, "register split");
+  static constexpr int kLoadWarps = E4M3 ? 8 : 3;  // widening takes more
+  // whole warpgroups: an e4m3 kernel's matrix warp has three idle beside it
+  static constexpr int kMmaWarp = kRowWarps + kLoadWarps;
+  static constexpr int kThreads = 32 * (kMmaWarp + (E4M3 ? 4 : 1));
+  // Registers of a thread of the rows', of the loading warps and of the matrix
+  // warp's group (bf16: the loading warps are in it; 0: no split).  setmaxnreg
+  // draws on what the launch gave the CTA, the same for each of the SM's four
+  // schedulers, and a warpgroup has a warp on each: their sum stays within it.
+  static constexpr int kRowRegs = E4M3 ? (kGroups == 2 ? 152 : 104) : kGroups == 2 ? 208 : 0;
+  static constexpr int kLoadRegs = E4M3 ? 64 : 88;
+  static constexpr int kMmaRegs = E4M3 ? (kGroups == 2 ? 48 : 40) : 88;
+  static_assert(kThreads % 128 == 0, "whole warpgroups");
+  static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
+  static_assert(kRowRegs == 0 || kRowRegs * kRowWarps + (E4M3 ? kLoadRegs * kLoadWarps : 0) +
+                                         kMmaRegs * 4 <= kLaunchRegs * (kThreads / 32),
+                "register split");
   // TMEM columns: S (and P over it) of group g at g * kKeys, O behind
   static constexpr uint32_t kTmemO = kGroups * kKeys;
   static_assert(kGroups * (kKeys + D) <= 512, "S and O of all groups");
@@ -95,8 +103,9 @@ struct PrefillState {
   int bad[6];
   uint64_t* armed[2][6];       // the barrier of each stage's last copy, and its phase
   uint32_t armed_parity[2][6];
-  int row[2][128];             // e4m3: pool row of each key of two tiles, -1: zeros
-  uint32_t scale[2][128];      // their scale bytes (key, value)
+  // e4m3, of three units of each half of the loading warps
+  int row[2][3][128];          // pool row of each key, -1: zeros
+  int scale[2][3][128];        // its scale byte
   uint4 poison[kGroup * kMaxGroups];
   float m[kGroup * kMaxGroups], l[kGroup * kMaxGroups];  // merge
 };
@@ -305,9 +314,9 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&st.k_full[s], 1);
+      mbar_init(&st.k_full[s], E4M3 ? S::kLoadWarps / 2 : 1);
       mbar_init(&st.k_empty[s], 1);
-      mbar_init(&st.v_full[s], 1);
+      mbar_init(&st.v_full[s], E4M3 ? S::kLoadWarps / 2 : 1);
       mbar_init(&st.v_empty[s], 1);
       mbar_init(&st.raw[s], 1);
       st.bad[s] = 0;
@@ -329,7 +338,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
                                         gridDim.x / (ranks * a.kv.kv_heads));
   if (tile.b < 0) return;  // the whole cluster, before any wait
   const int rows = min(R, tile.n * group - tile.row0);
-  const bool loads = warp >= S::kRowWarps && warp < S::kMmaWarp;  // these need neither Q nor TMEM
+  const bool loads = warp >= S::kRowWarps && warp != S::kMmaWarp;  // these need neither Q nor TMEM
   if (warp == S::kMmaWarp) tmem_alloc(&st.tmem, 512);
   if (warp < S::kRowWarps) {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
     const int r = warp * 32 + lane, row = tile.row0 + r, head = kvh * group + row % group;
@@ -556,9 +565,13 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks, 32 * S::kRowWarps);
     return;
   }
-  if constexpr (S::kRowRegs > 0)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
-  if (warp < S::kRowWarps + S::kLoadWarps) {
+  if constexpr (S::kRowRegs > 0) {
+    if (E4M3 && warp < S::kMmaWarp)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kLoadRegs));
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kMmaRegs));
+  }
+  if (warp < S::kMmaWarp) {
     // ---------------- keys and values ----------------
     const int lt = threadIdx.x - 32 * S::kRowWarps;
     uint32_t raw_phase = 0;            // a bit per stage
@@ -669,106 +682,123 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
         }
       }
     } else {
-      // A unit is one side of a tile.  Its raw vectors are loaded while the unit
-      // before is widened, and the list of a tile's rows while the tile before is
-      // in work, so that no load is waited for where it is issued.
-      constexpr int LT = 32 * S::kLoadWarps;
+      // A unit is one side of a tile (of a latent, a tile); the even units are the
+      // first four warps', the odd ones the others'.  A unit's raw vectors are
+      // loaded while the one before is widened, and the list of its rows takes
+      // three steps (page, row and scale, list), one a unit, so that no load is
+      // waited for where it is issued.
+      constexpr int LT = 16 * S::kLoadWarps;            // threads of a half
       constexpr int VR = D / 16;                        // 16-byte vectors of a raw row
-      constexpr int kPer = (T * VR + LT - 1) / LT;          // of a thread
+      constexpr int kPer = T * VR / LT;                 // of a thread
+      static_assert(T <= LT && kPer * LT == T * VR, "whole vectors, one row or none per thread");
+      const int half = lt / LT, ht = lt - half * LT;
+      // unit x of this half
+      auto tile_of = [&](int x) { return SEP ? x : 2 * x + half; };
+      const int units = SEP ? n : (n - half + 1) / 2;
+      const bool values = SEP && half == 1;
+      const uint4* pool = reinterpret_cast<const uint4*>(values ? a.kv.value : a.kv.key);
+      const uint8_t* pool_scale = values ? a.kv.value_scale : a.kv.key_scale;
+      uint64_t* full_bars = values ? st.v_full : st.k_full;
+      uint64_t* empty_bars = values ? st.v_empty : st.k_empty;
       uint4 raw[kPer];
-      auto rows_of = [&](int i, int list) {  // into st.row[list], st.scale[list]
-        if (i >= n) return;
-        for (int k = lt; k < T; k += LT) {
-          const int j = base_of(i) + k;
-          int at = -1;
-          if (some_row_sees(j)) {
-            const int page = page_of(a.batch, a.kv, tile.b, j, a.status);
-            if (page >= 0) at = (int)pool_row(a.kv, page, kvh, j);
-          }
-          st.row[list][k] = at;
-          st.scale[list][k] = at < 0 ? 0u : (uint32_t)a.kv.key_scale[at] |
-                                                (SEP ? (uint32_t)a.kv.value_scale[at] << 8 : 0u);
-        }
+      int page = -1, at = -1, scale = 0;  // of this thread's key: units x + 3, x + 2
+      auto page_step = [&](int x) {
+        const int j = base_of(tile_of(x)) + ht;
+        page = x < units && ht < T && some_row_sees(j)
+                   ? a.batch.page_table[(long long)tile.b * a.batch.table_width + (j >> a.kv.page_shift)]
+                   : -1;
       };
-      auto fetch = [&](int i, int side) {
-        if (i >= n) return;
-        const uint4* pool = reinterpret_cast<const uint4*>(side ? a.kv.value : a.kv.key);
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          const int v = lt + LT * x, k = v / VR;
-          if (T * VR % LT == 0 || v < T * VR) {
-            const int at = st.row[i & 1][k];
-            raw[x] = at >= 0 ? pool[(long long)at * VR + (v - k * VR)] : make_uint4(0, 0, 0, 0);
+      auto row_step = [&](int x) {
+        const int j = base_of(tile_of(x)) + ht;
+        at = -1;
+        scale = 0;
+        if (x < units && ht < T && some_row_sees(j)) {
+          if ((unsigned)page < (unsigned)a.kv.pages) {
+            at = (int)pool_row(a.kv, page, kvh, j);
+            scale = pool_scale[at];
+          } else {
+            report_status(a.status, kStatusBadIndex, 52, page);
           }
         }
       };
-      auto widen = [&](unsigned char* dst, int list, int shift, int s, bool check) {
-        bool any = false;
+      auto list_step = [&](int x) {
+        if (ht < T) {
+          st.row[half][x % 3][ht] = at;
+          st.scale[half][x % 3][ht] = scale;
+        }
+      };
+      auto fetch = [&](int x) {
+        if (x >= units) return;
+        const int* list = st.row[half][x % 3];
 #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          const int v = lt + LT * x, k = v / VR, c = v - k * VR;
-          if (T * VR % LT == 0 || v < T * VR) {
-            const uint32_t s2 = scale_pair(st.scale[list][k] >> shift & 0xff);
-            uint4 o[2];
-            e4m3x16_numbers(raw[x], o);
+        for (int v = 0; v < kPer; ++v) {
+          const int i = ht + LT * v, k = i / VR;
+          const int r = list[k];
+          raw[v] = r >= 0 ? pool[(long long)r * VR + (i - k * VR)] : make_uint4(0, 0, 0, 0);
+        }
+      };
+      page_step(0);
+      row_step(0);
+      page_step(1);
+      list_step(0);
+      row_step(1);
+      page_step(2);
+      list_step(1);
+      named_sync(3 + half, LT);
+      fetch(0);
+      row_step(2);
+      page_step(3);
+      for (int x = 0; x < units; ++x) {
+        const int i = tile_of(x), s = i % NS;
+        const bool check = (!SEP || values) && is_edge(base_of(i));
+        const bool mine = i < NS || wait_asleep(&empty_bars[s], (i / NS - 1) & 1, abort_flag, a.status, 63);
+        if (check && mine) {  // nobody reads what this stage noted before
+          if (ht < T) bad_cols[s * T + ht] = make_uint4(0, 0, 0, 0);
+          if (ht == 0) st.bad[s] = 0;
+        }
+        // all stop together; the lists and notes above are complete
+        if (named_or(3 + half, LT, !mine)) break;
+        unsigned char* dst = smem + S::kQ + (values ? S::kRing : 0) + s * S::kTile;
+        const int* list = st.scale[half][x % 3];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              o[h].x = mul_bf16x2_exact(o[h].x, s2);
-              o[h].y = mul_bf16x2_exact(o[h].y, s2);
-              o[h].z = mul_bf16x2_exact(o[h].z, s2);
-              o[h].w = mul_bf16x2_exact(o[h].w, s2);
-              if (check) {
-                const uint32_t bits = not_finite8(o[h]);
-                if (bits) {
-                  any = true;
-                  const int c8 = 2 * c + h;
-                  uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * T + k);
-                  if (SEP) {
-                    atomicOr(cols + (c8 >> 2), bits << (8 * (c8 & 3)));
-                  } else {
-                    for (int q = 0; q < 4; ++q) atomicOr(cols + q, 0xffffffffu);
-                  }
-                  o[h].x &= keep_mask(bits, 0);
-                  o[h].y &= keep_mask(bits, 1);
-                  o[h].z &= keep_mask(bits, 2);
-                  o[h].w &= keep_mask(bits, 3);
+        for (int v = 0; v < kPer; ++v) {
+          const int e = ht + LT * v, k = e / VR, c = e - k * VR;
+          const uint32_t s2 = scale_pair(list[k]);
+          uint4 o[2];
+          e4m3x16_numbers(raw[v], o);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            o[h].x = mul_bf16x2_exact(o[h].x, s2);
+            o[h].y = mul_bf16x2_exact(o[h].y, s2);
+            o[h].z = mul_bf16x2_exact(o[h].z, s2);
+            o[h].w = mul_bf16x2_exact(o[h].w, s2);
+            if (check) {
+              const uint32_t bits = not_finite8(o[h]);
+              if (bits) {
+                const int c8 = 2 * c + h;
+                uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * T + k);
+                if (SEP) {
+                  atomicOr(cols + (c8 >> 2), bits << (8 * (c8 & 3)));
+                } else {  // a latent's key is its value: a row that sees it has no score left
+                  for (int q = 0; q < 4; ++q) atomicOr(cols + q, 0xffffffffu);
                 }
+                *reinterpret_cast<volatile int*>(&st.bad[s]) = 1;
+                o[h].x &= keep_mask(bits, 0);
+                o[h].y &= keep_mask(bits, 1);
+                o[h].z &= keep_mask(bits, 2);
+                o[h].w &= keep_mask(bits, 3);
               }
-              *reinterpret_cast<uint4*>(dst + sw64_at<T>(k, 2 * c + h)) = o[h];
             }
+            *reinterpret_cast<uint4*>(dst + sw64_at<T>(k, 2 * c + h)) = o[h];
           }
         }
-        return any;
-      };
-      rows_of(0, 0);
-      named_sync(1, LT);
-      fetch(0, 0);
-      rows_of(1, 1);
-      bool ok = true;
-      for (int i = 0; ok && i < n; ++i) {
-        const int s = i % NS;
-        const bool edge = is_edge(base_of(i));
-        for (int side = 0; side < S::kSides; ++side) {
-          const bool check = edge && side == S::kSides - 1;
-          if (check)
-            for (int k = lt; k < T; k += LT) bad_cols[s * T + k] = make_uint4(0, 0, 0, 0);
-          uint64_t* empty = side ? &st.v_empty[s] : &st.k_empty[s];
-          const bool mine = i < NS || wait_asleep(empty, (i / NS - 1) & 1, abort_flag, a.status, 63);
-          ok = !named_or(1, LT, !mine);  // all stop together; the lists are complete
-          if (!ok) break;
-          const bool any = widen(smem + S::kQ + side * S::kRing + s * S::kTile, i & 1, 8 * side, s, check);
-          fence_async_shared();
-          // the next unit's loads, on their way while the others finish
-          if (side + 1 < S::kSides) fetch(i, side + 1);
-          else fetch(i + 1, 0);
-          const bool found = named_or(1, LT, any);
-          if (lt == 0) {
-            if (check) st.bad[s] = found;
-            mbar_arrive(side ? &st.v_full[s] : &st.k_full[s]);
-          }
-        }
-        // every thread is past this tile's list
-        if (ok) rows_of(i + 2, i & 1);
+        fetch(x + 1);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_bars[s]);
+        list_step(x + 2);
+        row_step(x + 3);
+        page_step(x + 4);
       }
     }
   } else if (warp == S::kMmaWarp) {
