@@ -120,11 +120,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
   extern __shared__ __align__(128) unsigned char dec_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  const ClusterPlace place = cluster_place();
+  const int ranks = a.cluster, rank = place.rank;
   const int kvh = blockIdx.y, group = a.heads / a.kv.kv_heads;
   griddep_wait();
   griddep_launch();
-  const Tile tile = find_tile(a.batch, group, kDecRows, blockIdx.x / ranks);
+  const Tile tile = find_tile(a.batch, group, kDecRows, place.index);
   if (tile.b < 0) return;  // the whole cluster
   const int n = clamp_context(a.batch, a.kv, tile.ctx, a.status);
   const int rows = min(kDecRows, tile.n * group - tile.row0);

@@ -41,7 +41,7 @@ struct RowMap {
 };
 
 // The tile with this number, sequences in order, ceil(n_b * group / rows_per)
-// tiles each.  A whole warp calls; 32 sequences a step, their lengths loaded
+// tiles each (tokens * heads fits 31 bits).  A whole warp calls; 32 sequences a step, their lengths loaded
 // side by side.
 __device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int rows_per, int tile) {
   const int lane = threadIdx.x & 31;
@@ -51,7 +51,7 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& s, int group, int ro
     int2 r = make_int2(0, 0);
     if (b < s.batch) r = batch_rows(s, b);
     const int n = r.y - r.x, len = b < s.batch ? s.context_len[b] : 0;
-    const int mine = (int)(((long long)n * group + rows_per - 1) / rows_per);
+    const int mine = (int)(((unsigned)(n * group) + rows_per - 1) / rows_per);
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -89,7 +89,7 @@ __device__ __forceinline__ Tile find_tile_from_ends(const PagedBatch& s, int gro
     len = s.context_len[lane];
   }
   const int n = r.y - r.x;
-  const int tiles = (int)(((long long)n * group + rows_per - 1) / rows_per);
+  const int tiles = (int)(((unsigned)(n * group) + rows_per - 1) / rows_per);
   if (index >= (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles)) return Tile{-1, 0, 0, 0, 0};
   // the round: the last one before which at most `index` tiles were taken
   int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)tiles);
@@ -112,6 +112,18 @@ __device__ __forceinline__ Tile find_tile_from_ends(const PagedBatch& s, int gro
   return t;
 }
 
+// This CTA's place in its cluster, the cluster's in the grid, and their number:
+// what divisions of blockIdx.x would give.
+struct ClusterPlace {
+  int rank, index, count;
+};
+__device__ __forceinline__ ClusterPlace cluster_place() {
+  ClusterPlace c;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(c.rank));
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(c.index));
+  asm("mov.u32 %0, %%nclusterid.x;" : "=r"(c.count));
+  return c;
+}
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;

@@ -246,8 +246,10 @@ __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pai
 // share of the tile's 16-byte vectors.
 template <int D>
 __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState& st,
-                                            unsigned char* smem, const Tile& tile, int rows,
-                                            int kvh, int group, int rank, int ranks, int threads) {
+                                            unsigned char* smem, const Tile& tile,
+                                            const RowMap& map, int rows, int kvh, int rank, int ranks,
+                                            int threads) {
+  const int group = map.group;
   tc_fence_before();
   __syncthreads();
   if (ranks == 1) return;
@@ -283,12 +285,12 @@ __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState
       o.w = fmaf(f, x[k].w, o.w);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int row = tile.row0 + r;
+    const int2 th = map(r);
     uint2 w;
     w.x = pack_bf16x2(o.x * inv, o.y * inv);
     w.y = pack_bf16x2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + row / group) * a.heads +
-                                       kvh * group + row % group) * D + c * 4) = w;
+    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D +
+                              c * 4) = w;
   }
   cluster_sync();  // nobody leaves while its result may be read
 }
@@ -308,8 +310,10 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
   const uint32_t q_u = smem_u32(smem), k_u = q_u + S::kQ, v_u = SEP ? k_u + S::kRing : k_u;
   uint4* bad_cols = reinterpret_cast<uint4*>(smem + S::kQ + S::kSides * S::kRing);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ranks = a.cluster, rank = blockIdx.x % ranks;
-  const int kvh = blockIdx.x / ranks % a.kv.kv_heads, group = a.heads / a.kv.kv_heads;
+  const ClusterPlace place = cluster_place();
+  const int ranks = a.cluster, rank = place.rank;
+  const int group = a.heads / a.kv.kv_heads, index = place.index / a.kv.kv_heads;
+  const int kvh = place.index - index * a.kv.kv_heads;
   volatile int* abort_flag = &st.abort;
 
   if (threadIdx.x == 0) {
@@ -334,16 +338,30 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
   }
   __syncthreads();
   griddep_wait();
-  const Tile tile = find_tile_from_ends(a.batch, group, R, blockIdx.x / (ranks * a.kv.kv_heads),
-                                        gridDim.x / (ranks * a.kv.kv_heads));
+  const Tile tile = find_tile_from_ends(a.batch, group, R, index, place.count / a.kv.kv_heads);
   if (tile.b < 0) return;  // the whole cluster, before any wait
   const int rows = min(R, tile.n * group - tile.row0);
+  const int ctx = clamp_context(a.batch, a.kv, tile.ctx, a.status);
+  const int groups = (rows + kGroup - 1) / kGroup;
+  const int pos0 = ctx - tile.n;
+  const RowMap map(tile.row0, group);
+  const int pmin = pos0 + map.token0, pmax = pos0 + map(rows - 1).x;
+  // key tiles: the sinks' that lie before the window's first, then the window's
+  const int lo = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+  const int t_lo = lo / T;
+  const int sink_tiles = min((min(a.sinks, lo) + T - 1) / T, t_lo);
+  const int all = pmax < 0 ? 0 : sink_tiles + pmax / T - t_lo + 1;
+  // all < 2^26: a position is below 2^31
+  const int i0 = (int)((unsigned)(all * rank) / (unsigned)ranks);
+  const int i1 = (int)((unsigned)(all * (rank + 1)) / (unsigned)ranks);
+  const int n = i1 - i0;  // of this CTA
   const bool loads = warp >= S::kRowWarps && warp != S::kMmaWarp;  // these need neither Q nor TMEM
   if (warp == S::kMmaWarp) tmem_alloc(&st.tmem, 512);
   if (warp < S::kRowWarps) {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
-    const int r = warp * 32 + lane, row = tile.row0 + r, head = kvh * group + row % group;
+    const int r = warp * 32 + lane;
+    const int2 th = map(r);
     const uint4* mine = reinterpret_cast<const uint4*>(
-        a.q + (long long)(tile.first + row / group) * a.q_row + (long long)head * D);
+        a.q + (long long)(tile.first + th.x) * a.q_row + (long long)(kvh * group + th.y) * D);
     const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(mine) : 0ull;
     constexpr int VR = D / 8;
     uint4 v[VR];
@@ -371,17 +389,6 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
   // one has finished
   if (!loads) griddep_launch();
 
-  const int ctx = clamp_context(a.batch, a.kv, tile.ctx, a.status);
-  const int groups = (rows + kGroup - 1) / kGroup;
-  const int pos0 = ctx - tile.n;
-  const int pmin = pos0 + tile.row0 / group, pmax = pos0 + (tile.row0 + rows - 1) / group;
-  // key tiles: the sinks' that lie before the window's first, then the window's
-  const int lo = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
-  const int t_lo = lo / T;
-  const int sink_tiles = min((min(a.sinks, lo) + T - 1) / T, t_lo);
-  const int all = pmax < 0 ? 0 : sink_tiles + pmax / T - t_lo + 1;
-  const int i0 = (int)((long long)all * rank / ranks), i1 = (int)((long long)all * (rank + 1) / ranks);
-  const int n = i1 - i0;  // of this CTA
   auto base_of = [&](int i) {
     i += i0;
     return (i < sink_tiles ? i : i - sink_tiles + t_lo) * T;
@@ -399,7 +406,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     if constexpr (S::kRowRegs > 0)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kRowRegs));
     const int g = warp >> 2, quarter = warp & 3, r = warp * 32 + lane;
-    const int pos = pos0 + (tile.row0 + min(r, rows - 1)) / group;
+    const int pos = pos0 + map(min(r, rows - 1)).x;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_at = lane_addr + g * T, o_at = lane_addr + S::kTmemO + g * D;
     const float scale2 = a.scale * kLog2e;
@@ -547,9 +554,8 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
       }
     }
     if (ranks == 1) {
-      const int row = tile.row0 + min(r, rows - 1);
-      __nv_bfloat16* out = a.out + ((long long)(tile.first + row / group) * a.heads +
-                                    kvh * group + row % group) * D;
+      const int2 th = map(min(r, rows - 1));
+      __nv_bfloat16* out = a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D;
       const unsigned long long at = ok && r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
       constexpr int VR = D / 8;
       __syncwarp();
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     }
     st.m[r] = m * scale2;
     st.l[r] = l;
-    finish_rows<D>(a, st, smem, tile, rows, kvh, group, rank, ranks, 32 * S::kRowWarps);
+    finish_rows<D>(a, st, smem, tile, map, rows, kvh, rank, ranks, 32 * S::kRowWarps);
     return;
   }
   if constexpr (S::kRowRegs > 0) {
