@@ -186,8 +186,8 @@ struct KeyType<float> {
 
 }  // namespace
 
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a) {
+template <typename T, int PER_SM>
+__global__ void __launch_bounds__(kSampleThreads, PER_SM) sample_kernel(SampleArgs a) {
   typedef typename KeyType<T>::type Key;
   constexpr int N = 16 / sizeof(T);  // logits, or keys, of a 16-byte vector
   __shared__ Scratch s;
@@ -203,6 +203,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
   griddep_wait();
   griddep_launch();
   Exchange exchange{a.cluster, (int)(blockIdx.x % a.cluster), 0};
+  // arrive now, wait before the first access: every CTA of the cluster has started
+  if (exchange.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int ranks = exchange.ranks, rank = exchange.rank;
   const int row = blockIdx.x / ranks, V = a.vocab;
   const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.row_stride;
@@ -283,6 +285,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
   if (x == 0) s.pick = V;
   top = block_max(top, s);
   low = block_max(~low, s);
+  if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   exchange(top, low, s);
   top = low = 0;
   for (int r = 0; r < ranks; ++r) {
@@ -727,24 +730,31 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(SampleArgs a)
 }
 
 // CTAs per row: as many as leave each thread a vector while all rows' CTAs
-// are resident at once (one per SM).
-static int sample_ranks(int rows, int vecs, int sms) {
+// are resident at once, `per_sm` on an SM.
+static int sample_ranks(int rows, int vecs, int sms, int per_sm) {
   int ranks = 1;
   while (ranks < kSampleMaxRanks && vecs >= 2 * ranks * kSampleThreads &&
-         2LL * ranks * rows <= sms)
+         2LL * ranks * rows <= (long long)per_sm * sms)
     ranks *= 2;
   return ranks;
 }
 
-template <typename T>
-static int launch_sample_t(SampleArgs a, int sms, cudaStream_t stream) {
-  const int n = 16 / (int)sizeof(T);
-  const int vecs = (a.vocab + n - 1) / n;
-  a.cluster = sample_ranks(a.rows, vecs, sms);
+// One CTA an SM has 110 registers a thread, two have 64: with few rows the
+// latency of each step counts (32 rows of 32,768: 28.8 us with one, 30.5 with
+// two), with rows for a quarter of the SMs the second CTA's warps cover it (64
+// rows: 37.7 and 35.0 us; 256: 91.6 and 80.3).  Rows of less than two vectors
+// a thread gain nothing (64 of 4096: 19.9 and 20.6).
+static bool sample_two_per_sm(int rows, int vecs, int sms) {
+  return 4LL * rows > sms && vecs >= 2 * kSampleThreads;
+}
+
+template <typename T, int PER_SM>
+static int launch_sample_t(SampleArgs a, int vecs, int sms, cudaStream_t stream) {
+  a.cluster = sample_ranks(a.rows, vecs, sms, PER_SM);
   if ((long long)a.rows * a.cluster > 0x7fffffffll) return -2;
   const int bytes = (vecs + a.cluster - 1) / a.cluster * 16;
   const int smem = kSampleFixed + (bytes <= kSampleStaged ? bytes : 0);
-  if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+  if (cudaFuncSetAttribute(sample_kernel<T, PER_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return -2;
   cudaLaunchConfig_t cfg = {};
@@ -759,12 +769,20 @@ static int launch_sample_t(SampleArgs a, int sms, cudaStream_t stream) {
   attr[1].val.clusterDim = {(unsigned)a.cluster, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a) == cudaSuccess ? 0 : -2;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, PER_SM>, a) == cudaSuccess ? 0 : -2;
+}
+
+template <typename T>
+static int launch_sample_of(const SampleArgs& a, int sms, cudaStream_t stream) {
+  const int n = 16 / (int)sizeof(T);
+  const int vecs = (a.vocab + n - 1) / n;
+  return sample_two_per_sm(a.rows, vecs, sms) ? launch_sample_t<T, 2>(a, vecs, sms, stream)
+                                              : launch_sample_t<T, 1>(a, vecs, sms, stream);
 }
 
 int launch_sample(const SampleArgs& a, int sms, cudaStream_t stream) {
-  return a.logits_f32 ? launch_sample_t<float>(a, sms, stream)
-                      : launch_sample_t<__nv_bfloat16>(a, sms, stream);
+  return a.logits_f32 ? launch_sample_of<float>(a, sms, stream)
+                      : launch_sample_of<__nv_bfloat16>(a, sms, stream);
 }
 
 }  // namespace parrot
