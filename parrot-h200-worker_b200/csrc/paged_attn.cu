@@ -92,12 +92,14 @@ __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) !
 // a power of two W per row above all its w so far, at 2^14 W^-1: 11 bits down to
 // 2^-28 W, nothing lost above 2^-39 W.
 // ---------------------------------------------------------------------------
-constexpr int kDecWarps = 4;
 constexpr int kDecKeys = 32;
 constexpr int kDecRows = 16;
 
-template <int D, bool E4M3, bool SEP>
+// Warps of a CTA: four, two CTAs an SM; for few tiles as many as one CTA's
+// registers and shared memory hold.
+template <int D, bool E4M3, bool SEP, bool WIDE>
 struct DecodeShape {
+  static constexpr int kWarps = !WIDE ? 4 : D == 128 && SEP && !E4M3 ? 6 : 8;
   static constexpr int kStages = 2;
   // bf16 rows are padded by 16 bytes: an odd number of 16-byte units, so the
   // eight rows of a matrix load fall in different banks
@@ -108,13 +110,15 @@ struct DecodeShape {
   static constexpr int kPoison = kDecRows * 16;  // e4m3: columns of each row that are NaN
   static constexpr int kWarp = E4M3 ? kDecRows * D * 4 + 2 * kDecRows * 4 + kPoison : kStage * kStages;
   static constexpr int kPart = kDecRows * D * 4 + 2 * kDecRows * 4;  // a CTA's result
-  static constexpr int kBytes = kWarp * kDecWarps + kPart;
+  static constexpr int kBytes = kWarp * kWarps + kPart;
   static_assert(kWarp >= kPart, "a warp's ring holds its result");
 };
 
-template <int D, bool E4M3, bool SEP>
-__global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAttnArgs a) {
-  using S = DecodeShape<D, E4M3, SEP>;
+template <int D, bool E4M3, bool SEP, bool WIDE>
+__global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, WIDE ? 1 : 2)
+    paged_decode_kernel(PagedAttnArgs a) {
+  using S = DecodeShape<D, E4M3, SEP, WIDE>;
+  constexpr int W = S::kWarps;
   constexpr int KS = D / 16;  // k steps of q . k
   constexpr int NT = D / 8;   // column tiles of the output
   extern __shared__ __align__(128) unsigned char dec_smem[];
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
   const int sink_chunks = min((min(a.sinks, lo) + kDecKeys - 1) / kDecKeys, c_lo);
   const int chunks = pmax < 0 ? 0 : sink_chunks + pmax / kDecKeys - c_lo + 1;
   auto base_of = [&](int c) { return (c < sink_chunks ? c : c - sink_chunks + c_lo) * kDecKeys; };
-  const int workers = ranks * kDecWarps, me = rank * kDecWarps + warp;
+  const int workers = ranks * W, me = rank * W + warp;
 
   unsigned char* ring = dec_smem + warp * S::kWarp;
   const uint32_t ring_u = tc::smem_u32(ring);
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
     }
   }
   __syncthreads();
-  float* part = reinterpret_cast<float*>(dec_smem + S::kWarp * kDecWarps);
+  float* part = reinterpret_cast<float*>(dec_smem + S::kWarp * W);
   auto write = [&](int r, int col, float4 v, float sum) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
     const int2 th = map(r);
@@ -575,16 +579,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
     w.y = tc::pack_bf16x2(v.z * inv, v.w * inv);
     *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D + col) = w;
   };
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kDecWarps) {
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * W) {
     const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
     float mx = -INFINITY, sum = 0.f;
     const float* w0 = reinterpret_cast<const float*>(dec_smem);
     constexpr int kStride = S::kWarp / 4;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, w0[w * kStride + kDecRows * D + r]);
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, w0[w * kStride + kDecRows * D + r]);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float* p = w0 + w * kStride;
       const float mw = p[kDecRows * D + r];
       const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
@@ -607,8 +611,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
   }
   if (ranks == 1) return;
   tc::cluster_sync();
-  for (int i = rank * 32 * kDecWarps + threadIdx.x; i < rows * (D / 4);
-       i += ranks * 32 * kDecWarps) {
+  for (int i = rank * 32 * W + threadIdx.x; i < rows * (D / 4);
+       i += ranks * 32 * W) {
     const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
     float mx = -INFINITY, sum = 0.f;
     for (int k = 0; k < ranks; ++k)
@@ -630,31 +634,36 @@ __global__ void __launch_bounds__(32 * kDecWarps, 2) paged_decode_kernel(PagedAt
 }
 
 // CTAs per tile: as many as keep every warp two chunks or more of the longest
-// possible context, while the grid stays within three CTAs per SM (one wave: measured at 64
-// sequences 26 us against 31 with four).
-int decode_ranks(const PagedAttnArgs& a, long long tiles, int sms) {
-  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
-  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
-  const long long chunks = (keys + kDecKeys - 1) / kDecKeys;
+// possible context, while the grid stays within `ctas`.
+//
+// That is three CTAs per SM (one wave: measured at 64 sequences 26 us against 31
+// with four).  A few tiles of long contexts, whose warps would go through many
+// chunks one after the other, take the wide kind and clusters of up to 16, on
+// half of the SMs at most (clusters of one CTA an SM fill the GPU's partitions
+// badly: 8 tiles of 16 CTAs run in two turns).  One sequence of a latent of 32,768
+// keys: 49 us with eight CTAs of four warps, 36 with eight of eight, 22 with
+// sixteen; of 8192: 16, 14 and 11; of 4096, where the wide kind begins: 10.5 and
+// 10.1; of 2048 it would lose: 7.6 and 10.0.
+int decode_ranks(long long chunks, long long tiles, int warps, int most, long long ctas) {
   int ranks = 1;
-  while (ranks < 8 && chunks >= 4LL * ranks * kDecWarps && tiles * ranks * 2 <= 3LL * sms) ranks *= 2;
+  while (ranks < most && chunks >= 4LL * ranks * warps && tiles * ranks * 2 <= ctas) ranks *= 2;
   return ranks;
 }
 
-template <int D, bool E4M3, bool SEP>
-int launch_decode(PagedAttnArgs a, cudaStream_t stream, int sms) {
-  using S = DecodeShape<D, E4M3, SEP>;
-  auto k = paged_decode_kernel<D, E4M3, SEP>;
-  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
-  const long long tiles = std::min(n * ((group + kDecRows - 1) / kDecRows),
-                                   n * group / kDecRows + std::min<long long>(a.batch.batch, n));
-  a.cluster = decode_ranks(a, tiles * a.kv.kv_heads, sms);
-  if (tiles * a.cluster > 0x7fffffffll) return -1;
+template <int D, bool E4M3, bool SEP, bool WIDE>
+int launch_decode(PagedAttnArgs a, long long tiles, int ranks, cudaStream_t stream) {
+  using S = DecodeShape<D, E4M3, SEP, WIDE>;
+  auto k = paged_decode_kernel<D, E4M3, SEP, WIDE>;
+  a.cluster = ranks;
+  if (tiles * ranks > 0x7fffffffll) return -1;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
     return -2;
+  if (ranks > 8 &&
+      cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return -2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * a.cluster), a.kv.kv_heads);
-  cfg.blockDim = dim3(32 * kDecWarps);
+  cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);
+  cfg.blockDim = dim3(32 * S::kWarps);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -667,11 +676,26 @@ int launch_decode(PagedAttnArgs a, cudaStream_t stream, int sms) {
   return cudaLaunchKernelEx(&cfg, k, a) == cudaSuccess ? 0 : -2;
 }
 
+template <int D, bool E4M3, bool SEP>
+int launch_decode_of(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
+  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
+  const long long tiles = std::min(n * ((group + kDecRows - 1) / kDecRows),
+                                   n * group / kDecRows + std::min<long long>(a.batch.batch, n));
+  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
+  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
+  const long long chunks = (keys + kDecKeys - 1) / kDecKeys, all = tiles * a.kv.kv_heads;
+  constexpr int kWide = DecodeShape<D, E4M3, SEP, true>::kWarps;
+  if (all * 16 <= sms && chunks >= 128)
+    return launch_decode<D, E4M3, SEP, true>(a, tiles, decode_ranks(chunks, all, kWide, 16, sms / 2), stream);
+  return launch_decode<D, E4M3, SEP, false>(a, tiles, decode_ranks(chunks, all, 4, 8, 3LL * sms), stream);
+}
+
 template <int D>
 int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
-  const bool e = a.kv.key_scale != nullptr, sep = a.kv.value != nullptr;
-  if (e) return sep ? launch_decode<D, true, true>(a, stream, sms) : launch_decode<D, true, false>(a, stream, sms);
-  return sep ? launch_decode<D, false, true>(a, stream, sms) : launch_decode<D, false, false>(a, stream, sms);
+  const bool sep = a.kv.value != nullptr;
+  if (a.kv.key_scale != nullptr)
+    return sep ? launch_decode_of<D, true, true>(a, stream, sms) : launch_decode_of<D, true, false>(a, stream, sms);
+  return sep ? launch_decode_of<D, false, true>(a, stream, sms) : launch_decode_of<D, false, false>(a, stream, sms);
 }
 
 }  // namespace

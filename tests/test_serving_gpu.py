@@ -233,6 +233,31 @@ def test_attention_at_the_model_window(e4m3, queries, contexts):
     _attend(cache, queries, 8, 2048, 4)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,latent", SHAPES)
+@pytest.mark.parametrize("queries,contexts,page,window,sinks", [
+    ([1], [5000], 64, 0, 0), ([2, 1, 0], [4097, 100, 9], 32, 0, 0), ([3], [9001], 128, 5000, 40)])
+def test_attention_of_few_rows_over_long_contexts(e4m3, heads, kv_heads, dim, latent, queries, contexts, page,
+                                                  window, sinks):
+    cache = Paged(contexts, kv_heads=kv_heads, dim=dim, page=page, e4m3=e4m3, latent=latent, seed=dim)
+    _attend(cache, queries, heads, window, sinks, seed=heads)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_attention_of_one_long_context_with_values_that_are_not_finite(e4m3):
+    """A NaN reaches the rows that see it, in its column alone; behind the rows it reaches nobody."""
+    cache = Paged([6000], kv_heads=1, dim=96, page=64, e4m3=e4m3, seed=3)
+    for at, column in ((4500, 17), (5999, 40)):
+        page = int(cache.table[0, at // 64])
+        if e4m3:
+            cache.value.view(torch.uint8)[page, 0, at % 64, column] = 0x7f
+        else:
+            cache.value[page, 0, at % 64, column] = math.nan
+    out = _attend(cache, [2], 4, 0, 0)
+    assert torch.isnan(out[..., 17]).all() and torch.isnan(out[1, :, 40]).all()
+    assert int(torch.isnan(out).sum()) == 3 * 4
+
+
 @pytest.mark.parametrize("queries", [[1, 1], [90, 1]])
 def test_attention_large_scores_keep_the_running_maximum(queries):
     """Scores of some hundreds, rising and falling along the keys."""
