@@ -700,10 +700,17 @@ int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
 
 }  // namespace
 
-// Up to four new tokens per sequence on the average, the kernel above (its
-// tile reads the keys for 16 rows); beyond, paged_prefill.cu's (for 256).
+// Few new tokens per sequence: the kernel above (its tile reads the keys for 16
+// rows); beyond, paged_prefill.cu's (for 256 or 384).  Measured with 8 heads on 2,
+// width 96, a window of 2048: 8 sequences of 4 tokens 16 us here and 24 there, of 8
+// 17 and 25, of 16 20 and 25, of 24 30 and 26; 32 sequences of 2 tokens 20 here, of
+// 4 30 and 26; one of 8 14 and 12.  Single tokens beside pieces go with the pieces
+// (8 beside one of 256: 21 us, and 29 in two launches; 64 beside 512: 58, and 64
+// in two, where the second finds most of its CTAs without work).
 bool paged_few_queries(const PagedAttnArgs& a) {
-  return a.batch.tokens <= 4LL * a.batch.batch;
+  const long long n = a.batch.tokens;
+  return n <= 4LL * a.batch.batch ||
+         (a.batch.batch >= 4 && n <= 16LL * a.batch.batch && n * a.heads <= 64LL * kDecRows);
 }
 
 int launch_paged_decode(const PagedAttnArgs& a, int sms, cudaStream_t stream) {
