@@ -84,9 +84,23 @@ struct MapKeyHash {
 std::mutex g_map_mutex;
 std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_maps;
 
-// Row-major bf16 [rows, cols] matrix, box = box_cols columns (one swizzle span) x box_rows rows.
-bool tensor_map(CUtensorMap* out, const MapKey& key, int box_cols, int box_rows,
-                CUtensorMapSwizzle swizzle) {
+// Row-major bf16 [rows, cols] matrix, boxes of box_cols columns (one swizzle span) x box_rows rows.
+bool encode_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_cols,
+                int box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Boxes of 64 columns, 128-byte swizzle.
+bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
+  const MapKey key{ptr, rows, cols, box_rows};
   {
     std::lock_guard<std::mutex> lock(g_map_mutex);
     auto it = g_maps.find(key);
@@ -95,17 +109,8 @@ bool tensor_map(CUtensorMap* out, const MapKey& key, int box_cols, int box_rows,
       return true;
     }
   }
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)key.cols, (cuuint64_t)key.rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)key.cols * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-  const cuuint32_t estr[2] = {1, 1};
   CUtensorMap map;
-  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(key.ptr), dims,
-                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return false;
+  if (!encode_map(&map, ptr, rows, cols, kGemmBlockK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
   std::lock_guard<std::mutex> lock(g_map_mutex);
   if (g_maps.size() > 4096) g_maps.clear();
   g_maps.emplace(key, map);
@@ -113,17 +118,10 @@ bool tensor_map(CUtensorMap* out, const MapKey& key, int box_cols, int box_rows,
   return true;
 }
 
-// Boxes of 64 columns, 128-byte swizzle.
-bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
-  return tensor_map(out, MapKey{ptr, rows, cols, box_rows}, kGemmBlockK, box_rows,
-                    CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-// A paged pool's rows: boxes of 32 columns, 64-byte swizzle; the key's row
-// count is negative to tell the two apart.
+// A paged pool's rows: boxes of 32 columns, 64-byte swizzle.  Encoded at each
+// call: pools come and go with a server's batches.
 bool pool_map(CUtensorMap* out, const void* ptr, long long rows, int cols, int page_size) {
-  const int box_rows = parrot::paged_prefill_box_rows(cols, page_size);
-  return tensor_map(out, MapKey{ptr, rows, cols, -box_rows}, 32, box_rows,
+  return encode_map(out, ptr, rows, cols, 32, parrot::paged_prefill_box_rows(cols, page_size),
                     CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
@@ -1720,17 +1718,16 @@ int paged_kv(const parrot_paged_kv* kv, parrot::PagedKV* out) {
     return fail(PARROT_EINVAL, "paged: page_size must be 16, 32, 64, 128 or 256%s");
   if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 96 && kv->head_dim != 128)
     return fail(PARROT_EUNSUPPORTED, "paged: head_dim must be 32, 64, 96 or 128%s");
-  if (kv->pages < 0 || kv->n_kv_heads <= 0 || kv->n_kv_heads > 1024)
-    return fail(PARROT_EINVAL, "paged: pages >= 0 and 1 <= n_kv_heads <= 1024 required%s");
+  if (kv->pages <= 0 || kv->n_kv_heads <= 0 || kv->n_kv_heads > 1024)
+    return fail(PARROT_EINVAL, "paged: pages >= 1 and 1 <= n_kv_heads <= 1024 required%s");
   // a row index of a pool, and the tile rows of one head, fit 31 bits
   if ((long long)kv->pages * kv->n_kv_heads * kv->page_size > 0x7fffffffll)
     return fail(PARROT_EINVAL, "paged: pools of more than 2^31 rows%s");
-  if (kv->pages > 0 && (kv->key == nullptr || !aligned16(kv->key) || !aligned16(kv->value)))
+  if (kv->key == nullptr || !aligned16(kv->key) || !aligned16(kv->value))
     return fail(PARROT_EINVAL, "paged: the pools must be given and 16-byte aligned%s");
   if (kv->e4m3 != 0 && kv->e4m3 != 1) return fail(PARROT_EINVAL, "paged: e4m3 must be 0 or 1%s");
-  if (kv->pages > 0 &&
-      ((kv->key_scale != nullptr) != (kv->e4m3 == 1) ||
-       (kv->value_scale != nullptr) != (kv->e4m3 == 1 && kv->value != nullptr)))
+  if ((kv->key_scale != nullptr) != (kv->e4m3 == 1) ||
+      (kv->value_scale != nullptr) != (kv->e4m3 == 1 && kv->value != nullptr))
     return fail(PARROT_EINVAL, "paged: e4m3 pools need their scales, bf16 pools have none%s");
   out->key = kv->key;
   out->value = kv->value;
@@ -1843,8 +1840,9 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
   a.q_row = q_row_stride;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.heads = n_heads;
-  a.window = window;
-  a.sinks = window > 0 ? sinks : 0;
+  // a window that no position of the table leaves is none
+  a.window = window < (long long)a.batch.table_width << a.kv.page_shift ? window : 0;
+  a.sinks = a.window > 0 ? sinks : 0;
   a.scale = scale;
   a.status = status;
   if (parrot::paged_few_queries(a)) {
@@ -1853,7 +1851,7 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
     return check_launch("paged_decode_kernel");
   }
   CUtensorMap k_map{}, v_map{};
-  if (!kv->e4m3 && kv->pages > 0) {
+  if (!kv->e4m3) {
     const long long pool_rows = (long long)kv->pages * kv->n_kv_heads * kv->page_size;
     if (!pool_map(&k_map, kv->key, pool_rows, kv->head_dim, kv->page_size) ||
         (kv->value != nullptr &&

@@ -752,6 +752,8 @@ class PagedKV:
         if page not in PAGE_SIZES or dim not in PAGED_HEAD_DIMS:
             raise ValueError(f"page size must be one of {PAGE_SIZES} and head_dim one of "
                              f"{PAGED_HEAD_DIMS}, got {page} and {dim}")
+        if pages < 1 or heads < 1:
+            raise ValueError("a pool holds at least one page of one head")
         if value is not None and (value.shape != key.shape or value.dtype != key.dtype):
             raise ValueError("value must match key in shape and type")
         e4m3 = key.dtype == torch.float8_e4m3fn
@@ -882,9 +884,9 @@ def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start:
     sequence ``b``, whose context holds ``context_len[b]`` tokens with them.
     ``rope = (cos, sin)``, fp32 [positions, head_dim / 2]: queries and keys are
     rotated at their positions (in fp32, rounded once).  Returns the queries
-    [tokens, n_heads, head_dim], or None for ``n_heads = 0``.  A token whose
-    page or position does not exist is not written; ``status`` (int32 [4])
-    records it.
+    [tokens, n_heads, head_dim], or None for ``n_heads = 0``; rows of no sequence
+    are not written.  A token whose page or position does not exist is not
+    written either; ``status`` (int32 [4]) records it.
     """
     dev = _serving_device(kv.key.device, "paged append")
     _require_inference("paged append")
@@ -951,7 +953,9 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
     sequence ``b`` sees the keys ``j <= p`` of its context with ``window == 0``,
     ``p - j < window`` or ``j < sinks``.  Query head ``h`` reads key head
     ``h // (heads / kv heads)``.  ``scale`` defaults to head_dim ** -0.5.  Returns
-    [tokens, heads, head_dim] bf16; zeros for a token that sees no key.
+    [tokens, heads, head_dim] bf16; zeros for a token that sees no key.  Rows of no
+    sequence are not written.  A page that does not exist counts as zeros, and
+    ``status`` (int32 [4]) records it.
     """
     dev = _serving_device(kv.key.device, "paged attention")
     _require_inference("paged attention")
@@ -963,6 +967,8 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
     if heads % s.n_kv_heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
+    if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
+        raise ValueError("window and sinks must be in [0, 2**31)")
     width = heads * dim
     if q.is_contiguous() and q.data_ptr() % 16 == 0:
         rows, stride = q, width
@@ -1019,6 +1025,8 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
         raise ValueError(f"uniform must be {torch.float32} [{rows}] on {dev}")
     t, t_all = param(temperature, "temperature", torch.float32)
     k, k_all = param(top_k, "top_k", torch.int32)
+    if k is None and not 0 <= k_all < 1 << 31:
+        raise ValueError("top_k must be in [0, 2**31)")
     p, p_all = param(top_p, "top_p", torch.float32)
     m, m_all = param(min_p, "min_p", torch.float32)
     ids = torch.empty((rows, 1), device=dev, dtype=torch.int64)

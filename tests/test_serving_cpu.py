@@ -55,6 +55,14 @@ def test_paged_calls_refuse_bad_batches(lib, kw):
     assert all(rc == E for rc in _calls(lib, _kv(), _batch(**kw)))
 
 
+def test_pools_without_pages_are_refused(lib):
+    """They could name nothing to the copy engine."""
+    assert all(rc == E for rc in _calls(lib, _kv(pages=0), _batch()))
+    for shape in ((0, 2, 64, 96), (3, 0, 64, 96)):
+        with pytest.raises(ValueError, match="at least one page"):
+            bridge.PagedKV(torch.zeros(shape, dtype=torch.bfloat16))
+
+
 def test_paged_calls_refuse_bad_arguments(lib):
     kv, batch = ctypes.byref(_kv()), ctypes.byref(_batch())
     latent = ctypes.byref(_kv(value=None))

@@ -401,6 +401,81 @@ def test_attention_repeats_bit_for_bit_in_graphs_on_two_streams(queries):
     assert torch.equal(outs[0], call(qs[0])) and not torch.equal(outs[0], eager[0])
 
 
+@pytest.mark.parametrize("queries", [[1, 1, 1], [70, 1, 40]])
+def test_a_captured_step_follows_the_lists_it_reads(queries):
+    """Append, attention and read-back captured once and replayed after the page table, the
+    lengths and the rows changed in place."""
+    contexts = [200, 33, 90]
+    cache = Paged(contexts, kv_heads=2, dim=96, page=16, e4m3=True, seed=4, spare=30)
+    kv, width = cache.device(), 18
+    free = [p for p in range(cache.pages) if p not in set(cache.table.flatten().tolist())]
+    table = torch.full((3, width), -1, dtype=torch.int32)
+    table[:, :cache.table.shape[1]] = cache.table
+    more = table.clone()
+    for b, n in enumerate(contexts):
+        have, need = -(-n // 16), -(-(n + 50) // 16)
+        for i in range(have, need):
+            more[b, i] = free.pop()
+    first = table.cuda()
+    start, length = starts(queries).cuda(), ints(contexts)
+    tables = tuple(t.cuda() for t in rope_tables(300, 96))
+    g = torch.Generator().manual_seed(3)
+    rows = [torch.randn(sum(queries), 12 * 96, generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    qkv = rows[0].clone()
+
+    def step(kv, table, length, qkv):
+        q = bridge.b200_paged_append(kv, qkv, table, start, length, 8, tables)
+        y = bridge.b200_paged_attention(q, kv, table, start, length, window=64, sinks=3)
+        return y, *bridge.b200_paged_gather(kv, table, length, 260)
+
+    def fresh():
+        return bridge.PagedKV(*(t.clone() for t in (kv.key, kv.value, kv.key_scale, kv.value_scale)))
+    eager_kv = fresh()
+    want = [step(eager_kv, first, length, rows[0]),
+            step(eager_kv, more.cuda(), length + 50, rows[1])]
+    step(fresh(), first, length, qkv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(kv, first, length, qkv)
+    graph.replay()
+    got = [t.clone() for t in out]
+    first.copy_(more)
+    length.add_(50)
+    qkv.copy_(rows[1])
+    graph.replay()
+    for a, b in zip(want[0] + want[1], got + list(out)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("most", [3, 40])
+def test_more_sequences_than_lanes(e4m3, most):
+    """Seventy sequences, some of them without new tokens, some without any."""
+    g = torch.Generator().manual_seed(most)
+    queries = torch.randint(0, most + 1, (70,), generator=g).tolist()
+    contexts = [n + int(torch.randint(0, 150, (1,), generator=g)) * (i % 5 > 0) for i, n in enumerate(queries)]
+    cache = Paged(contexts, kv_heads=2, dim=96, page=16, e4m3=e4m3, seed=1)
+    _attend(cache, queries, 8, 40, 2)
+
+
+def test_numbers_that_do_not_fit_the_call_are_refused():
+    cache = Paged([50], kv_heads=1, dim=96, page=16)
+    kv, q = cache.device(), torch.randn(1, 2, 96, device="cuda").to(torch.bfloat16)
+    lists = cache.table.cuda(), ints([0, 1]), ints([50])
+    whole = bridge.b200_paged_attention(q, kv, *lists)
+    for window in (50, 10 ** 6, 2 ** 31 - 1):       # no position is that far
+        assert torch.equal(whole, bridge.b200_paged_attention(q, kv, *lists, window=window, sinks=2 ** 31 - 1))
+    for kw in (dict(window=2 ** 32 + 5), dict(window=-1), dict(window=4, sinks=2 ** 32), dict(sinks=-1),
+               dict(window=2 ** 31)):
+        with pytest.raises(ValueError, match="window and sinks"):
+            bridge.b200_paged_attention(q, kv, *lists, **kw)
+    logits, u = torch.randn(1, 64, device="cuda"), torch.full((1,), 0.5, device="cuda")
+    for k in (-1, 2 ** 31, 2 ** 32 + 1):
+        with pytest.raises(ValueError, match="top_k"):
+            bridge.b200_sample(logits, u, top_k=k)
+
+
 def test_offsets_past_32_bits():
     """A pool whose last pages lie behind 2**31 numbers."""
     page, dim = 256, 128
