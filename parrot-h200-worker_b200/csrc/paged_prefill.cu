@@ -13,17 +13,23 @@
 // holds three groups of S and O up to width 96.  A row's maximum m is only moved
 // when it grows by more than 2^8 (p then stays below 2^8, and O and the sum are
 // fp32), so O is rarely rescaled.  The sum is of the unrounded p.
-// Measured slower on four prompts of 4096 each: two groups with tiles of 128
-// keys (135 us); with P in shared memory (its reads and Q's fill shared
-// memory's bandwidth: 151 us); with 96 keys, P apart from S and the next scores
-// computed early (152 us); with steps of 64 keys over two S blocks a group
-// (146 us); with two threads a row (145 us).
+// Measured (8 heads on 2, width 96, a window of 2048): four prompts of 4096 in 116
+// us, 660 TFLOP/s of what the mask leaves, the exponential unit busy for half of
+// the time and the tensor cores for 36%; what is left is the wait of a group for
+// its products and the start and end of a tile.  Slower on the same prompts: two
+// groups with tiles of 128 keys (135 us); with P in shared memory (its reads and
+// Q's fill shared memory's bandwidth: 151 us); with 96 keys, P apart from S and the
+// next scores computed early (152 us); with steps of 64 keys over two S blocks a
+// group (146 us); with two threads a row (145 us); with the maximum taken a tile
+// late (126 us).
 //
-// Warps: the groups' rows first, then three (seven for e4m3) that bring K and V
-// and one that issues the matrix instructions.  A bf16 cache comes by TMA, a page's rows of
-// 32 columns at a time into a 64-byte-swizzled tile (three boxes for a 96-wide
-// head); an e4m3 cache is read, widened and stored to the same tiles by the
-// seven.
+// Warps: the groups' rows first, then three (eight for e4m3) that bring K and V,
+// then the one that issues the matrix instructions.  A bf16 cache comes by TMA, a
+// page's rows of 32 columns at a time into a 64-byte-swizzled tile (three boxes for
+// a 96-wide head).  An e4m3 cache is read, widened and stored to the same tiles by
+// the eight: four for K and four for V, each half's loads a unit ahead of its
+// widening (a prompt of 4096: 69 us, 57 in bf16; seven warps for both sides in
+// turn: 104 us with the lists read where they are used, 91 with them ahead).
 //
 // Tiles at an edge of what the rows see (the diagonal, the window's start, the
 // sinks) pass through two of the three first: in a product 0 * NaN would carry a
