@@ -665,10 +665,11 @@ int launch_decode(PagedAttnArgs a, long long tiles, int ranks, cudaStream_t stre
   auto k = paged_decode_kernel<D, E4M3, SEP, WIDE>;
   a.cluster = ranks;
   if (tiles * ranks > 0x7fffffffll) return -1;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
-    return -2;
-  if (ranks > 8 &&
-      cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+  static std::atomic<unsigned long long> done{0};
+  if (!once_per_device(done, [&] {
+        return allow_shared(k, S::kBytes) &&
+               (!WIDE || cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess);
+      }))
     return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);

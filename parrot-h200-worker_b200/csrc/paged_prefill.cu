@@ -897,8 +897,8 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   const int ranks = (int)std::max(1LL, std::min<long long>(kMaxRanks, sms / (tiles * a.kv.kv_heads)));
   a.cluster = ranks;
   if (tiles * ranks * a.kv.kv_heads > 0x7fffffffll) return -1;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess)
-    return -2;
+  static std::atomic<unsigned long long> done{0};
+  if (!once_per_device(done, [&] { return allow_shared(k, S::kBytes); })) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ranks * a.kv.kv_heads));
   cfg.blockDim = dim3(S::kThreads);

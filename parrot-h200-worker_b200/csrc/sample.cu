@@ -756,8 +756,8 @@ static int launch_sample_t(SampleArgs a, int vecs, int sms, cudaStream_t stream)
   if ((long long)a.rows * a.cluster > 0x7fffffffll) return -2;
   const int bytes = (vecs + a.cluster - 1) / a.cluster * 16;
   const int smem = kSampleFixed + (bytes <= kSampleStaged ? bytes : 0);
-  if (cudaFuncSetAttribute(sample_kernel<T, PER_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-      cudaSuccess)
+  static std::atomic<unsigned long long> done{0};
+  if (!once_per_device(done, [&] { return allow_shared(sample_kernel<T, PER_SM>, kSampleFixed + kSampleStaged); }))
     return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * a.cluster));

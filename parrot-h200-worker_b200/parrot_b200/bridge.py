@@ -742,7 +742,7 @@ class PagedKV:
     ``page_table[b, p // page size]``.
     """
 
-    __slots__ = ("key", "value", "key_scale", "value_scale", "struct")
+    __slots__ = ("key", "value", "key_scale", "value_scale", "struct", "index")
 
     def __init__(self, key: Tensor, value: Tensor | None = None, key_scale: Tensor | None = None,
                  value_scale: Tensor | None = None):
@@ -767,7 +767,7 @@ class PagedKV:
                 pools += (scale,)
         elif key_scale is not None or value_scale is not None:
             raise ValueError("bf16 pools have no scales")
-        where = key.get_device()
+        where = self.index = key.get_device()
         for t in pools:
             if t.get_device() != where or not t.is_contiguous():
                 raise ValueError("the pools and scales must be contiguous, on one device")
@@ -796,31 +796,34 @@ class PagedKV:
         return cls(pool(), pool(), scale(), scale())
 
 
-def _serving_device(dev: torch.device, what: str) -> torch.device:
-    """``dev``, checked to be an sm_100 GPU."""
-    if dev.type != "cuda":
-        raise RuntimeError(f"The B200 {what} backend requires CUDA tensors, got {dev}")
-    ok = _SUPPORTED.get(dev.index)
-    if ok is None:
-        ok = _SUPPORTED[dev.index] = bool(_lib.load().parrot_b200_device_supported(dev.index))
-    if not ok:
-        raise RuntimeError(f"The B200 {what} backend requires an sm_100 GPU (device {dev.index})")
-    return dev
+def _serving_device(t: Tensor, what: str) -> int:
+    """The index of ``t``'s device, checked to be an sm_100 GPU; with autograd off."""
+    index = t.get_device()
+    if not _SUPPORTED.get(index):
+        if not t.is_cuda:
+            raise RuntimeError(f"The B200 {what} backend requires CUDA tensors, got {t.device}")
+        ok = _SUPPORTED[index] = bool(_lib.load().parrot_b200_device_supported(index))
+        if not ok:
+            raise RuntimeError(f"The B200 {what} backend requires an sm_100 GPU (device {index})")
+    _require_inference(what)
+    return index
 
 
 # the current stream's handle without the Stream object that
 # torch.cuda.current_stream() builds around it (2 us of a 15 us call)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
+# without the check that CUDA is initialised: the tensors are on it
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") \
+    else torch.cuda.current_device
 
 
-def _on_device(dev: torch.device, what: str, fn, args) -> None:
-    """``fn(*args, stream)`` with ``dev`` current, on its current stream."""
-    index = dev.index
-    if torch.cuda.current_device() == index:
+def _on_device(index: int, what: str, fn, args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current, on its current stream."""
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
@@ -835,7 +838,7 @@ def _int_list(t: Tensor, index: int) -> Tensor:
 def _paged_batch(kv: PagedKV, page_table: Tensor, query_start: Tensor | None, context_len: Tensor,
                  tokens: int):
     """(struct, the tensors it points into)."""
-    index = kv.key.get_device()
+    index = kv.index
     length = _int_list(context_len, index)
     table = _int_list(page_table, index)
     if table.ndim != 2 or length.ndim != 1:
@@ -852,12 +855,12 @@ def _paged_batch(kv: PagedKV, page_table: Tensor, query_start: Tensor | None, co
                                  length.data_ptr(), n, width, tokens), (table, start, length)
 
 
-def _status_ptr(status: Tensor | None, dev) -> int | None:
+def _status_ptr(status: Tensor | None, index: int) -> int | None:
     if status is None:
         return None
-    if status.dtype != torch.int32 or status.numel() < 4 or status.device != dev or \
+    if status.dtype != torch.int32 or status.numel() < 4 or status.get_device() != index or \
             not status.is_contiguous():
-        raise ValueError(f"status must be a contiguous int32 tensor of 4 on {dev}")
+        raise ValueError(f"status must be a contiguous int32 tensor of 4 on cuda:{index}")
     return status.data_ptr()
 
 
@@ -888,30 +891,30 @@ def b200_paged_append(kv: PagedKV, qkv: Tensor, page_table: Tensor, query_start:
     are not written.  A token whose page or position does not exist is not
     written either; ``status`` (int32 [4]) records it.
     """
-    dev = _serving_device(kv.key.device, "paged append")
-    _require_inference("paged append")
-    if qkv.ndim != 2 or qkv.dtype != torch.bfloat16 or qkv.device != dev:
-        raise RuntimeError(f"The B200 paged append takes bf16 rows [tokens, width] on {dev}")
+    index = _serving_device(kv.key, "paged append")
+    if qkv.ndim != 2 or qkv.dtype is not torch.bfloat16 or qkv.get_device() != index:
+        raise RuntimeError(f"The B200 paged append takes bf16 rows [tokens, width] on cuda:{index}")
     s = kv.struct
-    width = (n_heads + s.n_kv_heads * (1 if kv.value is None else 2)) * s.head_dim
-    if qkv.shape[1] != width:
-        raise ValueError(f"qkv rows must be {width} wide, got {qkv.shape[1]}")
-    tokens = qkv.shape[0]
+    head_dim = s.head_dim
+    width = (n_heads + s.n_kv_heads * (1 if kv.value is None else 2)) * head_dim
+    tokens, given = qkv.shape
+    if given != width:
+        raise ValueError(f"qkv rows must be {width} wide, got {given}")
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
     qkv, stride = _rows_of(qkv)
     cos = sin = None
     if rope is not None:
         cos, sin = rope
         for t in (cos, sin):
-            if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous() or \
-                    t.ndim != 2 or t.shape[1] * 2 != s.head_dim or t.shape != cos.shape:
+            if t.dtype is not torch.float32 or t.get_device() != index or not t.is_contiguous() or \
+                    t.ndim != 2 or t.shape[1] * 2 != head_dim or t.shape != cos.shape:
                 raise ValueError("rope tables must be contiguous fp32 [positions, head_dim / 2]")
-    out = qkv.new_empty((tokens, n_heads, s.head_dim)) if n_heads else None
-    _on_device(dev, "parrot_paged_append_bf16", _lib.load().parrot_paged_append_bf16, (
+    out = qkv.new_empty((tokens, n_heads, head_dim)) if n_heads else None
+    _on_device(index, "parrot_paged_append_bf16", _lib.load().parrot_paged_append_bf16, (
         s, batch, qkv.data_ptr(), max(stride, width), n_heads,
         None if out is None or tokens == 0 else out.data_ptr(),
         None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
-        0 if cos is None else cos.shape[0], _status_ptr(status, dev)))
+        0 if cos is None else cos.shape[0], _status_ptr(status, index)))
     return out
 
 
@@ -921,26 +924,25 @@ def b200_paged_gather(kv: PagedKV, page_table: Tensor, context_len: Tensor, max_
     """The sequences' cached keys and values as dense bf16 [sequences, kv heads,
     ``max_len``, head_dim] (``LocalKVCache``'s layout; value None for a latent
     cache), exactly; zeros past ``context_len``.  ``out``: tensors to fill."""
-    dev = _serving_device(kv.key.device, "paged gather")
-    _require_inference("paged gather")
+    index = _serving_device(kv.key, "paged gather")
     batch, keep = _paged_batch(kv, page_table, None, context_len, 0)
     s = kv.struct
     shape = (batch.batch, s.n_kv_heads, max_len, s.head_dim)
     if out is None:
-        key = torch.empty(shape, device=dev, dtype=torch.bfloat16)
+        key = kv.key.new_empty(shape, dtype=torch.bfloat16)
         value = None if kv.value is None else torch.empty_like(key)
     else:
         key, value = out
         if (value is None) != (kv.value is None):
             raise ValueError("out must hold a value tensor exactly when the cache does")
         for t in (key, value):
-            if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or
-                                  t.device != dev or not t.is_contiguous() or t.data_ptr() % 16):
-                raise ValueError(f"out must be contiguous bf16 {shape} on {dev}")
+            if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != index or
+                                  not t.is_contiguous() or t.data_ptr() % 16):
+                raise ValueError(f"out must be contiguous bf16 {shape} on cuda:{index}")
     if key.numel():
-        _on_device(dev, "parrot_paged_gather_bf16", _lib.load().parrot_paged_gather_bf16, (
+        _on_device(index, "parrot_paged_gather_bf16", _lib.load().parrot_paged_gather_bf16, (
             s, batch, key.data_ptr(), None if value is None else value.data_ptr(), max_len,
-            _status_ptr(status, dev)))
+            _status_ptr(status, index)))
     return key, value
 
 
@@ -957,12 +959,11 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
     sequence are not written.  A page that does not exist counts as zeros, and
     ``status`` (int32 [4]) records it.
     """
-    dev = _serving_device(kv.key.device, "paged attention")
-    _require_inference("paged attention")
+    index = _serving_device(kv.key, "paged attention")
     s = kv.struct
-    if q.ndim != 3 or q.dtype != torch.bfloat16 or q.device != dev or q.shape[2] != s.head_dim:
+    if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.get_device() != index or q.shape[2] != s.head_dim:
         raise RuntimeError(f"The B200 paged attention takes bf16 queries [tokens, heads, "
-                           f"{s.head_dim}] on {dev}")
+                           f"{s.head_dim}] on cuda:{index}")
     tokens, heads, dim = q.shape
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
     if heads % s.n_kv_heads:
@@ -979,9 +980,9 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
         rows, stride = _rows_of(q.as_strided((tokens, width), (q.stride(0), 1)))
         out = q.new_empty((tokens, heads, dim))
     if tokens:
-        _on_device(dev, "parrot_paged_attention_bf16", _lib.load().parrot_paged_attention_bf16, (
+        _on_device(index, "parrot_paged_attention_bf16", _lib.load().parrot_paged_attention_bf16, (
             s, batch, rows.data_ptr(), max(stride, width), out.data_ptr(), heads, window, sinks,
-            dim ** -0.5 if scale is None else scale, _status_ptr(status, dev)))
+            dim ** -0.5 if scale is None else scale, _status_ptr(status, index)))
     return out
 
 
@@ -999,10 +1000,9 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
     log-probability is the logarithm of its own share.  A row of only -inf or
     NaN gives id -1 and -inf.
     """
-    dev = _serving_device(logits.device, "sampling")
+    index = _serving_device(logits, "sampling")
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"The B200 sampling backend takes bf16 or fp32, got {logits.dtype}")
-    _require_inference("sampling")
     if logits.ndim == 3 and logits.shape[1] == 1:
         logits = logits[:, 0]
     if logits.ndim != 2:
@@ -1011,31 +1011,29 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
     if logits.stride(1) != 1 or logits.stride(0) < vocab:
         logits = logits.contiguous()
 
-    index = dev.index
-
     def param(v, name, dtype):
         if not isinstance(v, Tensor):
             return None, v
         if v.ndim != 1 or v.shape[0] != rows or v.dtype is not dtype or v.get_device() != index:
-            raise ValueError(f"{name} must be a number or {dtype} [{rows}] on {dev}")
+            raise ValueError(f"{name} must be a number or {dtype} [{rows}] on cuda:{index}")
         return v if v.is_contiguous() else v.contiguous(), 0
 
     uniform, _ = param(uniform, "uniform", torch.float32)
     if uniform is None:
-        raise ValueError(f"uniform must be {torch.float32} [{rows}] on {dev}")
+        raise ValueError(f"uniform must be {torch.float32} [{rows}] on cuda:{index}")
     t, t_all = param(temperature, "temperature", torch.float32)
     k, k_all = param(top_k, "top_k", torch.int32)
     if k is None and not 0 <= k_all < 1 << 31:
         raise ValueError("top_k must be in [0, 2**31)")
     p, p_all = param(top_p, "top_p", torch.float32)
     m, m_all = param(min_p, "min_p", torch.float32)
-    ids = torch.empty((rows, 1), device=dev, dtype=torch.int64)
+    ids = uniform.new_empty((rows, 1), dtype=torch.int64)
     logprobs = torch.empty_like(uniform)
 
     def ptr(v):
         return None if v is None else v.data_ptr()
 
-    _on_device(dev, "parrot_sample_rows", _lib.load().parrot_sample_rows, (
+    _on_device(index, "parrot_sample_rows", _lib.load().parrot_sample_rows, (
         ids.data_ptr(), logprobs.data_ptr(), logits.data_ptr(),
         int(logits.dtype == torch.float32), max(logits.stride(0), vocab), rows, vocab,
         uniform.data_ptr(), ptr(t), t_all, ptr(k), k_all, ptr(p), p_all, ptr(m), m_all))
