@@ -1,10 +1,42 @@
 // Device helpers shared by the two kernels of attention over the paged cache.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc.cuh"
 
 namespace parrot {
+
+// How many clusters of `ranks` CTAs of a kernel the current device holds at once,
+// asked once for each device and size: clusters of CTAs that fill an SM do not
+// fill the GPU's partitions evenly (8 CTAs: fewer than a GPU's SMs / 8), and one
+// cluster too many doubles a launch's time.
+struct ClusterCapacity {
+  std::atomic<int> plus_one[16][17];
+};
+template <typename K>
+inline int cluster_capacity(ClusterCapacity& cache, K kernel, int threads, int smem, int ranks) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 16 && (n = cache.plus_one[dev][ranks].load(std::memory_order_relaxed)) > 0) return n - 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)ranks, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 16) cache.plus_one[dev][ranks].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -248,56 +248,89 @@ __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pai
   return (bits >> (2 * i) & 1 ? 0u : 0xffffu) | (bits >> (2 * i) & 2 ? 0u : 0xffff0000u);
 }
 
-// The end of the rows' warps: with several CTAs to a tile, each merges its
-// share of the tile's 16-byte vectors.
+// A tile's results of up to K CTAs joined: U of the tile's 16-byte vectors at a
+// time, all of their remote loads on their way together.
+template <int D, int K, int U>
+__device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, PrefillState& st,
+                                           const float* part, const Tile& tile, const RowMap& map,
+                                           int rows, int kvh, int rank, int ranks, uint32_t live,
+                                           int threads) {
+  const int total = rows * (D / 4), stride = ranks * threads;
+  for (int v0 = rank * threads + threadIdx.x; v0 < total; v0 += U * stride) {
+    float mk[U][K], lk[U][K];
+    float4 x[U][K];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = min(v0 + u * stride, total - 1), r = v / (D / 4), c = v - r * (D / 4);
+      const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
+      const uint32_t m_at = smem_u32(&st.m[r]), l_at = smem_u32(&st.l[r]);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        mk[u][k] = -INFINITY;
+        lk[u][k] = 0.f;
+        x[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live >> k & 1) {
+          mk[u][k] = ld_cluster_f1(mapa_addr(m_at, k));
+          lk[u][k] = ld_cluster_f1(mapa_addr(l_at, k));
+          x[u][k] = ld_cluster_f4(mapa_addr(at, k));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * stride, r = v / (D / 4), c = v - r * (D / 4);
+      if (v >= total) break;
+      float mx = mk[u][0], sum = 0.f;
+#pragma unroll
+      for (int k = 1; k < K; ++k) mx = fmaxf(mx, mk[u][k]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float f = mk[u][k] == -INFINITY ? 0.f : exp2_fast(mk[u][k] - mx);
+        sum = fmaf(f, lk[u][k], sum);
+        o.x = fmaf(f, x[u][k].x, o.x);
+        o.y = fmaf(f, x[u][k].y, o.y);
+        o.z = fmaf(f, x[u][k].z, o.z);
+        o.w = fmaf(f, x[u][k].w, o.w);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int2 th = map(r);
+      uint2 w;
+      w.x = pack_bf16x2(o.x * inv, o.y * inv);
+      w.y = pack_bf16x2(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * map.group + th.y) * D +
+                                c * 4) = w;
+    }
+  }
+}
+
+// The end of the rows' warps: with several CTAs to a tile, each merges its share
+// of the tile's vectors.  (Working each row's weights out first and keeping eight
+// vectors on their way whatever the cluster: 3 us slower with eight CTAs.)
 template <int D>
 __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState& st,
                                             unsigned char* smem, const Tile& tile,
                                             const RowMap& map, int rows, int kvh, int rank, int ranks,
-                                            int threads) {
-  const int group = map.group;
+                                            int all, int threads) {
   tc_fence_before();
   __syncthreads();
   if (ranks == 1) return;
+  uint32_t live = 0;  // the CTAs that had key tiles (the others stored nothing)
+  for (int k = 0, left = 0; k < ranks; ++k) {
+    left += all;
+    if (left >= ranks) {
+      live |= 1u << k;
+      left -= ranks;
+    }
+  }
   cluster_sync();
   const float* part = reinterpret_cast<const float*>(smem);
-  for (int v = rank * threads + threadIdx.x; v < rows * (D / 4); v += ranks * threads) {
-    const int r = v / (D / 4), c = v - r * (D / 4);
-    const uint32_t at = smem_u32(part + r * D + ((c ^ (r & 7)) << 2));
-    const uint32_t m_at = smem_u32(&st.m[r]), l_at = smem_u32(&st.l[r]);
-    float mk[kMaxRanks], lk[kMaxRanks];
-    float4 x[kMaxRanks];
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      if (k >= ranks) break;
-      mk[k] = ld_cluster_f1(mapa_addr(m_at, k));
-      lk[k] = ld_cluster_f1(mapa_addr(l_at, k));
-      x[k] = ld_cluster_f4(mapa_addr(at, k));
-    }
-    float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k)
-      if (k < ranks) mx = fmaxf(mx, mk[k]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < kMaxRanks; ++k) {
-      if (k >= ranks) break;
-      const float f = mk[k] == -INFINITY ? 0.f : exp2_fast(mk[k] - mx);
-      sum = fmaf(f, lk[k], sum);
-      if (mk[k] == -INFINITY) continue;  // it saw nothing, and may have stored nothing
-      o.x = fmaf(f, x[k].x, o.x);
-      o.y = fmaf(f, x[k].y, o.y);
-      o.z = fmaf(f, x[k].z, o.z);
-      o.w = fmaf(f, x[k].w, o.w);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int2 th = map(r);
-    uint2 w;
-    w.x = pack_bf16x2(o.x * inv, o.y * inv);
-    w.y = pack_bf16x2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D +
-                              c * 4) = w;
-  }
+  if (ranks == 2)
+    merge_rows<D, 2, 4>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
+  else if (ranks <= 4)
+    merge_rows<D, 4, 2>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
+  else
+    merge_rows<D, kMaxRanks, 1>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
   cluster_sync();  // nobody leaves while its result may be read
 }
 
@@ -574,7 +607,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     }
     st.m[r] = m * scale2;
     st.l[r] = l;
-    finish_rows<D>(a, st, smem, tile, map, rows, kvh, rank, ranks, 32 * S::kRowWarps);
+    finish_rows<D>(a, st, smem, tile, map, rows, kvh, rank, ranks, all, 32 * S::kRowWarps);
     return;
   }
   if constexpr (S::kRowRegs > 0) {
@@ -893,12 +926,29 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
   const long long tiles = std::min(n * ((group + S::kRows - 1) / S::kRows),
                                    n * group / S::kRows + std::min<long long>(a.batch.batch, n));
-  // CTAs per tile while the GPU has SMs to spare
-  const int ranks = (int)std::max(1LL, std::min<long long>(kMaxRanks, sms / (tiles * a.kv.kv_heads)));
-  a.cluster = ranks;
-  if (tiles * ranks * a.kv.kv_heads > 0x7fffffffll) return -1;
   static std::atomic<unsigned long long> done{0};
   if (!once_per_device(done, [&] { return allow_shared(k, S::kBytes); })) return -2;
+  // CTAs per tile, while all are resident at once: the time of a tile's longest run
+  // of key tiles, and for a cluster three key tiles and a bit for each CTA.
+  // Measured, one piece alone, with 1, 2, 4 and 8 CTAs: 64 tokens at 4096 (width 96)
+  // 43, 28, 19 and 16 us; 512 at 512 18, 17, 15 and 16; 256 at 256 11.5, 15, 13 and
+  // 14; a latent (width 128) 64 at 4096 69, 44, 28 and 21, 512 at 512 17, 20, 18 and,
+  // with more clusters than are resident, 34.
+  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
+  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + S::kRows / group + 2 * S::kKeys);
+  const long long key_tiles = (keys + S::kKeys - 1) / S::kKeys, clusters = tiles * a.kv.kv_heads;
+  static ClusterCapacity capacity;
+  int ranks = 1;
+  long long best = 10 * key_tiles;
+  for (int r = 2; r <= kMaxRanks && clusters * r <= sms; ++r) {
+    const long long cost = 10 * ((key_tiles + r - 1) / r) + 30 + r;
+    if (cost < best && clusters <= cluster_capacity(capacity, k, S::kThreads, S::kBytes, r)) {
+      ranks = r;
+      best = cost;
+    }
+  }
+  a.cluster = ranks;
+  if (tiles * ranks * a.kv.kv_heads > 0x7fffffffll) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ranks * a.kv.kv_heads));
   cfg.blockDim = dim3(S::kThreads);
