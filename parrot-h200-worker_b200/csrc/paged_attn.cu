@@ -643,34 +643,36 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
 }
 
 // CTAs per tile: as many as keep every warp two chunks or more of the longest
-// possible context, while the grid stays within `ctas`.
+// possible context, while nineteen twentieths of the clusters that fit at once are enough
+// (against three CTAs an SM, whatever fits: 24 sequences of 4096, 8-bit 13.5 us and
+// 19.0, 80 of a latent 29 and 42, 8 of four heads of 128 12.6 and 23.9).
 //
-// That is three CTAs per SM (one wave: measured at 64 sequences 26 us against 31
-// with four).  A few tiles of long contexts, whose warps would go through many
-// chunks one after the other, take the wide kind and clusters of up to 16, on
-// half of the SMs at most (clusters of one CTA an SM fill the GPU's partitions
-// badly: 8 tiles of 16 CTAs run in two turns).  One sequence of a latent of 32,768
-// keys: 49 us with eight CTAs of four warps, 36 with eight of eight, 22 with
-// sixteen; of 8192: 16, 14 and 11; of 4096, where the wide kind begins: 10.5 and
-// 10.1; of 2048 it would lose: 7.6 and 10.0.
-int decode_ranks(long long chunks, long long tiles, int warps, int most, long long ctas) {
-  int ranks = 1;
-  while (ranks < most && chunks >= 4LL * ranks * warps && tiles * ranks * 2 <= ctas) ranks *= 2;
-  return ranks;
-}
-
+// A few tiles of long contexts, whose warps would go through many chunks one
+// after the other, take the wide kind and clusters of up to 16, on half of the SMs
+// at most (clusters of one CTA an SM fill the GPU's partitions badly: 8 tiles of 16
+// CTAs run in two turns).  One sequence of a latent of 32,768 keys: 49 us with eight
+// CTAs of four warps, 36 with eight of eight, 22 with sixteen; of 8192: 16, 14 and
+// 11; of 4096, where the wide kind begins: 10.5 and 10.1; of 2048 it would lose: 7.6
+// and 10.0.
 template <int D, bool E4M3, bool SEP, bool WIDE>
-int launch_decode(PagedAttnArgs a, long long tiles, int ranks, cudaStream_t stream) {
+int launch_decode(PagedAttnArgs a, long long tiles, long long chunks, int most, int sms, cudaStream_t stream) {
   using S = DecodeShape<D, E4M3, SEP, WIDE>;
   auto k = paged_decode_kernel<D, E4M3, SEP, WIDE>;
-  a.cluster = ranks;
-  if (tiles * ranks > 0x7fffffffll) return -1;
   static std::atomic<unsigned long long> done{0};
   if (!once_per_device(done, [&] {
         return allow_shared(k, S::kBytes) &&
                (!WIDE || cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess);
       }))
     return -2;
+  static ClusterCapacity capacity;
+  const long long clusters = tiles * a.kv.kv_heads;
+  int ranks = 1;
+  for (int r = 2; r <= most && chunks >= 2LL * r * S::kWarps; ++r)
+    if (WIDE ? clusters * r * 2 <= sms
+             : clusters * 20 <= 19LL * cluster_capacity(capacity, k, 32 * S::kWarps, S::kBytes, r))
+      ranks = r;
+  a.cluster = ranks;
+  if (tiles * ranks > 0x7fffffffll) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * ranks), a.kv.kv_heads);
   cfg.blockDim = dim3(32 * S::kWarps);
@@ -694,10 +696,9 @@ int launch_decode_of(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
   long long keys = (long long)a.batch.table_width << a.kv.page_shift;
   if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
   const long long chunks = (keys + kDecKeys - 1) / kDecKeys, all = tiles * a.kv.kv_heads;
-  constexpr int kWide = DecodeShape<D, E4M3, SEP, true>::kWarps;
   if (all * 16 <= sms && chunks >= 128)
-    return launch_decode<D, E4M3, SEP, true>(a, tiles, decode_ranks(chunks, all, kWide, 16, sms / 2), stream);
-  return launch_decode<D, E4M3, SEP, false>(a, tiles, decode_ranks(chunks, all, 4, 8, 3LL * sms), stream);
+    return launch_decode<D, E4M3, SEP, true>(a, tiles, chunks, 16, sms, stream);
+  return launch_decode<D, E4M3, SEP, false>(a, tiles, chunks, 8, sms, stream);
 }
 
 template <int D>
