@@ -79,9 +79,9 @@ struct PrefillShape {
   static constexpr int kMmaRegs = E4M3 ? (kGroups == 2 ? 48 : 40) : 88;
   static_assert(kThreads % 128 == 0, "whole warpgroups");
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-  static_assert(kRowRegs == 0 || kRowRegs * kRowWarps + (E4M3 ? kLoadRegs * kLoadWarps : 0) +
-                                         kMmaRegs * 4 <= kLaunchRegs * (kThreads / 32),
-                "register split");
+  static constexpr int kSplitRegs =
+      kRowRegs == 0 ? 0 : kRowRegs * kRowWarps + (E4M3 ? kLoadRegs * kLoadWarps : 0) + kMmaRegs * 4;
+  static_assert(kSplitRegs <= kLaunchRegs * (kThreads / 32), "register split");
   // TMEM columns: S (and P over it) of group g at g * kKeys, O behind
   static constexpr uint32_t kTmemO = kGroups * kKeys;
   static_assert(kGroups * (kKeys + D) <= 512, "S and O of all groups");
@@ -927,7 +927,13 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   const long long tiles = std::min(n * ((group + S::kRows - 1) / S::kRows),
                                    n * group / S::kRows + std::min<long long>(a.batch.batch, n));
   static std::atomic<unsigned long long> done{0};
-  if (!once_per_device(done, [&] { return allow_shared(k, S::kBytes); })) return -2;
+  if (!once_per_device(done, [&] {
+        // what the compiler gave the launch covers the split, or its waits would not end
+        cudaFuncAttributes got;
+        return cudaFuncGetAttributes(&got, k) == cudaSuccess &&
+               got.numRegs / 8 * 8 * (S::kThreads / 32) >= S::kSplitRegs && allow_shared(k, S::kBytes);
+      }))
+    return -2;
   // CTAs per tile, while all are resident at once: the time of a tile's longest run
   // of key tiles, and for a cluster three key tiles and a bit for each CTA.
   // Measured, one piece alone, with 1, 2, 4 and 8 CTAs: 64 tokens at 4096 (width 96)
