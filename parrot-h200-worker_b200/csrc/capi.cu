@@ -1845,8 +1845,9 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
   a.sinks = a.window > 0 ? sinks : 0;
   a.scale = scale;
   a.status = status;
-  if (parrot::paged_few_queries(a)) {
-    if (parrot::launch_paged_decode(a, sm_count(), static_cast<cudaStream_t>(stream)))
+  const int sms = sm_count();
+  if (parrot::paged_few_queries(a, sms)) {
+    if (parrot::launch_paged_decode(a, sms, static_cast<cudaStream_t>(stream)))
       return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
     return check_launch("paged_decode_kernel");
   }
@@ -1858,7 +1859,7 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
          !pool_map(&v_map, kv->value, pool_rows, kv->head_dim, kv->page_size)))
       return fail(PARROT_ECUDA, "paged_attention: tensor map encode failed%s");
   }
-  if (parrot::launch_paged_prefill(a, k_map, v_map, sm_count(), static_cast<cudaStream_t>(stream)))
+  if (parrot::launch_paged_prefill(a, k_map, v_map, sms, static_cast<cudaStream_t>(stream)))
     return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
   return check_launch("paged_prefill_kernel");
 }

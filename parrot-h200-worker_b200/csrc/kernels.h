@@ -382,7 +382,7 @@ struct PagedAttnArgs {
 };
 int launch_paged_append(const PagedAppendArgs& args, cudaStream_t stream);
 int launch_paged_gather(const PagedGatherArgs& args, cudaStream_t stream);
-bool paged_few_queries(const PagedAttnArgs& args);
+bool paged_few_queries(const PagedAttnArgs& args, int sms);
 int launch_paged_decode(const PagedAttnArgs& args, int sms, cudaStream_t stream);
 // k_map / v_map: the bf16 pools as [rows, head_dim], boxes of 32 columns x
 // paged_prefill_box_rows rows, 64-byte swizzle (not read for e4m3 pools)

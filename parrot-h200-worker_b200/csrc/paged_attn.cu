@@ -8,8 +8,6 @@
 // The query heads of one key head and a run of tokens share their keys: a
 // tile is 16 consecutive (token, head) rows of one sequence, token major, so
 // each key is read once for all of them.
-#include <algorithm>
-
 #include "paged_attn.cuh"
 
 namespace parrot {
@@ -690,12 +688,8 @@ int launch_decode(PagedAttnArgs a, long long tiles, long long chunks, int most, 
 
 template <int D, bool E4M3, bool SEP>
 int launch_decode_of(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
-  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
-  const long long tiles = std::min(n * ((group + kDecRows - 1) / kDecRows),
-                                   n * group / kDecRows + std::min<long long>(a.batch.batch, n));
-  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
-  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + 2 * kDecKeys);
-  const long long chunks = (keys + kDecKeys - 1) / kDecKeys, all = tiles * a.kv.kv_heads;
+  const long long tiles = most_tiles(a, kDecRows), all = tiles * a.kv.kv_heads;
+  const long long chunks = (most_keys(a, kDecRows, kDecKeys) + kDecKeys - 1) / kDecKeys;
   if (all * 16 <= sms && chunks >= 128)
     return launch_decode<D, E4M3, SEP, true>(a, tiles, chunks, 16, sms, stream);
   return launch_decode<D, E4M3, SEP, false>(a, tiles, chunks, 8, sms, stream);
@@ -712,16 +706,20 @@ int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
 }  // namespace
 
 // Few new tokens per sequence: the kernel above (its tile reads the keys for 16
-// rows); beyond, paged_prefill.cu's (for 256 or 384).  Measured with 8 heads on 2,
-// width 96, a window of 2048: 8 sequences of 4 tokens 16 us here and 24 there, of 8
-// 17 and 25, of 16 20 and 25, of 24 30 and 26; 32 sequences of 2 tokens 20 here, of
-// 4 30 and 26; one of 8 14 and 12.  Single tokens beside pieces go with the pieces
-// (8 beside one of 256: 21 us, and 29 in two launches; 64 beside 512: 58, and 64
-// in two, where the second finds most of its CTAs without work).
-bool paged_few_queries(const PagedAttnArgs& a) {
-  const long long n = a.batch.tokens;
-  return n <= 4LL * a.batch.batch ||
-         (a.batch.batch >= 4 && n <= 16LL * a.batch.batch && n * a.heads <= 64LL * kDecRows);
+// rows); beyond, paged_prefill.cu's (for 256 or 384).  Measured (8 heads on 2, width
+// 96, a window of 2048, contexts of 4096) in bf16: 64 single tokens 26 us here and 38
+// there, 32 sequences of 2 tokens 21 and 25, 8 of 2 15 and 13, 8 of 4 16 and 14, 32 of
+// 4 30 and 26.  An 8-bit cache, whose tiles paged_prefill.cu's warps have to widen:
+// 32 of 4 25 and 33, 8 of 8 15 and 17, 32 of 8 39 and 34.  Few rows over long contexts
+// get more warps here: one piece of 8 over 16,384 keys 18 and 39, 4 of 4 of a latent
+// 32 and 36.  Single tokens beside pieces go with the pieces (8 beside one of 256: 21
+// us, and 29 in two launches; 64 beside 512: 58, and 64 in two).
+bool paged_few_queries(const PagedAttnArgs& a, int sms) {
+  const long long n = a.batch.tokens, batch = a.batch.batch, rows = n * a.heads;
+  if (n <= 2 * batch) return true;
+  if (a.kv.key_scale != nullptr && (n <= 4 * batch || (n <= 8 * batch && rows <= 64 * kDecRows)))
+    return true;
+  return n <= 8 * batch && rows <= sms && most_keys(a, kDecRows, kDecKeys) >= 128 * kDecKeys;
 }
 
 int launch_paged_decode(const PagedAttnArgs& a, int sms, cudaStream_t stream) {

@@ -3,6 +3,9 @@
 
 #include <atomic>
 
+#include <algorithm>
+#include <numeric>
+
 #include "paged.cuh"
 #include "tc.cuh"
 
@@ -36,6 +39,20 @@ inline int cluster_capacity(ClusterCapacity& cache, K kernel, int threads, int s
   }
   if (dev < 16) cache.plus_one[dev][ranks].store(n + 1, std::memory_order_relaxed);
   return n;
+}
+
+// No more tiles of `rows_per` rows than this: a sequence's rows are a multiple of
+// d = gcd(group, rows_per), so its last tile wants rows_per - d at most.
+inline long long most_tiles(const PagedAttnArgs& a, int rows_per) {
+  const long long n = a.batch.tokens, group = a.heads / a.kv.kv_heads;
+  const long long seqs = std::min<long long>(a.batch.batch, n), d = std::gcd(group, (long long)rows_per);
+  return (n * group + seqs * (rows_per - d)) / rows_per;
+}
+// No more keys in sight of a tile of `rows` rows than this.
+inline long long most_keys(const PagedAttnArgs& a, int rows, int step) {
+  const long long keys = (long long)a.batch.table_width << a.kv.page_shift;
+  const long long tokens = rows / (a.heads / a.kv.kv_heads) + 1;
+  return a.window > 0 ? std::min(keys, (long long)a.window + a.sinks + tokens + 2 * step) : keys;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

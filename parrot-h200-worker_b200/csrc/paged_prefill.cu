@@ -39,8 +39,6 @@
 //
 // With few tiles a cluster of CTAs shares one, each taking a run of its key
 // tiles, and merges the results over distributed shared memory.
-#include <algorithm>
-
 #include "paged_attn.cuh"
 
 namespace parrot {
@@ -923,9 +921,7 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
                    cudaStream_t stream) {
   using S = PrefillShape<D, E4M3, SEP>;
   auto k = paged_prefill_kernel<D, E4M3, SEP>;
-  const long long group = a.heads / a.kv.kv_heads, n = a.batch.tokens;
-  const long long tiles = std::min(n * ((group + S::kRows - 1) / S::kRows),
-                                   n * group / S::kRows + std::min<long long>(a.batch.batch, n));
+  const long long tiles = most_tiles(a, S::kRows);
   static std::atomic<unsigned long long> done{0};
   if (!once_per_device(done, [&] {
         // what the compiler gave the launch covers the split, or its waits would not end
@@ -940,9 +936,8 @@ int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap&
   // 43, 28, 19 and 16 us; 512 at 512 18, 17, 15 and 16; 256 at 256 11.5, 15, 13 and
   // 14; a latent (width 128) 64 at 4096 69, 44, 28 and 21, 512 at 512 17, 20, 18 and,
   // with more clusters than are resident, 34.
-  long long keys = (long long)a.batch.table_width << a.kv.page_shift;
-  if (a.window > 0) keys = std::min(keys, (long long)a.window + a.sinks + S::kRows / group + 2 * S::kKeys);
-  const long long key_tiles = (keys + S::kKeys - 1) / S::kKeys, clusters = tiles * a.kv.kv_heads;
+  const long long key_tiles = (most_keys(a, S::kRows, S::kKeys) + S::kKeys - 1) / S::kKeys;
+  const long long clusters = tiles * a.kv.kv_heads;
   static ClusterCapacity capacity;
   int ranks = 1;
   long long best = 10 * key_tiles;
