@@ -651,7 +651,8 @@ typedef struct parrot_paged_kv {
   void* key_scale;    /* e4m3: [pages, n_kv_heads, page_size] bytes; a row's values are
                          its numbers times 2^(byte - 127).  bf16: NULL */
   void* value_scale;
-  int pages, n_kv_heads, page_size, head_dim;  /* page_size 16, 32, 64, 128 or 256;
+  int pages, n_kv_heads, page_size, head_dim;  /* pages * n_kv_heads * page_size in 1 .. 2^31 - 1;
+                                                  page_size 16, 32, 64, 128 or 256;
                                                   head_dim 32, 64, 96 or 128 */
   int e4m3;           /* 0: bf16 pools, 1: e4m3 pools with scales */
 } parrot_paged_kv;
