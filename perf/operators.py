@@ -12,7 +12,6 @@ sequence ``b`` is row ``p % page`` of page ``page_table[b, p // page]`` in pools
 ``[pages, kv heads, page, head width]``.  An 8-bit pool holds e4m3 numbers and, for each row of
 each head, one byte ``s``: the row's values are ``number * 2 ** (s - 127)``.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -31,7 +30,6 @@ _LOCAL = {"heads": 8, "kv_heads": 2, "width": 96}      # Parrot XL's sliding-win
 _LATENT = {"heads": 8, "kv_heads": 1, "width": 128}    # its absorbed latent layers: keys = values
 
 
-@functools.cache  # a user's program imports once
 def _bridge():
     root = str(Path(__file__).resolve().parent.parent / "parrot-h200-worker_b200")
     if root not in sys.path:
