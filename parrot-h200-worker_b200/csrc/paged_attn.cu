@@ -87,8 +87,11 @@ __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) !
 // power of two per row that puts its largest magnitude at 2^8 (what f16 loses is
 // below 2^-32 of that); the keys' scales multiply the scores.  The values'
 // scales multiply the probabilities, w = p 2^e, and these go to f16 relative to
-// a power of two W per row above all its w so far, at 2^14 W^-1: 11 bits down to
-// 2^-28 W, nothing lost above 2^-39 W.
+// a power of two W per row, at 2^14 W^-1: 11 bits down to 2^-28 W, nothing lost
+// above 2^-39 W.  W is the power of two next above the largest w so far, each w
+// taken at the present maximum: it falls when the maximum moves and what it stood
+// for no longer counts (a W that only grew made keys of small scales vanish behind
+// those of large ones that softmax had since put out of account).
 //
 // Measured (8 heads on 2, width 96, a window of 2048, contexts of 4096): one
 // sequence 7.5 us, most of it the launch, the lists and the merge; 64 sequences
@@ -262,6 +265,7 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
     __syncwarp();
   }
   float top_w[2] = {0.f, 0.f};        // e4m3: W of each row, 0 before its first
+  float most_w[2] = {0.f, 0.f};       // the largest of this thread's weights so far, at the present maximum
   const bool two = rows > 8;          // whether rows g + 8 exist
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -373,25 +377,31 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
       l[i] = fmaf(l[i], corr[i], sum);  // this thread's columns; the quad is summed at the end
     }
     if constexpr (E4M3) {
-      float most[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        most_w[i] *= corr[i];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             s[nt][2 * i + e] *= v_scale[nt][e];
-            most[i] = fmaxf(most[i], s[nt][2 * i + e]);
+            most_w[i] = fmaxf(most_w[i], s[nt][2 * i + e]);
           }
-      if (__any_sync(0xffffffffu, most[0] >= top_w[0] || (two && most[1] >= top_w[1]))) {
+      }
+      // W is set anew where a weight reaches it, and where the maximum moves (O is
+      // rescaled then in any case)
+      const bool moved0 = corr[0] != 1.f || most_w[0] >= top_w[0];
+      const bool moved1 = two && (corr[1] != 1.f || most_w[1] >= top_w[1]);
+      if (__any_sync(0xffffffffu, moved0 || moved1)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
-          most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
-          if (most[i] > 0.f && most[i] >= top_w[i]) {
+          float most = fmaxf(most_w[i], __shfl_xor_sync(0xffffffffu, most_w[i], 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          if (most > 0.f && (corr[i] != 1.f || most >= top_w[i])) {
             // the power of two above it (at least 2^-100: its reciprocal is finite)
-            const float w = fmaxf(__uint_as_float((__float_as_uint(most[i]) & 0x7f800000u) + 0x00800000u), pow2(-100));
-            corr[i] *= top_w[i] / w;
+            const float w = fmaxf(__uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u), pow2(-100));
+            // most >= corr W / 2, so the product is below 2 (W / w alone may be past fp32)
+            corr[i] = corr[i] * top_w[i] * __uint_as_float((254u << 23) - __float_as_uint(w));
             top_w[i] = w;
           }
         }
