@@ -705,7 +705,11 @@ int parrot_paged_gather_bf16(const parrot_paged_kv* kv, const parrot_paged_batch
  * n_heads, head_dim] bf16.  A token that sees no key gets zeros.  What no
  * token of the batch sees is not used: pages wholly outside the window and
  * the sinks may be given away, and numbers in masked places may be anything,
- * NaN and infinities included. */
+ * NaN and infinities included.  Where a token sees one, its result is what
+ * the formula gives: an infinite value that infinity in its column (NaN
+ * beside its opposite, or where its weight is zero: scores more than 87 below
+ * the largest may count as that), a score of -infinity no weight, one of
+ * +infinity or NaN a row of NaN, and so do scores of -infinity alone. */
 int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
                                 const void* q, long long q_row_stride, void* out, int n_heads,
                                 int window, int sinks, float scale, int* status, void* stream);

@@ -589,8 +589,8 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
   __syncthreads();
   float* part = reinterpret_cast<float*>(dec_smem + S::kWarp * W);
   auto write = [&](int r, int col, float4 v, float sum) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key seen: zeros
     const int2 th = map(r);
+    const float inv = row_inverse(sum, pos0 + th.x);
     uint2 w;
     w.x = tc::pack_bf16x2(v.x * inv, v.y * inv);
     w.y = tc::pack_bf16x2(v.z * inv, v.w * inv);

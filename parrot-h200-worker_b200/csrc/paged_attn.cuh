@@ -63,6 +63,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// 1 / sum of the weights of a row at position `pos`.  A row before the first
+// position sees no key: zeros.  One that sees keys of weight 0 alone (scores of
+// -infinity) has 0 / 0: NaN.
+__device__ __forceinline__ float row_inverse(float sum, int pos) {
+  return sum != 0.f ? 1.f / sum : pos < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+}
+
 // A tile: `rows_per` consecutive (token, head) rows of one sequence.
 struct Tile {
   int b;           // sequence, -1: no such tile

@@ -34,8 +34,9 @@
 // Tiles at an edge of what the rows see (the diagonal, the window's start, the
 // sinks) pass through two of the three first: in a product 0 * NaN would carry a
 // number from a masked place to every row, so rows of V that nobody sees become
-// zeros, and numbers that are not finite are taken out and noted; a row that
-// does see one gets NaN in that column.
+// zeros, and numbers that are not finite are taken out and noted by sign; a row
+// that does see one gets that infinity, or NaN, in that column.  Of a latent they
+// are taken out of the key as well, and a row that sees it puts its score right.
 //
 // With few tiles a cluster of CTAs shares one, each taking a run of its key
 // tiles, and merges the results over distributed shared memory.
@@ -93,7 +94,10 @@ struct PrefillShape {
   static constexpr int kQGroup = kGroup * D * 2, kQSlab = kGroup * 64;
   static constexpr int kQ = kGroups * kQGroup;
   static constexpr int kRing = kStages * kTile;
-  static constexpr int kBad = kStages * kKeys * 16;  // noted columns of each row of a V tile
+  // noted columns of each row of a V tile: those that are +inf or NaN, those that are
+  // -inf or NaN (e4m3 has only NaN)
+  static constexpr int kMarks = E4M3 ? 1 : 2;
+  static constexpr int kBad = kStages * kKeys * 16 * kMarks;
   static constexpr int kPart = kRows * D * 4;        // a CTA's result, over Q and the rings
   static constexpr int kBytes0 = kQ + kSides * kRing + kBad + 1024;
   static_assert(kPart <= kQ + kSides * kRing, "the result fits the tiles");
@@ -101,7 +105,9 @@ struct PrefillShape {
   static constexpr int kBytes = kBytes0 < 118784 ? 118784 : kBytes0;
 };
 
+template <int D, bool E4M3>
 struct PrefillState {
+  static constexpr int kRows = kGroup * tile_groups(D);
   uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6], raw[6];
   uint64_t s_full[kMaxGroups], p_ready[kMaxGroups], o_done[kMaxGroups], drain;
   uint32_t tmem;
@@ -110,10 +116,10 @@ struct PrefillState {
   uint64_t* armed[2][6];       // the barrier of each stage's last copy, and its phase
   uint32_t armed_parity[2][6];
   // e4m3, of three units of each half of the loading warps
-  int row[2][3][128];          // pool row of each key, -1: zeros
-  int scale[2][3][128];        // its scale byte
-  uint4 poison[kGroup * kMaxGroups];
-  float m[kGroup * kMaxGroups], l[kGroup * kMaxGroups];  // merge
+  int row[2][3][E4M3 ? 128 : 1];    // pool row of each key, -1: zeros
+  int scale[2][3][E4M3 ? 128 : 1];  // its scale byte
+  uint4 poison[E4M3 ? 1 : 2][kRows];  // columns of each row, as they are noted
+  float m[kRows], l[kRows];    // merge
 };
 
 // Shared-memory descriptors as two words: tiles with a 64-byte swizzle, 512 B
@@ -244,16 +250,34 @@ __device__ __forceinline__ uint32_t not_finite8(const uint4& v) {
   }
   return bits;
 }
+// of those: the ones that are +inf or NaN, and the ones that are -inf or NaN
+__device__ __forceinline__ uint2 marks8(const uint4& v, uint32_t bits) {
+  uint2 marks = make_uint2(0, 0);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = w[i >> 1] >> (16 * (i & 1));
+    const bool nan = (h & 0x7fu) != 0, minus = (h & 0x8000u) != 0;
+    if (nan || !minus) marks.x |= bits & 1u << i;
+    if (nan || minus) marks.y |= bits & 1u << i;
+  }
+  return marks;
+}
+__device__ __forceinline__ void or_into(uint4& a, const uint4& b) {
+  a.x |= b.x;
+  a.y |= b.y;
+  a.z |= b.z;
+  a.w |= b.w;
+}
 __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pair i
   return (bits >> (2 * i) & 1 ? 0u : 0xffffu) | (bits >> (2 * i) & 2 ? 0u : 0xffff0000u);
 }
 
 // A tile's results of up to K CTAs joined: U of the tile's 16-byte vectors at a
 // time, all of their remote loads on their way together.
-template <int D, int K, int U>
-__device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, PrefillState& st,
-                                           const float* part, const Tile& tile, const RowMap& map,
-                                           int rows, int kvh, int rank, int ranks, uint32_t live,
+template <int D, int K, int U, typename St>
+__device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, St& st, const float* part,
+                                           const Tile& tile, const RowMap& map, int pos0, int rows, int kvh, int rank, int ranks, uint32_t live,
                                            int threads) {
   const int total = rows * (D / 4), stride = ranks * threads;
   for (int v0 = rank * threads + threadIdx.x; v0 < total; v0 += U * stride) {
@@ -293,8 +317,8 @@ __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, PrefillState&
         o.z = fmaf(f, x[u][k].z, o.z);
         o.w = fmaf(f, x[u][k].w, o.w);
       }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int2 th = map(r);
+      const float inv = row_inverse(sum, pos0 + th.x);
       uint2 w;
       w.x = pack_bf16x2(o.x * inv, o.y * inv);
       w.y = pack_bf16x2(o.z * inv, o.w * inv);
@@ -307,10 +331,10 @@ __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, PrefillState&
 // The end of the rows' warps: with several CTAs to a tile, each merges its share
 // of the tile's vectors.  (Working each row's weights out first and keeping eight
 // vectors on their way whatever the cluster: 3 us slower with eight CTAs.)
-template <int D>
-__device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState& st,
+template <int D, typename St>
+__device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, St& st,
                                             unsigned char* smem, const Tile& tile,
-                                            const RowMap& map, int rows, int kvh, int rank, int ranks,
+                                            const RowMap& map, int pos0, int rows, int kvh, int rank, int ranks,
                                             int all, int threads) {
   tc_fence_before();
   __syncthreads();
@@ -326,11 +350,11 @@ __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, PrefillState
   cluster_sync();
   const float* part = reinterpret_cast<const float*>(smem);
   if (ranks == 2)
-    merge_rows<D, 2, 4>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, 2, 4>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   else if (ranks <= 4)
-    merge_rows<D, 4, 2>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, 4, 2>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   else
-    merge_rows<D, kMaxRanks, 1>(a, st, part, tile, map, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, kMaxRanks, 1>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   cluster_sync();  // nobody leaves while its result may be read
 }
 
@@ -343,7 +367,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
   using S = PrefillShape<D, E4M3, SEP>;
   constexpr int NS = S::kStages, T = S::kKeys, NG = S::kGroups, R = S::kRows;
   extern __shared__ unsigned char pf_raw[];
-  __shared__ PrefillState st;
+  __shared__ PrefillState<D, E4M3> st;
   // tiles start on 1024 bytes, the swizzle's period and more
   unsigned char* smem = pf_raw + (1024 - (smem_u32(pf_raw) & 1023)) % 1024;
   const uint32_t q_u = smem_u32(smem), k_u = q_u + S::kQ, v_u = SEP ? k_u + S::kRing : k_u;
@@ -475,6 +499,40 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) s[c][k] = seen >> k & 1 ? s[c][k] : 0xff800000u;
         }
+        if constexpr (!SEP && !E4M3) {
+          // A latent's numbers that are not finite were taken out of the key too: what
+          // they would have added to its score, an infinity by the query's sign or NaN.
+          const int stage = i % NS;
+          if (!(ok = wait_asleep(&st.k_full[stage], (i / NS) & 1, abort_flag, a.status, 61))) break;
+          if (*reinterpret_cast<volatile int*>(&st.bad[stage])) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              uint32_t up = 0, down = 0;  // a bit per key
+#pragma unroll 1
+              for (int k = 0; k < 32; ++k) {
+                const int key = base + 32 * c + k;
+                if (!(key <= pos && (a.window == 0 || pos - key < a.window || key < a.sinks))) continue;
+                const uint32_t* marks = reinterpret_cast<const uint32_t*>(bad_cols + (stage * T + 32 * c + k) * 2);
+#pragma unroll 1
+                for (int col = 0; col < D; ++col) {
+                  const bool plus = marks[col >> 5] >> (col & 31) & 1, minus = marks[4 + (col >> 5)] >> (col & 31) & 1;
+                  if (!plus && !minus) continue;
+                  const uint32_t q = *reinterpret_cast<const unsigned short*>(
+                      smem + g * S::kQGroup + sw64_at<kGroup>(r & (kGroup - 1), col >> 3) + (col & 7) * 2);
+                  const bool nan = (plus && minus) || (q & 0x7fffu) == 0 || (q & 0x7fffu) > 0x7f80u;
+                  const bool turned = (q & 0x8000u) != 0;
+                  if (nan || plus != turned) up |= 1u << k;
+                  if (nan || plus == turned) down |= 1u << k;
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                if (up >> k & 1) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) + INFINITY);
+                if (down >> k & 1) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) - INFINITY);
+              }
+            }
+          }
+        }
       }
       float mx[NC];
 #pragma unroll
@@ -529,18 +587,22 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
         uint64_t* full = SEP ? &st.v_full[stage] : &st.k_full[stage];
         if (!(ok = wait_asleep(full, (i / NS) & 1, abort_flag, a.status, 61))) break;
         if (*reinterpret_cast<volatile int*>(&st.bad[stage])) {
-          uint4 cols = poison ? st.poison[r] : make_uint4(0, 0, 0, 0);
+          uint4 cols[S::kMarks];
+#pragma unroll
+          for (int w = 0; w < S::kMarks; ++w) cols[w] = poison ? st.poison[w][r] : make_uint4(0, 0, 0, 0);
           for (int k = 0; k < T; ++k) {
             const int key = base + k;
             if (key <= pos && (a.window == 0 || pos - key < a.window || key < a.sinks)) {
-              const uint4 w = bad_cols[stage * T + k];
-              cols.x |= w.x;
-              cols.y |= w.y;
-              cols.z |= w.z;
-              cols.w |= w.w;
+#pragma unroll
+              for (int w = 0; w < S::kMarks; ++w) {
+                or_into(cols[w], bad_cols[(stage * T + k) * S::kMarks + w]);
+                // a latent's infinity has the weight 0 (score -inf) or NaN (score +inf)
+                if (!SEP && !E4M3) or_into(cols[w], bad_cols[(stage * T + k) * S::kMarks + 1 - w]);
+              }
             }
           }
-          st.poison[r] = cols;
+#pragma unroll
+          for (int w = 0; w < S::kMarks; ++w) st.poison[w][r] = cols[w];
           poison = true;
         }
       }
@@ -553,7 +615,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     for (int h = 0; h < groups && n > 0; ++h)
       if (h == g || ranks > 1) ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62) && ok;
     tc_fence_after();
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+    const float inv = row_inverse(l, pos);
     float* part = reinterpret_cast<float*>(smem);
     unsigned char* own = smem + g * S::kQGroup;  // the warp's rows, bf16, where Q was
     // loops, not straight lines: this runs once, and fetching its instructions
@@ -568,10 +630,13 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
         for (int k = 0; k < 32; ++k) o[k] = 0;
       }
       if (poison) {
-        const uint32_t cols = reinterpret_cast<const uint32_t*>(&st.poison[r])[c];
+        const uint32_t plus = reinterpret_cast<const uint32_t*>(&st.poison[0][r])[c];
+        const uint32_t minus = reinterpret_cast<const uint32_t*>(&st.poison[S::kMarks - 1][r])[c];
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (cols >> k & 1) o[k] = 0x7fc00000u;
+        for (int k = 0; k < 32; ++k) {
+          if (plus >> k & 1) o[k] = __float_as_uint(__uint_as_float(o[k]) + INFINITY);
+          if (minus >> k & 1) o[k] = __float_as_uint(__uint_as_float(o[k]) - INFINITY);
+        }
       }
       if (ranks == 1) {
 #pragma unroll
@@ -607,7 +672,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     }
     st.m[r] = m * scale2;
     st.l[r] = l;
-    finish_rows<D>(a, st, smem, tile, map, rows, kvh, rank, ranks, all, 32 * S::kRowWarps);
+    finish_rows<D>(a, st, smem, tile, map, pos0, rows, kvh, rank, ranks, all, 32 * S::kRowWarps);
     return;
   }
   if constexpr (S::kRowRegs > 0) {
@@ -692,7 +757,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
           bool any = false;
           for (int k = ct; k < T; k += 64) {
             const bool seen = some_row_sees(base + k);
-            uint32_t cols[4] = {0, 0, 0, 0};
+            uint32_t plus[4] = {0, 0, 0, 0}, minus[4] = {0, 0, 0, 0};
             bool row_bad = false;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
@@ -704,7 +769,9 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
               uint4 v = *p;
               const uint32_t bits = not_finite8(v);
               if (bits) {
-                cols[c >> 2] |= bits << (8 * (c & 3));
+                const uint2 marks = marks8(v, bits);
+                plus[c >> 2] |= marks.x << (8 * (c & 3));
+                minus[c >> 2] |= marks.y << (8 * (c & 3));
                 row_bad = true;
                 v.x &= keep_mask(bits, 0);
                 v.y &= keep_mask(bits, 1);
@@ -713,9 +780,8 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
                 *p = v;
               }
             }
-            // a latent's key is its value: a row that sees it has no score left
-            if (!SEP && row_bad) cols[0] = cols[1] = cols[2] = cols[3] = 0xffffffffu;
-            bad_cols[s * T + k] = make_uint4(cols[0], cols[1], cols[2], cols[3]);
+            bad_cols[(s * T + k) * 2] = make_uint4(plus[0], plus[1], plus[2], plus[3]);
+            bad_cols[(s * T + k) * 2 + 1] = make_uint4(minus[0], minus[1], minus[2], minus[3]);
             any |= row_bad;
           }
           fence_async_shared();
@@ -824,7 +890,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
                 uint32_t* cols = reinterpret_cast<uint32_t*>(bad_cols + s * T + k);
                 if (SEP) {
                   atomicOr(cols + (c8 >> 2), bits << (8 * (c8 & 3)));
-                } else {  // a latent's key is its value: a row that sees it has no score left
+                } else {  // a latent's key is its value: with a NaN in it the score is NaN
                   for (int q = 0; q < 4; ++q) atomicOr(cols + q, 0xffffffffu);
                 }
                 *reinterpret_cast<volatile int*>(&st.bad[s]) = 1;

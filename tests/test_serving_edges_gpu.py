@@ -145,3 +145,74 @@ def test_large_scores_keep_the_running_maximum_in_8_bits(queries):
     cache.key, cache.key_scale = quantise(x * ramp)
     q = (_queries(sum(queries), 4, 96, 1).float() * 4).to(torch.bfloat16)
     _assert_formula(_call(cache, queries, q), cache, queries, q)
+
+
+# ------------------------------------------------------------------------ numbers that are not finite
+SIGNS = [(math.inf,), (-math.inf,), (math.nan,), (math.inf, -math.inf), (math.inf, math.inf)]
+
+
+@pytest.mark.parametrize("bad", SIGNS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 96), (8, 2, 128), (3, 1, 32)])
+@pytest.mark.parametrize("queries,context,window,sinks,at", [
+    ([1], 300, 0, 0, 100), ([4], 60, 0, 0, 57), ([4], 400, 0, 0, 30), ([3], 5000, 0, 0, 4000),
+    ([130], 140, 0, 0, 100),        # on the diagonal
+    ([130], 1000, 0, 0, 200),       # where every row sees it
+    ([130], 400, 64, 0, 290),       # at the window's start
+    ([300], 700, 100, 5, 3),        # among the first tokens
+    ([500], 500, 0, 0, 0),
+])
+def test_an_infinite_value_is_what_the_formula_says(queries, context, window, sinks, at, heads, kv_heads, dim, bad):
+    """Wherever it lies in a tile: an infinity for the rows that see it, NaN beside its opposite."""
+    cache = Paged([context], kv_heads=kv_heads, dim=dim, page=16, seed=4)
+    for i, x in enumerate(bad):
+        cache.value[int(cache.table[0, (at + i) // 16]), 0, (at + i) % 16, 5] = x
+    q = _queries(sum(queries), heads, dim, 0)
+    out = _call(cache, queries, q, window, sinks)
+    _assert_formula(out, cache, queries, q, window, sinks)
+
+
+@pytest.mark.parametrize("column", [5, 100])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("queries,context,at", [
+    ([1], 300, 100), ([4], 60, 57), ([3], 5000, 4000), ([130], 140, 100), ([130], 1000, 200), ([500], 500, 0)])
+def test_an_infinite_latent_row_is_what_the_formula_says(queries, context, at, bad, column):
+    """Its score is an infinity of either sign, as the query has it: a row that turns away from it
+    loses its column alone (zero times infinity), one that turns to it, or a NaN, everything."""
+    cache = Paged([context], kv_heads=1, dim=128, page=16, latent=True, seed=4)
+    cache.key[int(cache.table[0, at // 16]), 0, at % 16, column] = bad
+    q = _queries(sum(queries), 8, 128, 0)
+    q[:, 2, column] = 0.0          # zero times infinity
+    out = _call(cache, queries, q)
+    _assert_formula(out, cache, queries, q)
+
+
+def test_two_infinite_numbers_in_a_latent_row():
+    cache = Paged([150], kv_heads=1, dim=128, page=16, latent=True, seed=4)
+    row = cache.key[int(cache.table[0, 100 // 16]), 0, 100 % 16]
+    row[5], row[70] = math.inf, -math.inf
+    for queries in ([130], [3]):
+        q = _queries(sum(queries), 8, 128, 0)
+        q[:, 0, 5], q[:, 0, 70] = 1.0, 1.0
+        q[:, 1, 5], q[:, 1, 70] = -1.0, 1.0
+        q[:, 2, 5], q[:, 2, 70] = 1.0, -1.0
+        q[:, 3, 9] = math.nan
+        _assert_formula(_call(cache, queries, q), cache, queries, q)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("queries,context,at", [
+    ([1], 300, 100), ([4], 60, 57), ([3], 5000, 4000), ([130], 140, 100), ([130], 1000, 200), ([500], 500, 0)])
+def test_an_infinite_key_is_what_the_formula_says(queries, context, at, bad, e4m3):
+    """A score of -infinity has no weight, one of +infinity or NaN leaves a row of NaN; a token whose
+    only key has no weight has 0 / 0."""
+    if e4m3 and not math.isnan(bad):
+        pytest.skip("8-bit numbers have no infinity")
+    cache = Paged([context], kv_heads=1, dim=96, page=16, e4m3=e4m3, seed=4)
+    page = int(cache.table[0, at // 16])
+    if e4m3:
+        cache.key.view(torch.uint8)[page, 0, at % 16, 7] = 0x7f
+    else:
+        cache.key[page, 0, at % 16, 7] = bad
+    q = _queries(sum(queries), 4, 96, 0)
+    _assert_formula(_call(cache, queries, q), cache, queries, q)
