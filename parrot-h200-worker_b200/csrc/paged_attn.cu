@@ -64,6 +64,19 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// *p, or zeros.  Volatile, as the products are: the load stays where it is written,
+// ahead of a chunk's softmax (moved behind it by the compiler: 64 sequences 26.4 us
+// and not 23.9).
+__device__ __forceinline__ uint2 load_or_zero(const uint2* p, bool live) {
+  uint2 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+      "@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y)
+      : "l"(p), "r"((int)live));
+  return v;
+}
+
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) != 0x7f80u; }
 
 // ---------------------------------------------------------------------------
@@ -88,16 +101,17 @@ __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7f80u) !
 // below 2^-32 of that); the keys' scales multiply the scores.  The values'
 // scales multiply the probabilities, w = p 2^e, and these go to f16 relative to
 // a power of two W per row, at 2^14 W^-1: 11 bits down to 2^-28 W, nothing lost
-// above 2^-39 W.  W is the power of two next above the largest w so far, each w
-// taken at the present maximum: it falls when the maximum moves and what it stood
-// for no longer counts (a W that only grew made keys of small scales vanish behind
-// those of large ones that softmax had since put out of account).
+// above 2^-39 W.  W is a power of two above the largest w so far, each w taken at
+// the present maximum, and at most 2^7 times that: it falls when the maximum has
+// moved and what it stood for no longer counts (a W that only grew made keys of
+// small scales vanish behind those of large ones that softmax had since put out of
+// account).
 //
 // Measured (8 heads on 2, width 96, a window of 2048, contexts of 4096): one
 // sequence 7.5 us, most of it the launch, the lists and the merge; 64 sequences
-// 25.6 us (3.9 TB/s) in bf16 and 24.4 (2.1 TB/s) in 8 bits, 256 of 2048 85 us
-// (4.7 TB/s) and 80.  In 8 bits what bounds it is the chain of a chunk's
-// instructions in each of the few warps that fit (240 registers, two CTAs an SM;
+// 25.7 us (3.9 TB/s) in bf16 and 24.0 (2.1 TB/s) in 8 bits, 256 of 2048 87 us
+// (4.6 TB/s) and 77.  In 8 bits what bounds it is the chain of a chunk's
+// instructions in each of the few warps that fit (246 registers, two CTAs an SM;
 // the schedulers issue in a fifth of the cycles); three CTAs of 168 registers are
 // slower, 34 us at 64 sequences, and so was the way over a widened tile in shared
 // memory (37 us).
@@ -243,7 +257,7 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
       const int rr = __shfl_sync(0xffffffffu, row, nt * 8 + g);
       const uint2* src = reinterpret_cast<const uint2*>(a.kv.key) + (long long)max(rr, 0) * (D / 8) + t;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) kr[nt][b] = rr < 0 ? make_uint2(0u, 0u) : src[4 * b];
+      for (int b = 0; b < NB; ++b) kr[nt][b] = load_or_zero(src + 4 * b, rr >= 0);
     }
     scales = row < 0 ? (uint32_t)kScaleBias * 0x101u
                      : (uint32_t)a.kv.key_scale[row] |
@@ -388,19 +402,19 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
             most_w[i] = fmaxf(most_w[i], s[nt][2 * i + e]);
           }
       }
-      // W is set anew where a weight reaches it, and where the maximum moves (O is
-      // rescaled then in any case)
-      const bool moved0 = corr[0] != 1.f || most_w[0] >= top_w[0];
-      const bool moved1 = two && (corr[1] != 1.f || most_w[1] >= top_w[1]);
-      if (__any_sync(0xffffffffu, moved0 || moved1)) {
+      // W is set anew where a weight reaches it or where a thread's have fallen 2^6
+      // below it (the quad's need not have: then it stays)
+      const bool off0 = most_w[0] >= top_w[0] || most_w[0] < top_w[0] * 0.015625f;
+      const bool off1 = two && (most_w[1] >= top_w[1] || most_w[1] < top_w[1] * 0.015625f);
+      if (__any_sync(0xffffffffu, off0 || off1)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float most = fmaxf(most_w[i], __shfl_xor_sync(0xffffffffu, most_w[i], 1));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          if (most > 0.f && (corr[i] != 1.f || most >= top_w[i])) {
+          if (most > 0.f) {
             // the power of two above it (at least 2^-100: its reciprocal is finite)
             const float w = fmaxf(__uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u), pow2(-100));
-            // most >= corr W / 2, so the product is below 2 (W / w alone may be past fp32)
+            // most >= corr W / 2^6, so the product is below 2^6 (W / w alone may be past fp32)
             corr[i] = corr[i] * top_w[i] * __uint_as_float((254u << 23) - __float_as_uint(w));
             top_w[i] = w;
           }
