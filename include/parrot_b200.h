@@ -641,8 +641,11 @@ int parrot_ep_read_status(const parrot_ep_dims* ep, const void* buffer, int* hos
  * streams or in several captured graphs at once, as long as no two write the
  * same rows.  A page number outside [0, pages) among the pages a call reads
  * or writes, a context longer than the table, or a position that does not
- * exist is recorded in `status` (device int[4], may be NULL): such a key and
- * value read as zeros, such a token is not written.
+ * exist is recorded in `status` (device int[4], may be NULL) as {2, site,
+ * number, 0}: such a key and value read as zeros, such a token is not written.
+ * The attention's waits are bounded: one that runs out (2 s) is recorded as
+ * {1, site, block, 0}, and the rows of its tile are NaN.  The first entry
+ * stays until the caller zeroes the word.
  * ---------------------------------------------------------------------- */
 typedef struct parrot_paged_kv {
   void* key;          /* [pages, n_kv_heads, page_size, head_dim] bf16 or e4m3 */

@@ -615,6 +615,8 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     for (int h = 0; h < groups && n > 0; ++h)
       if (h == g || ranks > 1) ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62) && ok;
     tc_fence_after();
+    // a wait that ran out: NaN, here or through the cluster's sum, not what is there by then
+    if (!ok) l = __uint_as_float(0x7fffffffu);
     const float inv = row_inverse(l, pos);
     float* part = reinterpret_cast<float*>(smem);
     unsigned char* own = smem + g * S::kQGroup;  // the warp's rows, bf16, where Q was
@@ -660,7 +662,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     if (ranks == 1) {
       const int2 th = map(min(r, rows - 1));
       __nv_bfloat16* out = a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D;
-      const unsigned long long at = ok && r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
+      const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
       constexpr int VR = D / 8;
       __syncwarp();
 #pragma unroll 4

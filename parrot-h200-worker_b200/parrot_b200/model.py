@@ -289,9 +289,11 @@ class LocalGQA(nn.Module):
         qkv = F.linear(x[0], w)
         q = bridge.b200_paged_append(kv, qkv, batch.page_table, batch.query_start,
                                      batch.context_len, c.n_heads,
-                                     rope=_rope_tables(c, x.device, torch.float32))
+                                     rope=_rope_tables(c, x.device, torch.float32),
+                                     status=batch.status)
         y = bridge.b200_paged_attention(q, kv, batch.page_table, batch.query_start,
-                                        batch.context_len, window=c.window_size, sinks=sinks)
+                                        batch.context_len, window=c.window_size, sinks=sinks,
+                                        status=batch.status)
         if batch.tokens < rows:
             y[batch.tokens:] = 0  # rows of no sequence
         return self.out(y.view(1, rows, -1))
@@ -399,10 +401,11 @@ class GlobalMLA(nn.Module):
         rows = x.shape[1]
         aq, ao = self._absorbed()
         bridge.b200_paged_append(kv, self.kv_down(x[0]), batch.page_table, batch.query_start,
-                                 batch.context_len, 0)
+                                 batch.context_len, 0, status=batch.status)
         q = F.linear(x[0], aq).view(rows, c.n_heads, c.kv_latent_dim)
         y = bridge.b200_paged_attention(q, kv, batch.page_table, batch.query_start,
-                                        batch.context_len, scale=c.head_dim ** -0.5)
+                                        batch.context_len, scale=c.head_dim ** -0.5,
+                                        status=batch.status)
         if batch.tokens < rows:
             y[batch.tokens:] = 0
         return F.linear(y.view(1, rows, -1), ao)
@@ -755,7 +758,9 @@ class Parrot(nn.Module):
     def extend(self, input_ids: Tensor, counts, state: PagedState, sequences=None) -> Tensor:
         """Append ``counts[i]`` tokens to sequence ``sequences[i]`` (default: 0, 1, ...) of
         ``state``.  ``input_ids`` [sum(counts)]: the new tokens, sequence by sequence.  Returns
-        the logits [with new tokens, vocab] after each of those sequences' last token."""
+        the logits [with new tokens, vocab] after each of those sequences' last token.
+        What the kernels find out of range, or a wait that runs out, is recorded in the state
+        (``state.read_status()``)."""
         cfg = self.config
         if self.training:
             raise RuntimeError("extend requires model.eval()")

@@ -13,6 +13,7 @@ keeps the pages and the lengths; the kernels read both from device memory.
     ids, logp = model.sample(logits, uniform, temperature=0.8, top_p=0.9)
     logits = model.extend(ids[:, 0], [1, 1], state, sequences=[0, 1])
     state.release(1)                     # its pages may be taken by another sequence
+    assert state.read_status()[0] == 0   # nothing was out of range, no wait ran out (synchronises)
 """
 from __future__ import annotations
 
@@ -51,6 +52,13 @@ class PagedState:
         self._free = list(range(pages - 1, -1, -1))
         self._owned: list[list[int]] = [[] for _ in range(sequences)]
         self._table = torch.full((sequences, width), -1, dtype=torch.int32)
+        self.status = torch.zeros(4, dtype=torch.int32, device=self.device)
+
+    def read_status(self) -> list[int]:
+        """The status word {code, site, info, 0} of the steps so far (synchronises): code 0 is ok,
+        1 a wait that ran out, 2 a page, position or length out of range.  The first entry stays;
+        ``status.zero_()`` clears it."""
+        return self.status.tolist()
 
     @property
     def free_pages(self) -> int:
@@ -103,7 +111,7 @@ class PagedState:
         ints = ints.to(self.device)
         n = len(seqs)
         return PagedBatch(ints[2 * n + 1:].view(n, width), ints[:n + 1], ints[n + 1:2 * n + 1],
-                          starts[-1])
+                          starts[-1], self.status)
 
     def advance(self, sequences: Sequence[int], counts: Sequence[int]) -> None:
         for b, n in zip(sequences, counts):
@@ -117,17 +125,18 @@ class PagedState:
         width = max(1, max(-(-n // self.page_size) for n in lengths))
         table = self._table[list(sequences), :width].to(self.device)
         return bridge.b200_paged_gather(self.layers[layer], table, torch.tensor(
-            lengths, dtype=torch.int32, device=self.device), max_len)
+            lengths, dtype=torch.int32, device=self.device), max_len, status=self.status)
 
 
 class PagedBatch:
-    """The device lists of one step (``bridge.b200_paged_*``)."""
+    """The device lists of one step (``bridge.b200_paged_*``), and where its calls report."""
 
-    __slots__ = ("page_table", "query_start", "context_len", "tokens")
+    __slots__ = ("page_table", "query_start", "context_len", "tokens", "status")
 
-    def __init__(self, page_table: Tensor, query_start: Tensor, context_len: Tensor, tokens: int):
+    def __init__(self, page_table: Tensor, query_start: Tensor, context_len: Tensor, tokens: int,
+                 status: Tensor | None = None):
         self.page_table, self.query_start, self.context_len = page_table, query_start, context_len
-        self.tokens = tokens
+        self.tokens, self.status = tokens, status
 
 
 def padded_rows(tokens: int) -> int:

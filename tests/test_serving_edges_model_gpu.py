@@ -1,0 +1,40 @@
+"""Serving through the model, at the edges: what a step reports, and which sequences it runs."""
+import pytest
+import torch
+
+from parrot_b200 import bridge
+from tests.test_model_gpu import TINY, _pair
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_step_reports_what_is_out_of_range_in_the_state():
+    prod, _ = _pair(TINY, seed=31)
+    ids = torch.randint(0, 32768, (40,), generator=torch.Generator().manual_seed(1)).cuda()
+    state = prod.paged_state(sequences=2, pages=8, page_size=16)
+    prod.extend(ids[:20], [20], state)
+    assert state.read_status() == [0, 0, 0, 0]
+    good = state._table.clone()
+    state._table[0, 0] = 77                       # a page that the pools do not have
+    prod.extend(ids[20:21], [1], state)           # read by the kernel for few queries
+    assert state.read_status()[:3] == [2, 52, 77]
+    state.status.zero_()
+    prod.extend(ids[21:], [19], state)            # and by the one for many
+    assert state.read_status()[:3] == [2, 52, 77]
+    state.status.zero_()
+    state.dense(0, [0])
+    assert state.read_status()[:3] == [2, 52, 77]
+    state.status.zero_()
+    state._table = good
+    state.release(0)
+    state.batch([0], [20])
+    state._table[0, 1] = -9                       # written by the append
+    prod.extend(ids[:20], [20], state)
+    assert state.read_status()[:3] == [2, 52, -9]
+
+
+def test_the_status_word_of_a_batch_is_the_states():
+    prod, _ = _pair(TINY, seed=31)
+    state = prod.paged_state(sequences=1, pages=2, page_size=16, kv_dtype=torch.float8_e4m3fn)
+    assert state.batch([0], [3]).status.data_ptr() == state.status.data_ptr()
+    assert state.status.device.type == "cuda" and bridge.PAGE_SIZES
