@@ -64,11 +64,29 @@ class PagedState:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _index(self, sequence: int) -> int:
+        b = int(sequence)
+        if not 0 <= b < len(self.lengths):
+            raise ValueError(f"sequences must be in [0, {len(self.lengths)}), got {b}")
+        return b
+
+    def _step(self, sequences: Sequence[int], counts: Sequence[int]) -> tuple[list[int], list[int]]:
+        """The step's sequences and counts as numbers, checked."""
+        seqs, counts = [self._index(b) for b in sequences], [int(n) for n in counts]
+        if len(seqs) != len(counts) or not seqs:
+            raise ValueError("one count for each sequence, and at least one sequence")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("sequences must be different")
+        if min(counts) < 0:
+            raise ValueError("counts must be >= 0")
+        return seqs, counts
+
     def pages_of(self, sequence: int) -> list[int]:
-        return list(self._owned[sequence])
+        return list(self._owned[self._index(sequence)])
 
     def reserve(self, sequences: Sequence[int], counts: Sequence[int]) -> None:
         """Pages for ``counts[i]`` more tokens of sequence ``sequences[i]``; all or none."""
+        sequences, counts = self._step(sequences, counts)
         need = []
         for b, n in zip(sequences, counts):
             if self.lengths[b] + n > self.max_positions:
@@ -84,6 +102,7 @@ class PagedState:
 
     def release(self, sequence: int) -> None:
         """Forget a sequence; its pages are free again."""
+        sequence = self._index(sequence)
         self._free.extend(reversed(self._owned[sequence]))
         self._owned[sequence] = []
         self._table[sequence] = -1
@@ -92,13 +111,9 @@ class PagedState:
     def batch(self, sequences: Sequence[int], counts: Sequence[int]) -> "PagedBatch":
         """Device lists of a step that appends ``counts[i]`` tokens to ``sequences[i]``
         (reserves their pages; the lengths grow when the step is done)."""
-        seqs, counts = [int(b) for b in sequences], [int(n) for n in counts]
-        if len(seqs) != len(counts) or not seqs:
-            raise ValueError("one count for each sequence, and at least one sequence")
-        if len(set(seqs)) != len(seqs) or min(seqs) < 0 or max(seqs) >= len(self.lengths):
-            raise ValueError(f"sequences must be different and in [0, {len(self.lengths)})")
-        if min(counts) < 0 or sum(counts) == 0:
-            raise ValueError("counts must be >= 0, and one of them positive")
+        seqs, counts = self._step(sequences, counts)
+        if sum(counts) == 0:
+            raise ValueError("one of the counts must be positive")
         self.reserve(seqs, counts)
         starts = [0]
         for n in counts:
@@ -114,16 +129,24 @@ class PagedState:
                           starts[-1], self.status)
 
     def advance(self, sequences: Sequence[int], counts: Sequence[int]) -> None:
+        """The tokens of a step are in the cache: on the pages that ``reserve`` gave them."""
+        sequences, counts = self._step(sequences, counts)
+        for b, n in zip(sequences, counts):
+            if self.lengths[b] + n > len(self._owned[b]) * self.page_size:
+                raise ValueError(f"sequence {b} has no pages for {n} more tokens")
         for b, n in zip(sequences, counts):
             self.lengths[b] += n
 
     def dense(self, layer: int, sequences: Sequence[int], max_len: int | None = None):
         """A layer's cache of these sequences as dense bf16 (key, value or None),
         [sequences, kv heads, max_len, width], zeros past each length."""
+        sequences = [self._index(b) for b in sequences]
+        if not sequences:
+            raise ValueError("at least one sequence")
         lengths = [self.lengths[b] for b in sequences]
         max_len = max(lengths) if max_len is None else max_len
         width = max(1, max(-(-n // self.page_size) for n in lengths))
-        table = self._table[list(sequences), :width].to(self.device)
+        table = self._table[sequences, :width].to(self.device)
         return bridge.b200_paged_gather(self.layers[layer], table, torch.tensor(
             lengths, dtype=torch.int32, device=self.device), max_len, status=self.status)
 

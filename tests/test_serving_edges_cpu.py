@@ -1,0 +1,36 @@
+"""Refusals of the paged state at the edges of its ranges."""
+import pytest
+import torch
+
+from tests.test_serving_cpu import _state
+
+
+@pytest.mark.parametrize("sequence", [-1, -3, 3, 100])
+def test_a_sequence_that_does_not_exist_is_refused_everywhere(sequence):
+    s = _state(pages=20)
+    s.batch([0, 1, 2], [17, 5, 33])
+    s.advance([0, 1, 2], [17, 5, 33])
+    pages, lengths, table = [s.pages_of(b) for b in range(3)], list(s.lengths), s._table.clone()
+    for call in (lambda: s.release(sequence), lambda: s.pages_of(sequence), lambda: s.dense(0, [0, sequence]),
+                 lambda: s.reserve([sequence], [1]), lambda: s.advance([sequence], [1]),
+                 lambda: s.batch([sequence], [1])):
+        with pytest.raises(ValueError, match="sequences must be in"):
+            call()
+    assert [s.pages_of(b) for b in range(3)] == pages and s.lengths == lengths and torch.equal(s._table, table)
+    assert s.free_pages == 20 - 6
+
+
+def test_reservations_and_lengths_that_do_not_fit_are_refused():
+    s = _state(pages=20)
+    for seqs, counts in (([0, 0], [10, 10]), ([0], [-1]), ([0, 1], [3]), ([], [])):
+        for call in (s.reserve, s.advance):
+            with pytest.raises(ValueError):
+                call(seqs, counts)
+    with pytest.raises(ValueError, match="at least one sequence"):
+        s.dense(0, [])
+    s.reserve([0], [16])
+    with pytest.raises(ValueError, match="no pages"):
+        s.advance([1, 0], [0, 17])
+    assert s.lengths == [0, 0, 0] and s.free_pages == 19
+    s.advance([0], [16])
+    assert s.lengths == [16, 0, 0]
