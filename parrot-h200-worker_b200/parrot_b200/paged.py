@@ -54,11 +54,15 @@ class PagedState:
         self._table = torch.full((sequences, width), -1, dtype=torch.int32)
         self.status = torch.zeros(4, dtype=torch.int32, device=self.device)
 
-    def read_status(self) -> list[int]:
+    @torch.inference_mode()
+    def read_status(self, clear: bool = False) -> list[int]:
         """The status word {code, site, info, 0} of the steps so far (synchronises): code 0 is ok,
-        1 a wait that ran out, 2 a page, position or length out of range.  The first entry stays;
-        ``status.zero_()`` clears it."""
-        return self.status.tolist()
+        1 a wait that ran out, 2 a page, position or length out of range.  The first entry stays
+        until it is read with ``clear``."""
+        word = self.status.tolist()
+        if clear:
+            self.status.zero_()
+        return word
 
     @property
     def free_pages(self) -> int:
@@ -137,6 +141,7 @@ class PagedState:
         for b, n in zip(sequences, counts):
             self.lengths[b] += n
 
+    @torch.inference_mode()
     def dense(self, layer: int, sequences: Sequence[int], max_len: int | None = None):
         """A layer's cache of these sequences as dense bf16 (key, value or None),
         [sequences, kv heads, max_len, width], zeros past each length."""

@@ -17,20 +17,19 @@ def test_a_step_reports_what_is_out_of_range_in_the_state():
     good = state._table.clone()
     state._table[0, 0] = 77                       # a page that the pools do not have
     prod.extend(ids[20:21], [1], state)           # read by the kernel for few queries
-    assert state.read_status()[:3] == [2, 52, 77]
-    state.status.zero_()
+    assert state.read_status(clear=True)[:3] == [2, 52, 77]
     prod.extend(ids[21:], [19], state)            # and by the one for many
-    assert state.read_status()[:3] == [2, 52, 77]
-    state.status.zero_()
+    assert state.read_status(clear=True)[:3] == [2, 52, 77]
     state.dense(0, [0])
-    assert state.read_status()[:3] == [2, 52, 77]
-    state.status.zero_()
+    assert state.read_status(clear=True)[:3] == [2, 52, 77]
     state._table = good
     state.release(0)
     state.batch([0], [20])
     state._table[0, 1] = -9                       # written by the append
     prod.extend(ids[:20], [20], state)
-    assert state.read_status()[:3] == [2, 52, -9]
+    assert state.read_status()[:3] == [2, 52, -9]   # the first entry stays
+    assert state.read_status(clear=True)[:3] == [2, 52, -9]
+    assert state.read_status() == [0, 0, 0, 0]
 
 
 def test_the_status_word_of_a_batch_is_the_states():
