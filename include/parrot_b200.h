@@ -665,7 +665,10 @@ typedef struct parrot_paged_kv {
  * query_start[b] + i is at position context_len[b] - (rows of b) + i.
  * Position p is row p % page_size of page page_table[b][p / page_size].  All
  * three arrays are in device memory; query_start does not decrease.  Rows from
- * query_start[batch] on belong to no sequence and nothing is written for them. */
+ * query_start[batch] on belong to no sequence and nothing is written for them.
+ * A sequence may have no rows; but which attention kernel runs follows from
+ * tokens / batch, so a batch of many such beside one long piece is slower than
+ * the piece alone. */
 typedef struct parrot_paged_batch {
   const int* page_table;    /* [batch, table_width] */
   const int* query_start;   /* [batch + 1] (parrot_paged_gather_bf16: not read) */

@@ -770,6 +770,7 @@ class Parrot(nn.Module):
         sequences = list(range(len(counts))) if sequences is None else list(sequences)
         if input_ids.ndim != 1 or input_ids.shape[0] != sum(counts):
             raise ValueError("input_ids must be [sum(counts)]")
+        sequences, counts = state.with_tokens(sequences, counts)
         batch = state.batch(sequences, counts)
         rows = padded_rows(batch.tokens)
         if rows > batch.tokens:

@@ -112,9 +112,16 @@ class PagedState:
         self._table[sequence] = -1
         self.lengths[sequence] = 0
 
+    def with_tokens(self, sequences: Sequence[int], counts: Sequence[int]) -> tuple[list[int], list[int]]:
+        """Of a step's sequences those that have new tokens, with their counts."""
+        step = [(b, n) for b, n in zip(*self._step(sequences, counts)) if n]
+        return [b for b, _ in step], [n for _, n in step]
+
     def batch(self, sequences: Sequence[int], counts: Sequence[int]) -> "PagedBatch":
         """Device lists of a step that appends ``counts[i]`` tokens to ``sequences[i]``
-        (reserves their pages; the lengths grow when the step is done)."""
+        (reserves their pages; the lengths grow when the step is done).  Sequences
+        without new tokens may be among them, but count when the attention kernel is
+        chosen by the tokens of a sequence: ``with_tokens`` leaves them out."""
         seqs, counts = self._step(sequences, counts)
         if sum(counts) == 0:
             raise ValueError("one of the counts must be positive")

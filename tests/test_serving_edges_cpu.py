@@ -34,3 +34,11 @@ def test_reservations_and_lengths_that_do_not_fit_are_refused():
     assert s.lengths == [0, 0, 0] and s.free_pages == 19
     s.advance([0], [16])
     assert s.lengths == [16, 0, 0]
+
+
+def test_the_sequences_of_a_step_that_have_tokens():
+    s = _state()
+    assert s.with_tokens([2, 0, 1], [0, 3, 1]) == ([0, 1], [3, 1]) and s.with_tokens([1], [0]) == ([], [])
+    for seqs, counts in (([0, 0], [1, 0]), ([3], [0]), ([0], [-1]), ([0, 1], [1])):
+        with pytest.raises(ValueError):
+            s.with_tokens(seqs, counts)

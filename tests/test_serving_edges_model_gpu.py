@@ -37,3 +37,28 @@ def test_the_status_word_of_a_batch_is_the_states():
     state = prod.paged_state(sequences=1, pages=2, page_size=16, kv_dtype=torch.float8_e4m3fn)
     assert state.batch([0], [3]).status.data_ptr() == state.status.data_ptr()
     assert state.status.device.type == "cuda" and bridge.PAGE_SIZES
+
+
+def test_sequences_without_new_tokens_do_not_change_a_step():
+    """Listed beside one long piece they chose the kernel for few tokens a sequence."""
+    prod, _ = _pair(TINY, seed=32)
+    ids = torch.randint(0, 32768, (200,), generator=torch.Generator().manual_seed(2)).cuda()
+    seen = []
+    attention = bridge.b200_paged_attention
+
+    def watch(q, kv, page_table, *args, **kw):
+        seen.append(page_table.shape[0])
+        return attention(q, kv, page_table, *args, **kw)
+    states = [prod.paged_state(sequences=120, pages=16, page_size=16) for _ in range(2)]
+    alone = prod.extend(ids, [200], states[0], sequences=[5])
+    bridge.b200_paged_attention = watch
+    try:
+        beside = prod.extend(ids, [200 * (b == 5) for b in range(120)], states[1])
+    finally:
+        bridge.b200_paged_attention = attention
+    assert set(seen) == {1} and torch.equal(alone, beside)
+    assert states[1].lengths == [200 * (b == 5) for b in range(120)]
+    with pytest.raises(ValueError):
+        prod.extend(ids[:0], [0, 0], states[1], sequences=[0, 1])
+    with pytest.raises(ValueError):
+        prod.extend(ids[:1], [1, 0], states[1], sequences=[0, 0])
