@@ -732,8 +732,10 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
  * drawn, and a row of nothing else gives id -1 and -inf.  temperature, top_k,
  * top_p, min_p: [rows] in device memory, or NULL for the *_all value in every
  * row.  Beside parrot_vocab_argmax_bf16 / parrot_argmax_rows_bf16, the greedy
- * choice of parrot/model.py:927-931.  Masses are summed exactly (fixed
- * point), so a draw depends on nothing but its arguments. */
+ * choice of parrot/model.py:927-931.  Masses are w rounded to multiples of
+ * 2^-44 and summed exactly, so a draw depends on nothing but its arguments;
+ * a border between two tokens is off by vocab * 2^-45 of the largest w at
+ * most, and a token of w <= 2^-45 is never drawn. */
 int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int logits_f32,
                        long long row_stride, int rows, int vocab, const float* uniform,
                        const float* temperature, float temperature_all, const int* top_k,

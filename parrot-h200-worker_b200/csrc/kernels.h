@@ -407,7 +407,7 @@ struct SampleArgs {
   int rows, vocab;
   int cluster;               // CTAs per row (set at launch)
 };
-constexpr int kSampleMaxVocab = 1 << 19;  // 2^19 masses of at most 2^44 fit 63 bits
+constexpr int kSampleMaxVocab = 1 << 19;  // 2^19 masses of at most 2^44 fit 64 bits
 int launch_sample(const SampleArgs& args, int sms, cudaStream_t stream);
 
 int launch_rmsnorm(__nv_bfloat16* out, const __nv_bfloat16* x, const __nv_bfloat16* w,

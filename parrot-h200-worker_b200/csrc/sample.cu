@@ -8,11 +8,13 @@
 // the first token always stays.  The token drawn is the first, by index, whose
 // cumulative mass over the kept set exceeds uniform times the set's mass.
 //
-// A draw near a border between two tokens must not depend on rounding or on
-// the order of a sum, so masses are 64-bit fixed point: w in double, rounded
-// once to multiples of 2^-44.  Integer sums are exact in any order, 2^19
-// tokens fit 63 bits, and the 2^-45 error of a term is far below a double's
-// error over a sum of that length.
+// A draw near a border between two tokens must not depend on the order of a
+// sum, so masses are 64-bit fixed point: w in double, rounded once to multiples of
+// 2^-44.  Integer sums are exact in any order, and the masses of 2^19 tokens (2^63
+// at most) fit.  A mass is off by at most 2^-45 of the largest, so a border by at
+// most vocab * 2^-45: 2^-30 for 32,768 tokens and 2^-26 for 2^19, below the 2^-24
+// of an fp32 uniform.  Over a long flat tail these errors have one sign: a token of
+// w <= 2^-45 has no mass at all and is never drawn.
 //
 // A cluster of CTAs shares a row (one CTA where the rows fill the GPU).  The
 // logits become order-preserving integer keys in shared memory, read from HBM

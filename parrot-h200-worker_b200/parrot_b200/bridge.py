@@ -997,8 +997,9 @@ def b200_sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float = 1
     ``min_p`` is a number for every row or a tensor [rows] (fp32; ``top_k``
     int32).  The filters apply in that order; the token is the first by index
     whose cumulative share of the kept set exceeds ``uniform``, and its
-    log-probability is the logarithm of its own share.  A row of only -inf or
-    NaN gives id -1 and -inf.
+    log-probability is the logarithm of its own share.  Weights count in multiples
+    of 2**-44 of the largest: a token of 2**-45 of it or less is never drawn.  A row
+    of only -inf or NaN gives id -1 and -inf.
     """
     index = _serving_device(logits, "sampling")
     if logits.dtype not in (torch.bfloat16, torch.float32):

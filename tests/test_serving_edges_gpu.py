@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from parrot_b200 import bridge
-from tests.serving_support import Paged, attention, quantise, starts
+from tests.serving_support import Paged, attention, quantise, sample_row, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,70 @@ def test_an_infinite_key_is_what_the_formula_says(queries, context, at, bad, e4m
         cache.key[page, 0, at % 16, 7] = bad
     q = _queries(sum(queries), 4, 96, 0)
     _assert_formula(_call(cache, queries, q), cache, queries, q)
+
+
+# ------------------------------------------------------------------------------------------ sampling
+def _assert_draws(logits, u, t, k, p, m, rows=None):
+    ids, logp = bridge.b200_sample(logits.cuda(), u.cuda(), t.cuda(), k.cuda(), p.cuda(), m.cuda())
+    for r in range(logits.shape[0]) if rows is None else rows:
+        token, want = sample_row(logits[r], float(u[r]), float(t[r]), int(k[r]), float(p[r]), float(m[r]))
+        assert int(ids[r, 0]) == token, (r, int(ids[r, 0]), token)
+        assert abs(float(logp[r]) - want) <= 2.0 ** -23 * abs(want) + 1e-7
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("where", ["at the top", "below it", "everywhere", "near one another"])
+def test_sampling_among_thousands_of_equal_logits(where, dtype):
+    """More tokens in one step of the histogram than the list of a step holds."""
+    rows, vocab = 8, 9001
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn(rows, vocab, generator=g)
+    at = torch.randperm(vocab, generator=g)[:6000]
+    if where == "at the top":
+        logits[:, at] = 5.0
+    elif where == "below it":
+        logits[:, at] = 2.0
+    elif where == "everywhere":
+        logits[:] = -1.5
+    else:   # a wide range, so that a step of it holds thousands of different logits
+        logits = logits * 1e-3
+        logits[:, 17] = -300.0
+    i = torch.arange(rows)
+    u = torch.rand(rows, generator=g)
+    one = torch.ones(rows)
+    for k, p in ((3000, 1.0), (0, 0.4), (5000, 0.5), (1, 1.0), (0, 0.9)):
+        _assert_draws(logits.to(dtype), u, one, (0 * i + k).int(), 0 * one + p, 0 * one)
+
+
+@pytest.mark.parametrize("dtype,vocab,rows", [(torch.bfloat16, 131072, 200), (torch.float32, 131072, 200),
+                                              (torch.float32, 500001, 2), (torch.bfloat16, 524288, 3)])
+def test_sampling_rows_longer_than_shared_memory_holds(dtype, vocab, rows):
+    g = torch.Generator().manual_seed(vocab)
+    logits = (2 * torch.randn(rows, vocab, generator=g)).to(dtype)
+    u = torch.rand(rows, generator=g)
+    i = torch.arange(rows)
+    t = torch.tensor([1.0, 0.7, 0.0])[i % 3]
+    k = torch.tensor([0, 40, 100000, 7])[i % 4].int()
+    p = torch.tensor([0.9, 1.0, 0.3])[(i // 2) % 3]
+    m = torch.tensor([0.0, 0.01])[(i // 3) % 2]
+    _assert_draws(logits, u, t, k, p, m, rows=list(range(0, rows, max(1, rows // 12))))
+
+
+@pytest.mark.parametrize("below", [28.0, 30.0, 31.0, 32.0])
+def test_sampling_a_long_flat_tail_near_the_last_bit(below):
+    """2**18 equal logits some 2**-43 below the largest: a mass is off by at most 2**-45 of the
+    largest, so a border by at most vocab * 2**-45."""
+    vocab = 1 << 18
+    logits = torch.full((vocab,), -below)
+    top = vocab // 3
+    logits[top] = 0.0
+    u = torch.cat([torch.tensor([0.0, 2.0 ** -44, 1 - 2.0 ** -24, 0.5]), torch.exp2(-torch.linspace(24, 32, 60))])
+    ids, logp = bridge.b200_sample(logits.cuda().expand(len(u), -1).contiguous(), u.cuda())
+    w = torch.exp(logits.double())
+    upto, total = torch.cumsum(w, 0), float(w.sum())
+    off = vocab * 2.0 ** -45
+    for r in range(len(u)):
+        token, target = int(ids[r]), float(u[r].double()) * total
+        assert float(upto[token] - w[token]) - off <= target <= float(upto[token]) + off
+        want = math.log(float(w[token]) / total)
+        assert abs(float(logp[r]) - want) <= off + 2.0 ** -23 * abs(want) + 1e-7
