@@ -652,7 +652,10 @@ typedef struct parrot_paged_kv {
   void* value;        /* the same, or NULL: the values are the keys (the latent cache
                          of parrot/model.py:399-432, one head) */
   void* key_scale;    /* e4m3: [pages, n_kv_heads, page_size] bytes; a row's values are
-                         its numbers times 2^(byte - 127).  bf16: NULL */
+                         its numbers times 2^(byte - 127), byte in 17 .. 246: what the
+                         append writes, and every value is then a bf16.  (Reading back
+                         takes 1 .. 254, with one rounding to bf16; the attention is
+                         not made for those.)  bf16: NULL */
   void* value_scale;
   int pages, n_kv_heads, page_size, head_dim;  /* pages * n_kv_heads * page_size in 1 .. 2^31 - 1;
                                                   page_size 16, 32, 64, 128 or 256;

@@ -737,7 +737,8 @@ class PagedKV:
     ``key`` [pages, kv heads, page size, head_dim] bf16 or ``float8_e4m3fn``;
     ``value`` the same, or None when the values are the keys (a latent cache).
     An 8-bit pool comes with ``key_scale`` / ``value_scale`` [pages, kv heads,
-    page size] uint8: a row's values are its numbers times 2**(byte - 127).
+    page size] uint8: a row's values are its numbers times 2**(byte - 127), byte in
+    17 .. 246 (what the append writes: every value is then a bf16).
     Position ``p`` of sequence ``b`` is row ``p % page size`` of page
     ``page_table[b, p // page size]``.
     """

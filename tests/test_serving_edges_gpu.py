@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from parrot_b200 import bridge
-from tests.serving_support import Paged, attention, quantise, sample_row, starts
+from tests.serving_support import E4M3, Paged, attention, quantise, sample_row, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -216,6 +216,51 @@ def test_an_infinite_key_is_what_the_formula_says(queries, context, at, bad, e4m
         cache.key[page, 0, at % 16, 7] = bad
     q = _queries(sum(queries), 4, 96, 0)
     _assert_formula(_call(cache, queries, q), cache, queries, q)
+
+
+# ------------------------------------------------------------------------------------------- scales
+def test_every_scale_reads_as_the_power_of_two_it_stands_for():
+    """Read back, all 256 numbers at the bytes 1 .. 254: number * 2**(byte - 127), rounded once to bf16 where that
+    leaves its normal numbers (the bytes that the append writes, 17 .. 246, never do)."""
+    page = 128
+    cache = Paged([4 * page], kv_heads=1, dim=128, page=page, e4m3=True, latent=True)
+    at = torch.arange(508)
+    numbers = torch.arange(256, dtype=torch.uint8).view(2, 128)[at % 2]
+    byte = (1 + at // 2).to(torch.uint8)
+    for j in range(508):
+        p = int(cache.table[0, j // page])
+        cache.key.view(torch.uint8)[p, 0, j % page] = numbers[j]
+        cache.key_scale[p, 0, j % page] = byte[j]
+    got, _ = bridge.b200_paged_gather(cache.device(), cache.table.cuda(), ints([508]), 508)
+    got = got[0, 0].cpu()
+    exact = numbers.view(E4M3).double() * torch.exp2(byte.double() - 127)[:, None]
+    want = exact.to(torch.bfloat16)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[~nan].view(torch.int16), want[~nan].view(torch.int16))
+    written = (byte >= 17) & (byte <= 246)
+    assert torch.equal(want[written].double().nan_to_num(), exact[written].nan_to_num())
+
+
+# --------------------------------------------------------------------------- pages that do not exist
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 60, 400])
+def test_a_missing_page_of_an_8_bit_cache_reads_as_zeros_and_is_reported(n, latent):
+    cache = Paged([600], kv_heads=1, dim=128 if latent else 64, page=32, seed=6, e4m3=True, latent=latent)
+    for wrong in (cache.pages, -1):
+        table = cache.table.clone()
+        table[0, 4] = wrong
+        status = ints([0, 0, 0, 0])
+        q = _queries(n, 2, cache.dim, 0)
+        out = _call(cache, [n], q, table=table, status=status)
+        zeroed = Paged.__new__(Paged)
+        zeroed.__dict__.update(cache.__dict__, key=cache.key.clone())
+        zeroed.key.view(torch.uint8)[int(cache.table[0, 4])] = 0
+        if not latent:
+            zeroed.value = cache.value.clone()
+            zeroed.value.view(torch.uint8)[int(cache.table[0, 4])] = 0
+        _assert_formula(out, zeroed, [n], q)
+        assert status.tolist()[0] == 2 and status.tolist()[2] == wrong
 
 
 # ------------------------------------------------------------------------------------------ sampling
