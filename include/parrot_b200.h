@@ -723,6 +723,15 @@ int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_ba
                                 const void* q, long long q_row_stride, void* out, int n_heads,
                                 int window, int sinks, float scale, int* status, void* stream);
 
+/* The same with fp32 queries and results over a bf16 latent cache (kv->value
+ * NULL, kv->e4m3 0): the absorbed query and its context, as
+ * parrot_decode_attention_bf16 takes them for the dense latent cache
+ * (parrot/model.py:417-432).  Queries and weights count to 2^-16 or better,
+ * sums are fp32.  q: [tokens, q_row_stride] fp32, a multiple of 4. */
+int parrot_paged_attention_f32(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                               const float* q, long long q_row_stride, float* out, int n_heads,
+                               int window, int sinks, float scale, int* status, void* stream);
+
 /* Draws one token per row of logits [rows, row_stride] (bf16, or fp32 with
  * logits_f32; vocab <= 2^19).  With w_i = exp((l_i - max l) / temperature):
  * the top_k tokens of largest w (0, or vocab and above: all; the lower index

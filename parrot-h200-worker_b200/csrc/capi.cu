@@ -1760,6 +1760,57 @@ int paged_batch(const parrot_paged_batch* b, const parrot_paged_kv* kv, bool rag
   return PARROT_OK;
 }
 
+// Attention with queries and results in bf16, or in fp32 over a bf16 latent cache.
+int paged_attention(const char* what, const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                    const void* q, long long q_row_stride, void* out, int f32, int n_heads,
+                    int window, int sinks, float scale, int* status, void* stream) {
+  parrot::PagedAttnArgs a{};
+  int rc = paged_kv(kv, &a.kv);
+  if (rc || (rc = paged_batch(batch, kv, true, &a.batch))) return rc;
+  if (f32 && (kv->value != nullptr || kv->e4m3))
+    return fail(PARROT_EUNSUPPORTED, "paged_attention: fp32 queries need a bf16 latent cache (value NULL)%s");
+  if (n_heads <= 0 || n_heads > 4096 || n_heads % kv->n_kv_heads)
+    return fail(PARROT_EINVAL, "paged_attention: n_heads must be a multiple of n_kv_heads, <= 4096%s");
+  if (window < 0 || sinks < 0)
+    return fail(PARROT_EINVAL, "paged_attention: window and sinks must be >= 0%s");
+  if (!(scale > 0.f) || scale > 1e30f)
+    return fail(PARROT_EINVAL, "paged_attention: scale must be positive and finite%s");
+  if (q_row_stride < (long long)n_heads * kv->head_dim || q_row_stride % (f32 ? 4 : 8))
+    return fail(PARROT_EINVAL, "paged_attention: q rows must hold every head, in whole 16-byte steps%s");
+  if ((long long)a.batch.tokens * n_heads > 0x7fffffffll)
+    return fail(PARROT_EINVAL, "paged_attention: tokens * n_heads must fit 31 bits%s");
+  if (a.batch.tokens == 0 || a.batch.batch == 0) return PARROT_OK;
+  if (q == nullptr || out == nullptr || !aligned16(q) || !aligned16(out))
+    return fail(PARROT_EINVAL, "paged_attention: null or misaligned pointer%s");
+  a.q = q;
+  a.q_row = q_row_stride;
+  a.out = out;
+  a.f32 = f32;
+  a.heads = n_heads;
+  // a window that no position of the table leaves is none
+  a.window = window < (long long)a.batch.table_width << a.kv.page_shift ? window : 0;
+  a.sinks = a.window > 0 ? sinks : 0;
+  a.scale = scale;
+  a.status = status;
+  const int sms = sm_count();
+  if (parrot::paged_few_queries(a, sms)) {
+    if (parrot::launch_paged_decode(a, sms, static_cast<cudaStream_t>(stream)))
+      return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
+    return check_launch(what);
+  }
+  CUtensorMap k_map{}, v_map{};
+  if (!kv->e4m3) {
+    const long long pool_rows = (long long)kv->pages * kv->n_kv_heads * kv->page_size;
+    if (!pool_map(&k_map, kv->key, pool_rows, kv->head_dim, kv->page_size) ||
+        (kv->value != nullptr &&
+         !pool_map(&v_map, kv->value, pool_rows, kv->head_dim, kv->page_size)))
+      return fail(PARROT_ECUDA, "paged_attention: tensor map encode failed%s");
+  }
+  if (parrot::launch_paged_prefill(a, k_map, v_map, sms, static_cast<cudaStream_t>(stream)))
+    return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
+  return check_launch(what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1820,48 +1871,15 @@ int parrot_paged_gather_bf16(const parrot_paged_kv* kv, const parrot_paged_batch
 int parrot_paged_attention_bf16(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
                                 const void* q, long long q_row_stride, void* out, int n_heads,
                                 int window, int sinks, float scale, int* status, void* stream) {
-  parrot::PagedAttnArgs a{};
-  int rc = paged_kv(kv, &a.kv);
-  if (rc || (rc = paged_batch(batch, kv, true, &a.batch))) return rc;
-  if (n_heads <= 0 || n_heads > 4096 || n_heads % kv->n_kv_heads)
-    return fail(PARROT_EINVAL, "paged_attention: n_heads must be a multiple of n_kv_heads, <= 4096%s");
-  if (window < 0 || sinks < 0)
-    return fail(PARROT_EINVAL, "paged_attention: window and sinks must be >= 0%s");
-  if (!(scale > 0.f) || scale > 1e30f)
-    return fail(PARROT_EINVAL, "paged_attention: scale must be positive and finite%s");
-  if (q_row_stride < (long long)n_heads * kv->head_dim || q_row_stride % 8)
-    return fail(PARROT_EINVAL, "paged_attention: q rows must hold every head, stride %% 8 == 0%s");
-  if ((long long)a.batch.tokens * n_heads > 0x7fffffffll)
-    return fail(PARROT_EINVAL, "paged_attention: tokens * n_heads must fit 31 bits%s");
-  if (a.batch.tokens == 0 || a.batch.batch == 0) return PARROT_OK;
-  if (q == nullptr || out == nullptr || !aligned16(q) || !aligned16(out))
-    return fail(PARROT_EINVAL, "paged_attention: null or misaligned pointer%s");
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.q_row = q_row_stride;
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.heads = n_heads;
-  // a window that no position of the table leaves is none
-  a.window = window < (long long)a.batch.table_width << a.kv.page_shift ? window : 0;
-  a.sinks = a.window > 0 ? sinks : 0;
-  a.scale = scale;
-  a.status = status;
-  const int sms = sm_count();
-  if (parrot::paged_few_queries(a, sms)) {
-    if (parrot::launch_paged_decode(a, sms, static_cast<cudaStream_t>(stream)))
-      return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
-    return check_launch("paged_decode_kernel");
-  }
-  CUtensorMap k_map{}, v_map{};
-  if (!kv->e4m3) {
-    const long long pool_rows = (long long)kv->pages * kv->n_kv_heads * kv->page_size;
-    if (!pool_map(&k_map, kv->key, pool_rows, kv->head_dim, kv->page_size) ||
-        (kv->value != nullptr &&
-         !pool_map(&v_map, kv->value, pool_rows, kv->head_dim, kv->page_size)))
-      return fail(PARROT_ECUDA, "paged_attention: tensor map encode failed%s");
-  }
-  if (parrot::launch_paged_prefill(a, k_map, v_map, sms, static_cast<cudaStream_t>(stream)))
-    return fail(PARROT_ECUDA, "paged_attention: launch failed%s");
-  return check_launch("paged_prefill_kernel");
+  return paged_attention("paged_attention_bf16", kv, batch, q, q_row_stride, out, 0, n_heads, window,
+                         sinks, scale, status, stream);
+}
+
+int parrot_paged_attention_f32(const parrot_paged_kv* kv, const parrot_paged_batch* batch,
+                               const float* q, long long q_row_stride, float* out, int n_heads,
+                               int window, int sinks, float scale, int* status, void* stream) {
+  return paged_attention("paged_attention_f32", kv, batch, q, q_row_stride, out, 1, n_heads, window,
+                         sinks, scale, status, stream);
 }
 
 int parrot_sample_rows(long long* ids, float* logprobs, const void* logits, int logits_f32,

@@ -372,9 +372,10 @@ struct PagedGatherArgs {
 struct PagedAttnArgs {
   PagedKV kv;
   PagedBatch batch;
-  const __nv_bfloat16* q;    // [tokens, heads, head_dim]
+  const void* q;             // [tokens, heads, head_dim] bf16, or fp32
   long long q_row;           // elements between tokens
-  __nv_bfloat16* out;        // [tokens, heads, head_dim]
+  void* out;                 // [tokens, heads, head_dim] of the same type
+  int f32;                   // fp32 queries and results (a bf16 latent cache)
   int heads, window, sinks;
   int cluster;               // CTAs that share a tile (set at launch)
   float scale;

@@ -138,7 +138,12 @@ struct DecodeShape {
   static_assert(kWarp >= kPart, "a warp's ring holds its result");
 };
 
-template <int D, bool E4M3, bool SEP, bool WIDE>
+// F32 (a bf16 latent): fp32 queries and results.  Queries and probabilities go to
+// the products as two bf16 numbers each, a high part and what it leaves, 2^-16 or
+// better: as good as fp32 beside the latents' own bf16, and what the single-token
+// kernel of the dense latent cache keeps.  Measured (8 heads, width 128, contexts of
+// 4096): one sequence 12.2 us, 64 sequences 25.2 (bf16 queries 10.2 and 22.1).
+template <int D, bool E4M3, bool SEP, bool WIDE, bool F32>
 __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, WIDE ? 1 : 2)
     paged_decode_kernel(PagedAttnArgs a) {
   using S = DecodeShape<D, E4M3, SEP, WIDE>;
@@ -164,16 +169,29 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
   // the two (token, head) rows of this thread in the product's layout
   int pos[2];
   uint32_t qf[KS][4];
+  [[maybe_unused]] uint32_t ql[F32 ? KS : 1][4];  // the low parts
   float row_scale[2];
-  const __nv_bfloat16* qrow[2];
+  typedef typename std::conditional<F32, float, __nv_bfloat16>::type Q;
+  const Q* qrow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int2 th = map(min(g + 8 * i, rows - 1));
     pos[i] = pos0 + th.x;
-    qrow[i] = a.q + (long long)(tile.first + th.x) * a.q_row + (long long)(kvh * group + th.y) * D;
+    qrow[i] = static_cast<const Q*>(a.q) + (long long)(tile.first + th.x) * a.q_row +
+              (long long)(kvh * group + th.y) * D;
     row_scale[i] = a.scale * kLog2e;
   }
-  if constexpr (!E4M3) {
+  if constexpr (F32) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = *reinterpret_cast<const float2*>(qrow[j & 1] + k * 16 + 2 * t + 8 * (j >> 1));
+        const Bf16Pairs p = split_queries(f.x, f.y);
+        qf[k][j] = p.hi;
+        ql[k][j] = p.lo;
+      }
+  } else if constexpr (!E4M3) {
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -348,6 +366,10 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
           ldmatrix_x4(b, k_u + (nt * 8 + (lane & 7)) * S::kRow + k2 * 64 + (lane >> 3) * 16);
           mma_16816(s[nt], qf[2 * k2], b[0], b[1]);
           mma_16816(s[nt], qf[2 * k2 + 1], b[2], b[3]);
+          if constexpr (F32) {
+            mma_16816(s[nt], ql[2 * k2], b[0], b[1]);
+            mma_16816(s[nt], ql[2 * k2 + 1], b[2], b[3]);
+          }
         }
     }
     const int base = base_of(c);
@@ -540,10 +562,17 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         uint32_t p[4];
+        [[maybe_unused]] uint32_t pl[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int nt = 2 * kk + (j >> 1);
-          p[j] = tc::pack_bf16x2(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
+          if constexpr (F32) {
+            const Bf16Pairs w = split_weights(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
+            p[j] = w.hi;
+            pl[j] = w.lo;
+          } else {
+            p[j] = tc::pack_bf16x2(s[nt][2 * (j & 1)], s[nt][2 * (j & 1) + 1]);
+          }
         }
 #pragma unroll
         for (int n2 = 0; n2 < NT / 2; ++n2) {
@@ -551,6 +580,10 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
           ldmatrix_x4_trans(b, v_u + (kk * 16 + (lane & 15)) * S::kRow + n2 * 32 + (lane >> 4) * 16);
           mma_16816(o[2 * n2], p, b[0], b[1]);
           mma_16816(o[2 * n2 + 1], p, b[2], b[3]);
+          if constexpr (F32) {
+            mma_16816(o[2 * n2], pl, b[0], b[1]);
+            mma_16816(o[2 * n2 + 1], pl, b[2], b[3]);
+          }
         }
       }
       __syncwarp();  // the stage may be filled again
@@ -605,10 +638,8 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
   auto write = [&](int r, int col, float4 v, float sum) {
     const int2 th = map(r);
     const float inv = row_inverse(sum, pos0 + th.x);
-    uint2 w;
-    w.x = tc::pack_bf16x2(v.x * inv, v.y * inv);
-    w.y = tc::pack_bf16x2(v.z * inv, v.w * inv);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D + col) = w;
+    const long long at = ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D + col;
+    store_out<F32>(a, at, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
   };
   for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * W) {
     const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
@@ -676,10 +707,10 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
 // CTAs of four warps, 36 with eight of eight, 22 with sixteen; of 8192: 16, 14 and
 // 11; of 4096, where the wide kind begins: 10.5 and 10.1; of 2048 it would lose: 7.6
 // and 10.0.
-template <int D, bool E4M3, bool SEP, bool WIDE>
+template <int D, bool E4M3, bool SEP, bool WIDE, bool F32>
 int launch_decode(PagedAttnArgs a, long long tiles, long long chunks, int most, int sms, cudaStream_t stream) {
   using S = DecodeShape<D, E4M3, SEP, WIDE>;
-  auto k = paged_decode_kernel<D, E4M3, SEP, WIDE>;
+  auto k = paged_decode_kernel<D, E4M3, SEP, WIDE, F32>;
   static std::atomic<unsigned long long> done{0};
   if (!once_per_device(done, [&] {
         return allow_shared(k, S::kBytes) &&
@@ -710,18 +741,19 @@ int launch_decode(PagedAttnArgs a, long long tiles, long long chunks, int most, 
   return cudaLaunchKernelEx(&cfg, k, a) == cudaSuccess ? 0 : -2;
 }
 
-template <int D, bool E4M3, bool SEP>
+template <int D, bool E4M3, bool SEP, bool F32 = false>
 int launch_decode_of(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
   const long long tiles = most_tiles(a, kDecRows), all = tiles * a.kv.kv_heads;
   const long long chunks = (most_keys(a, kDecRows, kDecKeys) + kDecKeys - 1) / kDecKeys;
   if (all * 16 <= sms && chunks >= 128)
-    return launch_decode<D, E4M3, SEP, true>(a, tiles, chunks, 16, sms, stream);
-  return launch_decode<D, E4M3, SEP, false>(a, tiles, chunks, 8, sms, stream);
+    return launch_decode<D, E4M3, SEP, true, F32>(a, tiles, chunks, 16, sms, stream);
+  return launch_decode<D, E4M3, SEP, false, F32>(a, tiles, chunks, 8, sms, stream);
 }
 
 template <int D>
 int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
   const bool sep = a.kv.value != nullptr;
+  if (a.f32) return launch_decode_of<D, false, false, true>(a, stream, sms);
   if (a.kv.key_scale != nullptr)
     return sep ? launch_decode_of<D, true, true>(a, stream, sms) : launch_decode_of<D, true, false>(a, stream, sms);
   return sep ? launch_decode_of<D, false, true>(a, stream, sms) : launch_decode_of<D, false, false>(a, stream, sms);

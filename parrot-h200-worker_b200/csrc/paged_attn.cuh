@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <numeric>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tc.cuh"
@@ -63,11 +64,53 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Four numbers of the output, from element `at` on.
+template <bool F32>
+__device__ __forceinline__ void store_out(const PagedAttnArgs& a, long long at, float4 v) {
+  if constexpr (F32)
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+  else
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+        make_uint2(tc::pack_bf16x2(v.x, v.y), tc::pack_bf16x2(v.z, v.w));
+}
+
 // 1 / sum of the weights of a row at position `pos`.  A row before the first
 // position sees no key: zeros.  One that sees keys of weight 0 alone (scores of
 // -infinity) has 0 / 0: NaN.
 __device__ __forceinline__ float row_inverse(float sum, int pos) {
   return sum != 0.f ? 1.f / sum : pos < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+}
+
+// A pair as two pairs of bf16, high parts and what they leave, together 2^-16 of
+// each number or better.
+struct Bf16Pairs {
+  uint32_t hi, lo;
+};
+// Of probabilities: both parts rounded to nearest.
+__device__ __forceinline__ Bf16Pairs split_weights(float x, float y) {
+  Bf16Pairs p;
+  p.hi = tc::pack_bf16x2(x, y);
+  const float2 h = bf16x2_to_float2(p.hi);
+  p.lo = tc::pack_bf16x2(x - h.x, y - h.y);
+  return p;
+}
+// Of queries: the high part cut off, so that the low part has its sign, and a low
+// part that would be zero 2^-24 of the high one.  An infinite key then gives both
+// products the same infinity, as it would give the number itself; zero stays zero.
+__device__ __forceinline__ float query_high(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x != x ? x : __uint_as_float(b & 0xffff0000u);
+}
+__device__ __forceinline__ float query_low(float x, float high) {
+  const float rest = x - high;
+  return rest != 0.f && fabsf(high) < INFINITY ? rest : high * 5.9604644775390625e-08f;
+}
+__device__ __forceinline__ Bf16Pairs split_queries(float x, float y) {
+  const float hx = query_high(x), hy = query_high(y);
+  Bf16Pairs p;
+  p.hi = tc::pack_bf16x2(hx, hy);
+  p.lo = tc::pack_bf16x2(query_low(x, hx), query_low(y, hy));
+  return p;
 }
 
 // A tile: `rows_per` consecutive (token, head) rows of one sequence.

@@ -40,6 +40,13 @@
 //
 // With few tiles a cluster of CTAs shares one, each taking a run of its key
 // tiles, and merges the results over distributed shared memory.
+//
+// F32 (a bf16 latent): fp32 queries and results.  Queries and probabilities are two
+// bf16 numbers each, a high part and what it leaves (2^-16 or better): a product of Q
+// K^T is two, of the two parts of Q in shared memory, and P's low parts take the half
+// of S that its high ones leave free in TMEM.  Twice the products, and two stages of
+// keys instead of four at width 128: 8 pieces of 256 at 4096 74.6 us (bf16 queries
+// 45.5), a prompt of 4096 122 (71).
 #include "paged_attn.cuh"
 
 namespace parrot {
@@ -61,8 +68,9 @@ __host__ __device__ constexpr int paged_box_rows(int d, int page) {
   return page < tile_keys(d) ? page : tile_keys(d);
 }
 
-template <int D, bool E4M3, bool SEP>
+template <int D, bool E4M3, bool SEP, bool F32 = false>
 struct PrefillShape {
+  static_assert(!F32 || (!E4M3 && !SEP), "fp32 queries: a bf16 latent");
   static constexpr int kGroups = tile_groups(D), kKeys = tile_keys(D);
   static constexpr int kRows = kGroup * kGroups, kRowWarps = 4 * kGroups;
   static constexpr int kLoadWarps = E4M3 ? 8 : 3;  // widening takes more
@@ -89,10 +97,11 @@ struct PrefillShape {
   static constexpr int kSlabs = D / 32;              // 64-byte columns of a tile
   static constexpr int kTile = kKeys * D * 2;
   static constexpr int kSlab = kKeys * 64;
-  static constexpr int kStages = D == 128 ? (SEP ? 2 : 4) : SEP ? 4 : 6;
+  static constexpr int kStages = D == 128 ? (SEP || F32 ? 2 : 4) : SEP || F32 ? 4 : 6;
   static constexpr int kSides = SEP ? 2 : 1;
   static constexpr int kQGroup = kGroup * D * 2, kQSlab = kGroup * 64;
-  static constexpr int kQ = kGroups * kQGroup;
+  static constexpr int kQHigh = kGroups * kQGroup;   // F32: the low parts lie behind
+  static constexpr int kQ = kQHigh * (F32 ? 2 : 1);
   static constexpr int kRing = kStages * kTile;
   // noted columns of each row of a V tile: those that are +inf or NaN, those that are
   // -inf or NaN (e4m3 has only NaN)
@@ -275,7 +284,7 @@ __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pai
 
 // A tile's results of up to K CTAs joined: U of the tile's 16-byte vectors at a
 // time, all of their remote loads on their way together.
-template <int D, int K, int U, typename St>
+template <int D, bool F32, int K, int U, typename St>
 __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, St& st, const float* part,
                                            const Tile& tile, const RowMap& map, int pos0, int rows, int kvh, int rank, int ranks, uint32_t live,
                                            int threads) {
@@ -319,11 +328,8 @@ __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, St& st, const
       }
       const int2 th = map(r);
       const float inv = row_inverse(sum, pos0 + th.x);
-      uint2 w;
-      w.x = pack_bf16x2(o.x * inv, o.y * inv);
-      w.y = pack_bf16x2(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(a.out + ((long long)(tile.first + th.x) * a.heads + kvh * map.group + th.y) * D +
-                                c * 4) = w;
+      const long long at = ((long long)(tile.first + th.x) * a.heads + kvh * map.group + th.y) * D + c * 4;
+      store_out<F32>(a, at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
   }
 }
@@ -331,7 +337,7 @@ __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, St& st, const
 // The end of the rows' warps: with several CTAs to a tile, each merges its share
 // of the tile's vectors.  (Working each row's weights out first and keeping eight
 // vectors on their way whatever the cluster: 3 us slower with eight CTAs.)
-template <int D, typename St>
+template <int D, bool F32, typename St>
 __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, St& st,
                                             unsigned char* smem, const Tile& tile,
                                             const RowMap& map, int pos0, int rows, int kvh, int rank, int ranks,
@@ -350,21 +356,21 @@ __device__ __forceinline__ void finish_rows(const PagedAttnArgs& a, St& st,
   cluster_sync();
   const float* part = reinterpret_cast<const float*>(smem);
   if (ranks == 2)
-    merge_rows<D, 2, 4>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, F32, 2, 4>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   else if (ranks <= 4)
-    merge_rows<D, 4, 2>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, F32, 4, 2>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   else
-    merge_rows<D, kMaxRanks, 1>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
+    merge_rows<D, F32, kMaxRanks, 1>(a, st, part, tile, map, pos0, rows, kvh, rank, ranks, live, threads);
   cluster_sync();  // nobody leaves while its result may be read
 }
 
 }  // namespace
 
-template <int D, bool E4M3, bool SEP>
-__global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
+template <int D, bool E4M3, bool SEP, bool F32>
+__global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP, F32>::kThreads, 1)
     paged_prefill_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map) {
-  using S = PrefillShape<D, E4M3, SEP>;
+  using S = PrefillShape<D, E4M3, SEP, F32>;
   constexpr int NS = S::kStages, T = S::kKeys, NG = S::kGroups, R = S::kRows;
   extern __shared__ unsigned char pf_raw[];
   __shared__ PrefillState<D, E4M3> st;
@@ -423,22 +429,40 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
   if (warp < S::kRowWarps) {  // the warp's 32 queries, swizzled; rows that do not exist are zeros
     const int r = warp * 32 + lane;
     const int2 th = map(r);
-    const uint4* mine = reinterpret_cast<const uint4*>(
-        a.q + (long long)(tile.first + th.x) * a.q_row + (long long)(kvh * group + th.y) * D);
+    const long long q_at = (long long)(tile.first + th.x) * a.q_row + (long long)(kvh * group + th.y) * D;
+    const void* mine = static_cast<const char*>(a.q) + q_at * (F32 ? 4 : 2);
     const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(mine) : 0ull;
     constexpr int VR = D / 8;
-    uint4 v[VR];
+    if constexpr (!F32) {
+      uint4 v[VR];
 #pragma unroll
-    for (int x = 0; x < VR; ++x) {  // side by side: 32 vectors of the warp's rows a step
-      const int i = 32 * x + lane;
-      const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
-      v[x] = src != nullptr ? src[i % VR] : make_uint4(0, 0, 0, 0);
-    }
+      for (int x = 0; x < VR; ++x) {  // side by side: 32 vectors of the warp's rows a step
+        const int i = 32 * x + lane;
+        const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
+        v[x] = src != nullptr ? src[i % VR] : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-    for (int x = 0; x < VR; ++x) {
-      const int i = 32 * x + lane;
-      *reinterpret_cast<uint4*>(smem + (warp >> 2) * S::kQGroup +
-                                sw64_at<kGroup>((warp & 3) * 32 + i / VR, i % VR)) = v[x];
+      for (int x = 0; x < VR; ++x) {
+        const int i = 32 * x + lane;
+        *reinterpret_cast<uint4*>(smem + (warp >> 2) * S::kQGroup +
+                                  sw64_at<kGroup>((warp & 3) * 32 + i / VR, i % VR)) = v[x];
+      }
+    } else {
+#pragma unroll 4
+      for (int x = 0; x < VR; ++x) {
+        const int i = 32 * x + lane;
+        const float4* src = reinterpret_cast<const float4*>(__shfl_sync(0xffffffffu, at, i / VR));
+        float4 f[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (src != nullptr) {
+          f[0] = src[2 * (i % VR)];
+          f[1] = src[2 * (i % VR) + 1];
+        }
+        const Bf16Pairs p0 = split_queries(f[0].x, f[0].y), p1 = split_queries(f[0].z, f[0].w);
+        const Bf16Pairs p2 = split_queries(f[1].x, f[1].y), p3 = split_queries(f[1].z, f[1].w);
+        unsigned char* dst = smem + (warp >> 2) * S::kQGroup + sw64_at<kGroup>((warp & 3) * 32 + i / VR, i % VR);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(p0.hi, p1.hi, p2.hi, p3.hi);
+        *reinterpret_cast<uint4*>(dst + S::kQHigh) = make_uint4(p0.lo, p1.lo, p2.lo, p3.lo);
+      }
     }
     fence_async_shared();
   }
@@ -567,6 +591,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         uint32_t p[16];
+        [[maybe_unused]] uint32_t pl[F32 ? 16 : 1];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float2 x = make_float2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
@@ -574,9 +599,16 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
           x.x = exp2_fast(x.x);
           x.y = exp2_fast(x.y);
           sum[k & 3] = __fadd2_rn(sum[k & 3], x);
-          p[k] = pack_bf16x2(x.x, x.y);
+          if constexpr (F32) {
+            const Bf16Pairs w = split_weights(x.x, x.y);
+            p[k] = w.hi;
+            pl[k] = w.lo;
+          } else {
+            p[k] = pack_bf16x2(x.x, x.y);
+          }
         }
         tmem_st16(s_at + 16 * c, p);
+        if constexpr (F32) tmem_st16(s_at + T / 2 + 16 * c, pl);
       }
       sum[0] = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
       l = sum[0].x + sum[0].y;
@@ -611,9 +643,9 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
       if (lane == 0) mbar_arrive(&st.p_ready[g]);
     }
     // ---------------- result ----------------
-    // a CTA's result for the cluster lies over all groups' tiles
+    // a CTA's result for the cluster, or in fp32, lies over all groups' tiles
     for (int h = 0; h < groups && n > 0; ++h)
-      if (h == g || ranks > 1) ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62) && ok;
+      if (h == g || ranks > 1 || F32) ok = wait_asleep(&st.o_done[h], 0, abort_flag, a.status, 62) && ok;
     tc_fence_after();
     // a wait that ran out: NaN, here or through the cluster's sum, not what is there by then
     if (!ok) l = __uint_as_float(0x7fffffffu);
@@ -640,7 +672,7 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
           if (minus >> k & 1) o[k] = __float_as_uint(__uint_as_float(o[k]) - INFINITY);
         }
       }
-      if (ranks == 1) {
+      if (ranks == 1 && !F32) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           uint4 w;
@@ -650,7 +682,11 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
           w.w = pack_bf16x2(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
           *reinterpret_cast<uint4*>(own + sw64_at<kGroup>(r & (kGroup - 1), c * 4 + v)) = w;
         }
-      } else if (n > 0) {
+      } else if (n > 0 || ranks == 1) {
+        if (F32 && ranks == 1) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+        }
         // rows of D floats, 16-byte vectors exchanged by the row's low bits so
         // that the lanes' stores fall in different banks
 #pragma unroll
@@ -661,20 +697,27 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
     }
     if (ranks == 1) {
       const int2 th = map(min(r, rows - 1));
-      __nv_bfloat16* out = a.out + ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D;
+      const long long out_at = ((long long)(tile.first + th.x) * a.heads + kvh * group + th.y) * D;
+      void* out = static_cast<char*>(a.out) + out_at * (F32 ? 4 : 2);
       const unsigned long long at = r < rows ? reinterpret_cast<unsigned long long>(out) : 0ull;
-      constexpr int VR = D / 8;
+      constexpr int VR = F32 ? D / 4 : D / 8;  // 16-byte vectors of a row
+      // (in fp32 over the tiles: with a wait that ran out, copies may still land there)
+      const uint32_t lost = F32 ? __ballot_sync(0xffffffffu, !ok) : 0u;
       __syncwarp();
 #pragma unroll 4
       for (int x = 0; x < VR; ++x) {
-        const int i = 32 * x + lane;
-        uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, at, i / VR));
-        if (dst != nullptr) dst[i % VR] = *reinterpret_cast<const uint4*>(own + sw64_at<kGroup>(quarter * 32 + i / VR, i % VR));
+        const int i = 32 * x + lane, ri = i / VR, c = i % VR;
+        uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, at, ri));
+        const void* src = F32 ? static_cast<const void*>(part + (warp * 32 + ri) * D + ((c ^ (ri & 7)) << 2))
+                              : static_cast<const void*>(own + sw64_at<kGroup>(quarter * 32 + ri, c));
+        uint4 w = *static_cast<const uint4*>(src);
+        if (lost >> ri & 1) w = make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
+        if (dst != nullptr) dst[c] = w;
       }
     }
     st.m[r] = m * scale2;
     st.l[r] = l;
-    finish_rows<D>(a, st, smem, tile, map, pos0, rows, kvh, rank, ranks, all, 32 * S::kRowWarps);
+    finish_rows<D, F32>(a, st, smem, tile, map, pos0, rows, kvh, rank, ranks, all, 32 * S::kRowWarps);
     return;
   }
   if constexpr (S::kRowRegs > 0) {
@@ -927,6 +970,13 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
         for (int k = 0; k < D / 16; ++k)
           mma_ss(tmem + h * T, qd + ((uint32_t)((k >> 1) * S::kQSlab + (k & 1) * 32) >> 4),
                  kd + ((uint32_t)((k >> 1) * S::kSlab + (k & 1) * 32) >> 4), id_s, k != 0, leader);
+        if constexpr (F32) {
+          const uint32_t ql = qd + (S::kQHigh >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tmem + h * T, ql + ((uint32_t)((k >> 1) * S::kQSlab + (k & 1) * 32) >> 4),
+                   kd + ((uint32_t)((k >> 1) * S::kSlab + (k & 1) * 32) >> 4), id_s, 1u, leader);
+        }
       };
       auto values = [&](int h, int s, uint32_t accumulate) {
         const uint32_t vd = sw64_lo(v_u + s * S::kTile, S::kSlab);
@@ -934,6 +984,12 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
         for (int k = 0; k < T / 16; ++k)
           mma_ts(tmem + S::kTmemO + h * D, tmem + h * T + k * 8, vd + (uint32_t)(k * 1024 >> 4), id_o,
                  k == 0 ? accumulate : 1u, leader);
+        if constexpr (F32) {
+#pragma unroll
+          for (int k = 0; k < T / 16; ++k)
+            mma_ts(tmem + S::kTmemO + h * D, tmem + h * T + T / 2 + k * 8, vd + (uint32_t)(k * 1024 >> 4), id_o, 1u,
+                   leader);
+        }
       };
       if ((ok = wait_asleep(&st.k_full[0], 0, abort_flag, a.status, 66))) {
         tc_fence_after();
@@ -986,11 +1042,11 @@ __global__ void __launch_bounds__(PrefillShape<D, E4M3, SEP>::kThreads, 1)
 
 namespace {
 
-template <int D, bool E4M3, bool SEP>
+template <int D, bool E4M3, bool SEP, bool F32 = false>
 int launch_prefill(PagedAttnArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map, int sms,
                    cudaStream_t stream) {
-  using S = PrefillShape<D, E4M3, SEP>;
-  auto k = paged_prefill_kernel<D, E4M3, SEP>;
+  using S = PrefillShape<D, E4M3, SEP, F32>;
+  auto k = paged_prefill_kernel<D, E4M3, SEP, F32>;
   const long long tiles = most_tiles(a, S::kRows);
   static std::atomic<unsigned long long> done{0};
   if (!once_per_device(done, [&] {
@@ -1039,6 +1095,7 @@ template <int D>
 int launch_prefill_d(const PagedAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, int sms,
                      cudaStream_t stream) {
   const bool sep = a.kv.value != nullptr;
+  if (a.f32) return launch_prefill<D, false, false, true>(a, k, v, sms, stream);
   if (a.kv.key_scale != nullptr)
     return sep ? launch_prefill<D, true, true>(a, k, v, sms, stream)
                : launch_prefill<D, true, false>(a, k, v, sms, stream);

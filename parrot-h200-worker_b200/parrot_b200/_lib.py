@@ -187,6 +187,9 @@ _SIGNATURES = {
     "parrot_paged_attention_bf16": (c_int, [POINTER(PagedKVStruct), POINTER(PagedBatchStruct),
                                             c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int,
                                             c_int, c_float, c_void_p, c_void_p]),
+    "parrot_paged_attention_f32": (c_int, [POINTER(PagedKVStruct), POINTER(PagedBatchStruct),
+                                           c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int,
+                                           c_int, c_float, c_void_p, c_void_p]),
     "parrot_sample_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int, ctypes.c_longlong, c_int,
                                    c_int, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p,
                                    c_float, c_void_p, c_float, c_void_p]),

@@ -865,10 +865,11 @@ def _status_ptr(status: Tensor | None, index: int) -> int | None:
     return status.data_ptr()
 
 
-def _rows_of(t: Tensor) -> tuple[Tensor, int]:
-    """``t`` [rows, width] with 16-byte rows (a copy if need be), and its row stride."""
+def _rows_of(t: Tensor, vector: int = 8) -> tuple[Tensor, int]:
+    """``t`` [rows, width] with rows of whole 16-byte vectors (of ``vector`` numbers; a copy if
+    need be), and its row stride."""
     stride, step = t.stride()
-    if step != 1 or stride % 8 or t.data_ptr() % 16 or stride < t.shape[1]:
+    if step != 1 or stride % vector or t.data_ptr() % 16 or stride < t.shape[1]:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -952,19 +953,22 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
                          scale: float | None = None, status: Tensor | None = None) -> Tensor:
     """Causal attention of a ragged batch over the paged cache (append first).
 
-    ``q`` [tokens, heads, head_dim] bf16 (rows may be strided); token ``i`` of
+    ``q`` [tokens, heads, head_dim] bf16, or fp32 over a bf16 latent cache (the absorbed
+    query, as ``b200_decode_attention`` takes it); rows may be strided.  Token ``i`` of
     sequence ``b`` sees the keys ``j <= p`` of its context with ``window == 0``,
     ``p - j < window`` or ``j < sinks``.  Query head ``h`` reads key head
     ``h // (heads / kv heads)``.  ``scale`` defaults to head_dim ** -0.5.  Returns
-    [tokens, heads, head_dim] bf16; zeros for a token that sees no key.  Rows of no
+    [tokens, heads, head_dim] of ``q``'s type; zeros for a token that sees no key.  Rows of no
     sequence are not written.  A page that does not exist counts as zeros, and
     ``status`` (int32 [4]) records it.
     """
     index = _serving_device(kv.key, "paged attention")
     s = kv.struct
-    if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.get_device() != index or q.shape[2] != s.head_dim:
+    fp32 = q.dtype is torch.float32 and kv.value is None and not s.e4m3
+    if q.ndim != 3 or (q.dtype is not torch.bfloat16 and not fp32) or q.get_device() != index or \
+            q.shape[2] != s.head_dim:
         raise RuntimeError(f"The B200 paged attention takes bf16 queries [tokens, heads, "
-                           f"{s.head_dim}] on cuda:{index}")
+                           f"{s.head_dim}] on cuda:{index} (fp32 too over a bf16 latent cache)")
     tokens, heads, dim = q.shape
     batch, keep = _paged_batch(kv, page_table, query_start, context_len, tokens)
     if heads % s.n_kv_heads:
@@ -978,10 +982,12 @@ def b200_paged_attention(q: Tensor, kv: PagedKV, page_table: Tensor, query_start
     else:
         if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
             q = q.contiguous()
-        rows, stride = _rows_of(q.as_strided((tokens, width), (q.stride(0), 1)))
+        rows, stride = _rows_of(q.as_strided((tokens, width), (q.stride(0), 1)), 4 if fp32 else 8)
         out = q.new_empty((tokens, heads, dim))
     if tokens:
-        _on_device(index, "parrot_paged_attention_bf16", _lib.load().parrot_paged_attention_bf16, (
+        lib = _lib.load()
+        _on_device(index, "parrot_paged_attention", lib.parrot_paged_attention_f32 if fp32
+                   else lib.parrot_paged_attention_bf16, (
             s, batch, rows.data_ptr(), max(stride, width), out.data_ptr(), heads, window, sinks,
             dim ** -0.5 if scale is None else scale, _status_ptr(status, index)))
     return out

@@ -350,6 +350,14 @@ class GlobalMLA(nn.Module):
             self.__dict__["_absorbed_cache"] = hit
         return hit[1]
 
+    def _absorbed_twice(self) -> Tensor:
+        """The output weight beside itself, for a context in two parts."""
+        self._absorbed()
+        hit = self.__dict__["_absorbed_cache"]
+        if len(hit) == 3:
+            hit = self.__dict__["_absorbed_cache"] = (*hit, torch.cat((hit[1][1],) * 2, 1))
+        return hit[3]
+
     def _absorbed_f32(self) -> tuple[Tensor, Tensor]:
         """``_absorbed()`` as fp32 tensors (the bf16-rounded values, exactly)."""
         self._absorbed()
@@ -396,19 +404,37 @@ class GlobalMLA(nn.Module):
 
     def extend(self, x: Tensor, kv: bridge.PagedKV, batch: PagedBatch, sinks: int) -> Tensor:
         """New tokens of a ragged batch ``x`` [1, rows, dim] over the paged latent cache, by the
-        absorbed weights (every earlier token is visible: no window, no sinks)."""
+        absorbed weights (every earlier token is visible: no window, no sinks).  Over a bf16 cache
+        the absorbed query and its context are fp32, as ``decode`` has them (``model.py:417-432``);
+        over an 8-bit one, whose rows are off by up to 2**-4, they are bf16."""
         c = self.cfg
         rows = x.shape[1]
         aq, ao = self._absorbed()
+        fp32 = kv.key.dtype == torch.bfloat16
+        small = fp32 and rows <= _SMALL_LINEAR_ROWS
+        aq32, ao32 = self._absorbed_f32()
         bridge.b200_paged_append(kv, self.kv_down(x[0]), batch.page_table, batch.query_start,
                                  batch.context_len, 0, status=batch.status)
-        q = F.linear(x[0], aq).view(rows, c.n_heads, c.kv_latent_dim)
+        if small:
+            q = bridge.b200_linear_small(x[0], aq32, torch.float32)
+        else:  # products of bf16 numbers, summed in fp32
+            q = torch.mm(x[0], aq.t(), out_dtype=torch.float32) if fp32 else F.linear(x[0], aq)
+        q = q.view(rows, c.n_heads, c.kv_latent_dim)
         y = bridge.b200_paged_attention(q, kv, batch.page_table, batch.query_start,
                                         batch.context_len, scale=c.head_dim ** -0.5,
                                         status=batch.status)
         if batch.tokens < rows:
             y[batch.tokens:] = 0
-        return F.linear(y.view(1, rows, -1), ao)
+        y = y.view(rows, -1)
+        if small:
+            return bridge.b200_linear_small(y, ao32, x.dtype).view(1, rows, -1)
+        if not fp32:
+            return F.linear(y, ao).view(1, rows, -1)
+        # an fp32 context as the sum of two bf16 ones, a high part and what it leaves
+        high = y.to(x.dtype)
+        parts = torch.cat((high, (y - high).to(x.dtype)), 1)
+        out = torch.mm(parts, self._absorbed_twice().t(), out_dtype=torch.float32)
+        return out.to(x.dtype).view(1, rows, -1)
 
 
 class SwiGLU(nn.Module):

@@ -1,8 +1,12 @@
-"""Refusals of the paged state at the edges of its ranges."""
+"""Refusals of the serving calls and the paged state at the edges of their ranges."""
+import ctypes
+
 import pytest
 import torch
 
-from tests.test_serving_cpu import _state
+from tests.test_serving_cpu import E, _batch, _kv, _state, lib  # noqa: F401 (lib is a fixture)
+
+UNSUPPORTED = -3
 
 
 @pytest.mark.parametrize("sequence", [-1, -3, 3, 100])
@@ -42,3 +46,15 @@ def test_the_sequences_of_a_step_that_have_tokens():
     for seqs, counts in (([0, 0], [1, 0]), ([3], [0]), ([0], [-1]), ([0, 1], [1])):
         with pytest.raises(ValueError):
             s.with_tokens(seqs, counts)
+
+
+def test_attention_in_fp32_refuses_what_it_cannot_take(lib):  # noqa: F811
+    def attend(kv=_kv(value=None), q=256, stride=768, out=256, heads=8, scale=0.1, **batch):
+        return lib.parrot_paged_attention_f32(ctypes.byref(kv), ctypes.byref(_batch(**batch)), q, stride, out, heads,
+                                              0, 0, scale, None, None)
+    for kw in (dict(kv=_kv()), dict(kv=_kv(value=None, e4m3=1, key_scale=256))):
+        assert attend(**kw) == UNSUPPORTED, kw
+    for kw in (dict(q=None), dict(q=8), dict(stride=766), dict(stride=767), dict(out=None), dict(out=4), dict(heads=7),
+               dict(scale=0.0), dict(kv=_kv(value=None, page_size=48)), dict(tokens=-1)):
+        assert attend(**kw) == E, kw
+    assert attend(tokens=0) == 0

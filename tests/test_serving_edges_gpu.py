@@ -218,6 +218,81 @@ def test_an_infinite_key_is_what_the_formula_says(queries, context, at, bad, e4m
     _assert_formula(_call(cache, queries, q), cache, queries, q)
 
 
+# ------------------------------------------------------------------------------------- fp32 queries
+def _assert_formula_f32(out, cache, queries, q, window=0, sinks=0, scale=None):
+    """Within a bound that bf16 queries, weights or results would miss.
+
+    Queries and weights are two bf16 numbers each, off by at most 2**-16 and 2**-17.  With
+    S = scale sum |q| |k|, a score is off by 2**-16 S and by D + 3 fp32 roundings of its terms (2**-22 S
+    each at most, however the products are summed), so a weight by twice that, relative; the sums over
+    the keys by 2**-16 more.  Where S is small beside 1 a result is off by less than a step of 2**-14.
+    """
+    scale = cache.dim ** -0.5 if scale is None else scale
+    want, bound = attention(q, cache, queries, window, sinks, scale)
+    mass = bound / (2.0 ** -8 + 2.0 ** -12)                 # at least sum p |v| / sum p
+    first = 0
+    size = torch.zeros(q.shape[0], q.shape[1], 1, dtype=torch.float64)
+    for b, n in enumerate(queries):
+        k = cache.rows("key", b).abs().nan_to_num(0.0, 0.0)
+        if n:
+            size[first:first + n] = (q[first:first + n].double().abs().nan_to_num(0.0, 0.0)
+                                     @ k[0].T).amax(-1, keepdim=True) * scale
+        first += n
+    tight = mass * (2 * (2.0 ** -16 + (cache.dim + 3) * 2.0 ** -22) * size + 2.0 ** -16 + 2.0 ** -17)
+    assert out.dtype == torch.float32
+    got = out.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    finite = torch.isfinite(want)
+    assert bool(((got - want).abs() <= tight.expand_as(want))[finite].all())
+
+
+@pytest.mark.parametrize("heads,dim", [(8, 128), (3, 96), (40, 64), (4, 32)])
+@pytest.mark.parametrize("queries,contexts,page,window,sinks", [
+    ([1], [1], 16, 0, 0), ([1, 1, 1, 1], [1, 63, 64, 65], 64, 0, 0), ([1, 1], [300, 1000], 16, 7, 100),
+    ([2, 4, 3, 1], [2, 400, 64, 513], 64, 60, 1), ([1], [5000], 64, 0, 0), ([40], [40], 64, 0, 0),
+    ([129, 1, 0, 65], [129, 500, 30, 700], 32, 0, 0), ([300, 130], [300, 513], 128, 100, 5),
+    ([257], [1024], 64, 200, 130), ([64] * 40, [200] * 40, 32, 0, 0)])
+def test_fp32_queries_over_a_latent_cache(queries, contexts, page, window, sinks, heads, dim):
+    cache = Paged(contexts, kv_heads=1, dim=dim, page=page, latent=True, seed=len(queries) + page)
+    q = torch.randn(sum(queries), heads, dim, generator=torch.Generator().manual_seed(page + window))
+    out = _call(cache, queries, q, window, sinks)
+    _assert_formula_f32(out, cache, queries, q, window, sinks)
+
+
+@pytest.mark.parametrize("queries", [[1], [200]])
+def test_fp32_queries_strided_and_rows_of_nobody(queries):
+    n = sum(queries)
+    cache = Paged([n + 30], kv_heads=1, dim=96, page=16, latent=True, seed=2)
+    wide = torch.randn(n + 3, 5, 104, generator=torch.Generator().manual_seed(3))
+    for view in (wide[:, 1:4, 4:100], wide.flatten(1)[:, 4:292].unflatten(1, (3, 96)),
+                 wide.flatten(1)[:, 1:289].unflatten(1, (3, 96))):
+        dev = wide.cuda()
+        q = torch.as_strided(dev, view.shape, view.stride(), view.storage_offset())
+        out = bridge.b200_paged_attention(q, cache.device(), cache.table.cuda(), starts(queries).cuda(),
+                                          ints(cache.contexts))
+        _assert_formula_f32(out[:n].cpu(), cache, queries, view[:n].contiguous())
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("queries,context,at", [([1], 300, 100), ([4], 60, 57), ([130], 140, 100), ([130], 1000, 200)])
+def test_fp32_queries_and_an_infinite_latent_row(queries, context, at, bad):
+    """Both parts of a query have its sign: their products with an infinity are the same one."""
+    cache = Paged([context], kv_heads=1, dim=128, page=16, latent=True, seed=4)
+    cache.key[int(cache.table[0, at // 16]), 0, at % 16, 5] = bad
+    q = torch.randn(sum(queries), 8, 128, generator=torch.Generator().manual_seed(0))
+    q[:, 1] = q[:, 1].to(torch.bfloat16).float()     # nothing left for the low part
+    q[:, 2, 5] = 0.0
+    _assert_formula_f32(_call(cache, queries, q), cache, queries, q)
+
+
+def test_fp32_queries_need_a_bf16_latent_cache():
+    q = torch.zeros(1, 2, 96, device="cuda")
+    for kw in (dict(latent=False), dict(latent=True, e4m3=True)):
+        cache = Paged([4], kv_heads=1, dim=96, page=16, **kw)
+        with pytest.raises(RuntimeError, match="bf16 latent"):
+            bridge.b200_paged_attention(q, cache.device(), cache.table.cuda(), ints([0, 1]), ints([4]))
+
+
 # ------------------------------------------------------------------------------------------- scales
 def test_every_scale_reads_as_the_power_of_two_it_stands_for():
     """Read back, all 256 numbers at the bytes 1 .. 254: number * 2**(byte - 127), rounded once to bf16 where that

@@ -62,3 +62,64 @@ def test_sequences_without_new_tokens_do_not_change_a_step():
         prod.extend(ids[:0], [0, 0], states[1], sequences=[0, 1])
     with pytest.raises(ValueError):
         prod.extend(ids[:1], [1, 0], states[1], sequences=[0, 0])
+
+
+@pytest.mark.parametrize("pieces", [(1,), (3, 5), (9, 1), (200, 1, 40)])
+def test_the_latent_layer_keeps_the_precision_of_the_dense_decode_step(pieces):
+    """Over a bf16 cache the absorbed query, the weights and the context are not rounded to bf16.
+
+    Against the formula in 64 bits from the same bf16 inputs, weights and latents: the result's one
+    rounding (half a step, 2**-8 relative), and 2**-12 of its terms for the sums in fp32 and the two-part
+    products (2**-16 each, times scores of up to 8).  A bf16 query or context would add 2**-8 of a
+    context's numbers, which the second assertion holds to a quarter of that over the whole result.
+    """
+    from parrot_b200 import ModelConfig
+    from parrot_b200.model import GlobalMLA, MLALatentCache
+    cfg = ModelConfig()
+    torch.manual_seed(5)
+    layer = GlobalMLA(cfg).to("cuda", torch.bfloat16).eval()
+    contexts = [n + 60 for n in pieces]
+    with torch.inference_mode():
+        for p in layer.parameters():
+            p.normal_(0, 0.036)
+        aq, ao = (w.double() for w in layer._absorbed())
+        state = pm_state(cfg, contexts)
+        kv = state.layers[0]
+        prefix = [torch.randn(1, 60, cfg.dim, device="cuda").bfloat16() for _ in pieces]
+        for b, x in enumerate(prefix):
+            layer.extend(x, kv, state.batch([b], [60]), 0)
+            state.advance([b], [60])
+        x = torch.randn(1, sum(pieces), cfg.dim, device="cuda").bfloat16()
+        got = layer.extend(x, kv, state.batch(range(len(pieces)), pieces), 0)[0]
+        state.advance(range(len(pieces)), pieces)
+        lat, _ = state.dense(0, range(len(pieces)))
+        first, err, size = 0, 0.0, 0.0
+        for b, n in enumerate(pieces):
+            k = lat[b, 0, :contexts[b]].double()
+            q = (x[0, first:first + n].double() @ aq.T).view(n, cfg.n_heads, -1)
+            z = torch.einsum("thd,sd->hts", q, k) * cfg.head_dim ** -0.5
+            assert float(z.abs().max()) < 8
+            pos = torch.arange(contexts[b] - n, contexts[b], device="cuda")[:, None]
+            z = z.masked_fill(torch.arange(contexts[b], device="cuda")[None] > pos, -float("inf"))
+            ctx = torch.einsum("hts,sd->thd", torch.softmax(z, -1), k).reshape(n, -1)
+            want = ctx @ ao.T
+            terms = ctx.abs() @ ao.abs().T
+            off = (got[first:first + n].double() - want).abs()
+            assert bool((off <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * terms).all())
+            rounded = (want.bfloat16().double() - want)
+            err += float((got[first:first + n].double() - want).pow(2).sum())
+            size += float(rounded.pow(2).sum())
+            # and the dense cache's step gives the last token the same
+            cache = MLALatentCache(lat[b:b + 1, 0, :contexts[b]].clone())
+            at = torch.full((1,), contexts[b] - 1, device="cuda", dtype=torch.int32)
+            dense = layer.decode(x[:, first + n - 1:first + n], cache, contexts[b] - 1, position_device=at)[0, 0]
+            assert bool(((dense - got[first + n - 1]).double().abs()
+                         <= 2.0 ** -7 * want[-1].abs() + 2.0 ** -11 * terms[-1]).all())
+            first += n
+        # root mean square: the result's rounding alone, and a quarter of one more at most
+        assert err ** 0.5 <= 1.04 * size ** 0.5
+
+
+def pm_state(cfg, contexts):
+    from parrot_b200 import PagedState
+    return PagedState(cfg, len(contexts), sum(-(-n // 16) for n in contexts), 16, torch.bfloat16, 0, "cuda", [False])
