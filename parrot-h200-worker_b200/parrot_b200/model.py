@@ -411,7 +411,8 @@ class GlobalMLA(nn.Module):
         rows = x.shape[1]
         aq, ao = self._absorbed()
         fp32 = kv.key.dtype == torch.bfloat16
-        small = fp32 and rows <= _SMALL_LINEAR_ROWS
+        # (b200_linear_small takes inputs of up to 1024 numbers)
+        small = fp32 and rows <= _SMALL_LINEAR_ROWS and max(c.dim, aq.shape[0]) <= 1024
         aq32, ao32 = self._absorbed_f32()
         bridge.b200_paged_append(kv, self.kv_down(x[0]), batch.page_table, batch.query_start,
                                  batch.context_len, 0, status=batch.status)

@@ -120,6 +120,32 @@ def test_the_latent_layer_keeps_the_precision_of_the_dense_decode_step(pieces):
         assert err ** 0.5 <= 1.04 * size ** 0.5
 
 
+@pytest.mark.parametrize("n", [1, 8, 30])
+def test_a_latent_layer_of_more_heads_than_a_small_projection_takes(n):
+    """16 heads of a latent of 128: 2048 numbers a row, more than b200_linear_small holds."""
+    from parrot_b200 import ModelConfig
+    from parrot_b200.model import GlobalMLA
+    cfg = ModelConfig(n_heads=16, head_dim=32)
+    torch.manual_seed(6)
+    layer = GlobalMLA(cfg).to("cuda", torch.bfloat16).eval()
+    with torch.inference_mode():
+        for p in layer.parameters():
+            p.normal_(0, 0.036)
+        state = pm_state(cfg, [n])
+        x = torch.randn(1, n, cfg.dim, device="cuda").bfloat16()
+        got = layer.extend(x, state.layers[0], state.batch([0], [n]), 0)[0]
+        state.advance([0], [n])
+        k = state.dense(0, [0])[0][0, 0].double()
+        aq, ao = (w.double() for w in layer._absorbed())
+        z = torch.einsum("thd,sd->hts", (x[0].double() @ aq.T).view(n, 16, -1), k) * 32 ** -0.5
+        z = z.masked_fill(torch.ones(n, n, device="cuda").triu(1).bool(), -float("inf"))
+        ctx = torch.einsum("hts,sd->thd", torch.softmax(z, -1), k).reshape(n, -1)
+        want, terms = ctx @ ao.T, ctx.abs() @ ao.abs().T
+    # the bound of the test above, its 2**-12 for scores of up to 8 taken by size
+    size = 1 + float(z[z > -1e30].abs().max()) / 8
+    assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * size * terms).all())
+
+
 def pm_state(cfg, contexts):
     from parrot_b200 import PagedState
     return PagedState(cfg, len(contexts), sum(-(-n // 16) for n in contexts), 16, torch.bfloat16, 0, "cuda", [False])
