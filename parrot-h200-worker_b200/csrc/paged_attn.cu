@@ -769,7 +769,12 @@ int launch_decode_d(const PagedAttnArgs& a, cudaStream_t stream, int sms) {
 // 32 of 4 25 and 33, 8 of 8 15 and 17, 32 of 8 39 and 34.  Few rows over long contexts
 // get more warps here: one piece of 8 over 16,384 keys 18 and 39, 4 of 4 of a latent
 // 32 and 36.  Single tokens beside pieces go with the pieces (8 beside one of 256: 21
-// us, and 29 in two launches; 64 beside 512: 58, and 64 in two).
+// us, and 29 in two launches; 64 beside 512: 58, and 64 in two).  The mean stands for
+// uneven batches too, on either side of its limits (one piece among single tokens at
+// 4096; here, and there with two more tokens in the piece): 255 and 256 at 2048 111 us
+// and 153, 127 and 128 74 and 76, 31 and 32 21 and 27, of a latent 67 and 73; in 8 bits
+// 127 and 385 74 and 115, 31 and 96 24 and 43; only 127 and 385 of an 8-bit latent lose,
+// 118 and 100.
 bool paged_few_queries(const PagedAttnArgs& a, int sms) {
   const long long n = a.batch.tokens, batch = a.batch.batch, rows = n * a.heads;
   if (n <= 2 * batch) return true;

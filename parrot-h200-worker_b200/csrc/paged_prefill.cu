@@ -286,8 +286,8 @@ __device__ __forceinline__ uint32_t keep_mask(uint32_t bits, int i) {  // of pai
 // time, all of their remote loads on their way together.
 template <int D, bool F32, int K, int U, typename St>
 __device__ __forceinline__ void merge_rows(const PagedAttnArgs& a, St& st, const float* part,
-                                           const Tile& tile, const RowMap& map, int pos0, int rows, int kvh, int rank, int ranks, uint32_t live,
-                                           int threads) {
+                                           const Tile& tile, const RowMap& map, int pos0, int rows,
+                                           int kvh, int rank, int ranks, uint32_t live, int threads) {
   const int total = rows * (D / 4), stride = ranks * threads;
   for (int v0 = rank * threads + threadIdx.x; v0 < total; v0 += U * stride) {
     float mk[U][K], lk[U][K];
