@@ -434,8 +434,9 @@ __global__ void __launch_bounds__(32 * DecodeShape<D, E4M3, SEP, WIDE>::kWarps, 
           float most = fmaxf(most_w[i], __shfl_xor_sync(0xffffffffu, most_w[i], 1));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
           if (most > 0.f) {
-            // the power of two above it (at least 2^-100: its reciprocal is finite)
-            const float w = fmaxf(__uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u), pow2(-100));
+            // the power of two above it (at least 2^-112, so that 2^14 / W is finite: below
+            // every weight of p = 1)
+            const float w = fmaxf(__uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u), pow2(-112));
             // most >= corr W / 2^6, so the product is below 2^6 (W / w alone may be past fp32)
             corr[i] = corr[i] * top_w[i] * __uint_as_float((254u << 23) - __float_as_uint(w));
             top_w[i] = w;

@@ -97,7 +97,7 @@ def test_values_of_very_different_size(order, rise, context, queries, e4m3):
 
 @pytest.mark.parametrize("queries", [[1], [2], [100]])
 @pytest.mark.parametrize("first,later,rise", [(120, -100, 200.0), (-100, 120, -200.0), (-100, 120, 0.0),
-                                              (120, -100, 60.0)])
+                                              (120, -100, 60.0), (-102, -102, 10.0), (-102, -102, -10.0)])
 def test_values_at_both_ends_of_the_range(first, later, rise, queries):
     """Half of the context at one scale, half at the other, with a step of the scores between them."""
     context, dim = 700, 96
