@@ -285,6 +285,25 @@ def test_fp32_queries_and_an_infinite_latent_row(queries, context, at, bad):
     _assert_formula_f32(_call(cache, queries, q), cache, queries, q)
 
 
+@pytest.mark.parametrize("queries", [[1, 1, 1], [1, 200, 3]])
+def test_fp32_queries_in_a_graph_follow_the_lists(queries):
+    contexts = [900, 400, 64]
+    cache = Paged(contexts, kv_heads=1, dim=128, page=64, latent=True, seed=8)
+    kv, table, start, length = cache.device(), cache.table.cuda(), starts(queries).cuda(), ints(contexts)
+    q = torch.randn(sum(queries), 8, 128, device="cuda")
+    eager = bridge.b200_paged_attention(q, kv, table, start, length)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bridge.b200_paged_attention(q, kv, table, start, length)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, eager)
+    length.copy_(ints([500, 400, 20]))
+    graph.replay()
+    assert torch.equal(out, bridge.b200_paged_attention(q, kv, table, start, length)) and not torch.equal(out, eager)
+
+
 def test_fp32_queries_need_a_bf16_latent_cache():
     q = torch.zeros(1, 2, 96, device="cuda")
     for kw in (dict(latent=False), dict(latent=True, e4m3=True)):
